@@ -1,0 +1,345 @@
+// What makes microscaled numbers (mx.cuh), and what turns them back:
+//   alofa_mx_rows        rows [T, K] in bf16 or fp32 -> E4M3 codes [T, Kp], scales [T, Kp / 32]
+//   alofa_mx_norm        h = base + sum_z owed[z] (+ bias); the RMSNorm (or layer norm) of h's rows as such rows
+//   alofa_mx_gate        the sums of a gated product, one per part of its depth, as rows of silu(g) * u
+//   alofa_mx_pack        a weight [N, K] in bf16 or fp32 -> tiles of E2M1 codes and scales
+//   alofa_mx_rows_values, alofa_mx_weight_values   the numbers that rows, or a weight, stand for
+// Kp is K rounded up to whole groups of 128; the codes behind K are zeros.
+//
+// All of them are bound by memory: a lane takes eight neighbouring numbers (16 or 32 bytes of input, 8 of
+// rows or 4 of a weight), four lanes have a block and find its largest magnitude by two shuffles.
+#include "mx.cuh"
+
+template <typename T>
+__device__ __forceinline__ void load8(float (&v)[8], const T* src, int have, bool whole) {
+  if (whole && have >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      const uint4 p = *reinterpret_cast<const uint4*>(src);
+      const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    } else {
+      const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < have ? to_f(src[j]) : 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* dst, const float (&v)[8], int have, bool whole) {
+  if (whole && have >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      uint4 p;
+      __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+      __nv_bfloat162 c = __floats2bfloat162_rn(v[4], v[5]), d = __floats2bfloat162_rn(v[6], v[7]);
+      p.x = *reinterpret_cast<uint32_t*>(&a), p.y = *reinterpret_cast<uint32_t*>(&b);
+      p.z = *reinterpret_cast<uint32_t*>(&c), p.w = *reinterpret_cast<uint32_t*>(&d);
+      *reinterpret_cast<uint4*>(dst) = p;
+    } else {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < have) dst[j] = from_f<T>(v[j]);
+}
+
+static inline int padded(int k) { return (k + MX_GROUP - 1) / MX_GROUP * MX_GROUP; }
+static inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// ---------------------------------------------------------------------------
+// Rows
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) mx_rows_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, long long chunks, int k, int kp, bool whole) {
+  pdl_wait();
+  pdl_launch();
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;  // kp / 8 is a multiple of 16: four lanes with a block are in one row
+  const bool live = i < chunks;
+  const int per_row = kp >> 3;
+  const long long row = live ? i / per_row : 0;
+  const int c = live ? (int)(i - row * per_row) * 8 : 0;
+  float v[8];
+  load8(v, x + row * k + c, live ? k - c : 0, whole);
+  mx_put8(v, codes + row * kp + c, scales + row * (kp / MX_BLOCK) + c / MX_BLOCK, live);
+}
+
+ALOFA_API int alofa_mx_rows(void* codes, void* scales, const void* x, int t, int k, int bf16_x, void* stream) {
+  if (t < 0 || k <= 0 || k > (1 << 30) || !aligned(codes, 8)) return ALOFA_ERR_ARGUMENT;
+  if (t == 0) return ALOFA_OK;
+  const int kp = padded(k);
+  const long long chunks = (long long)t * (kp / 8), blocks = (chunks + 255) / 256;
+  if (blocks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  const bool whole = k % 8 == 0 && aligned(x, 16);
+  if (bf16_x)
+    launch_dep(mx_rows_kernel<bf16>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const bf16*)x, chunks, k, kp, whole);
+  else
+    launch_dep(mx_rows_kernel<float>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const float*)x, chunks, k, kp, whole);
+  return launch_status();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) mx_rows_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long chunks, int k, int kp, bool whole) {
+  pdl_wait();
+  pdl_launch();
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= chunks) return;
+  const int per_row = (k + 7) >> 3;
+  const long long row = i / per_row;
+  const int c = (int)(i - row * per_row) * 8;
+  const uint2 p = *reinterpret_cast<const uint2*>(codes + row * kp + c);
+  const float by = mx_power(scales[row * (kp / MX_BLOCK) + c / MX_BLOCK]);
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] = mx_from_e4m3((p.x >> (8 * j)) & 255u) * by;
+    v[4 + j] = mx_from_e4m3((p.y >> (8 * j)) & 255u) * by;
+  }
+  store8(out + row * k + c, v, k - c, whole);
+}
+
+ALOFA_API int alofa_mx_rows_values(void* out, const void* codes, const void* scales, int t, int k, int bf16_out, void* stream) {
+  if (t < 0 || k <= 0 || k > (1 << 30) || !aligned(codes, 8)) return ALOFA_ERR_ARGUMENT;
+  if (t == 0) return ALOFA_OK;
+  const long long chunks = (long long)t * ((k + 7) / 8), blocks = (chunks + 255) / 256;
+  if (blocks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  const bool whole = k % 8 == 0 && aligned(out, 16);
+  if (bf16_out)
+    launch_dep(mx_rows_values_kernel<bf16>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, chunks, k, padded(k), whole);
+  else
+    launch_dep(mx_rows_values_kernel<float>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (float*)out, (const uint8_t*)codes, (const uint8_t*)scales, chunks, k, padded(k), whole);
+  return launch_status();
+}
+
+// ---------------------------------------------------------------------------
+// The norm.  A block has a row; a thread keeps its CH chunks of eight numbers in registers, so the row is
+// read once; sums are taken in a fixed order.  Formula: src/alofa/kernels/cpu/scalar.mojo:93-129.
+// ---------------------------------------------------------------------------
+template <int CH>
+__global__ void mx_norm_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, float* __restrict__ h, const float* __restrict__ base, const float* __restrict__ owed, int splits,
+                               const float* __restrict__ bias, const float* __restrict__ w, const float* __restrict__ shift, int t, int k, int kp, float eps, bool whole) {
+  __shared__ float scratch[32];
+  pdl_wait();
+  const int row = blockIdx.x;
+  const size_t at = (size_t)row * k, plane = (size_t)t * k;
+  float v[CH][8];
+  float ss = 0.f, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = (threadIdx.x + i * blockDim.x) * 8, have = k - c;
+    load8(v[i], base + at + c, have, whole);
+  }
+  for (int z = 0; z < splits; ++z) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = (threadIdx.x + i * blockDim.x) * 8;
+      float p[8];
+      load8(p, owed + z * plane + at + c, k - c, whole);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] += p[j];
+    }
+  }
+  pdl_launch();
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = (threadIdx.x + i * blockDim.x) * 8, have = k - c;
+    if (bias) {
+      float p[8];
+      load8(p, bias + c, have, whole);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] += p[j];
+    }
+    if (owed || bias || h != base) store8(h + at + c, v[i], have, whole);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ss = fmaf(v[i][j], v[i][j], ss);
+      sum += v[i][j];
+    }
+  }
+  float mean = 0.f;
+  if (shift) {
+    mean = block_sum(sum, scratch) / (float)k;
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = (threadIdx.x + i * blockDim.x) * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = c + j < k ? v[i][j] - mean : 0.f;
+        ss = fmaf(d, d, ss);
+      }
+    }
+  }
+  ss = block_sum(ss, scratch);
+  const float scale = 1.0f / sqrtf(ss / (float)k + eps);
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = (threadIdx.x + i * blockDim.x) * 8, have = k - c;
+    float g[8], s[8];
+    load8(g, w + c, have, whole);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = 0.f;
+    if (shift) load8(s, shift + c, have, whole);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = c + j < k ? fmaf((v[i][j] - mean) * scale, g[j], s[j]) : 0.f;
+    mx_put8(v[i], codes + (size_t)row * kp + c, scales + (size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK, c < kp);
+  }
+}
+
+ALOFA_API int alofa_mx_norm(void* codes, void* scales, float* h, const float* base, const float* owed, int splits, const float* bias, const float* w, const float* shift, int t, int k, float eps,
+                            void* stream) {
+  if (t < 0 || k <= 0 || splits < 0 || !aligned(codes, 8)) return ALOFA_ERR_ARGUMENT;
+  if (t == 0) return ALOFA_OK;
+  const int kp = padded(k), chunks = kp / 8;
+  const int threads = chunks <= 128 ? 128 : chunks <= 2048 ? 256 : 512, per = (chunks + threads - 1) / threads;
+  if (per > 8) return ALOFA_ERR_ARGUMENT;
+  bool whole = k % 8 == 0 && aligned(h, 16) && aligned(base, 16) && aligned(owed, 16) && aligned(bias, 16) && aligned(w, 16) && aligned(shift, 16);
+  if (!splits) owed = nullptr;
+#define GO(CH) launch_dep(mx_norm_kernel<CH>, t, threads, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, h, base, owed, splits, bias, w, shift, t, k, kp, eps, whole)
+  if (per <= 1) GO(1);
+  else if (per <= 2) GO(2);
+  else if (per <= 4) GO(4);
+  else GO(8);
+#undef GO
+  return launch_status();
+}
+
+// ---------------------------------------------------------------------------
+// The gate: sums [splits, T, 2 F16] of a gated weight's rows (16 of the gate, the same 16 of the up
+// projection, and so on; F16 is F rounded up to 16), added in split order
+// (silu(gate) * up: src/alofa/kernels/cpu/scalar.mojo:208-231).
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) mx_gate_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const float* __restrict__ sums, int splits, int t, int f, int fp, float alpha, float limit) {
+  pdl_wait();
+  pdl_launch();
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const int per_row = fp >> 3, f16 = (f + 15) / 16 * 16;
+  const bool live = i < (long long)t * per_row;
+  const long long row = live ? i / per_row : 0;
+  const int c = live ? (int)(i - row * per_row) * 8 : 0;
+  float g[8], u[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) g[j] = u[j] = 0.f;
+  if (live && c < f16) {
+    const float* src = sums + row * (2 * f16) + mx_gated_row(c, 0);
+    const size_t plane = (size_t)t * 2 * f16;
+    for (int z = 0; z < splits; ++z) {
+      float a[8], b[8];
+      load8(a, src + z * plane, 8, true);
+      load8(b, src + z * plane + MX_GATE_ROWS, 8, true);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] += a[j], u[j] += b[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) g[j] = c + j < f ? fast_gate_times(g[j], u[j], alpha, limit) : 0.f;
+  mx_put8(g, codes + row * fp + c, scales + row * (fp / MX_BLOCK) + c / MX_BLOCK, live);
+}
+
+ALOFA_API int alofa_mx_gate(void* codes, void* scales, const float* sums, int splits, int t, int f, float alpha, float limit, void* stream) {
+  if (t < 0 || f <= 0 || f > (1 << 29) || splits < 1 || !aligned(codes, 8) || !aligned(sums, 16)) return ALOFA_ERR_ARGUMENT;
+  if (t == 0) return ALOFA_OK;
+  const int fp = padded(f);
+  const long long blocks = ((long long)t * (fp / 8) + 255) / 256;
+  if (blocks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  launch_dep(mx_gate_kernel, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, sums, splits, t, f, fp, alpha, limit);
+  return launch_status();
+}
+
+// ---------------------------------------------------------------------------
+// Weights: a block makes one tile of 128 rows and 128 numbers of each; a warp has two rows at a time, 256
+// bytes of bf16 from each.  `features` > 0: a gated weight whose row f is the gate's and features + f the up
+// projection's.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int weight_source_row(int r, int n, int features) {
+  if (!features) return r < n ? r : -1;
+  const int f = r / (2 * MX_GATE_ROWS) * MX_GATE_ROWS + r % MX_GATE_ROWS, half = r / MX_GATE_ROWS % 2;
+  return f < features ? half * features + f : -1;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) mx_pack_kernel(uint8_t* __restrict__ tiles, const T* __restrict__ w, int n, int k, int features, bool whole) {
+  uint8_t* tile = tiles + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * MX_TILE_BYTES;
+  const int c = (threadIdx.x & 15) * 8, kc = blockIdx.x * MX_GROUP + c;
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int src = weight_source_row(blockIdx.y * MX_TILE_ROWS + i * 16 + (threadIdx.x >> 4), n, features);
+    load8(v[i], w + (size_t)max(src, 0) * k + kc, src < 0 ? 0 : k - kc, whole);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 16 + (threadIdx.x >> 4);
+    const uint32_t s = mx_weight_scale(mx_largest4(v[i]));
+    const float over = mx_over(s);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] *= over;
+    *reinterpret_cast<uint32_t*>(tile + r * (MX_GROUP / 2) + c / 2) = s == 255u ? 0u : mx_e2m1(v[i]);
+    if ((threadIdx.x & 3) == 0) tile[MX_TILE_CODES + mx_scale_at(r, c / MX_BLOCK)] = (uint8_t)s;
+  }
+}
+
+// Products read a weight before the kernel ahead of them in the stream has ended (it is constant by then).  What
+// makes one therefore ends with this: an ordinary launch, which begins when the tiles are complete and visible, and
+// so does whatever may begin beside it.
+__global__ void mx_settle_kernel() {}
+
+ALOFA_API int alofa_mx_settle(void* stream) {
+  launch_whole(mx_settle_kernel, 1, 32, 0, (cudaStream_t)stream);
+  return launch_status();
+}
+
+// n: rows of the weight; gated: they are the gate's n / 2 and the up projection's.
+ALOFA_API int alofa_mx_pack(void* tiles, const void* w, int n, int k, int gated, int bf16_w, void* stream) {
+  if (n <= 0 || k <= 0 || k > (1 << 30) || (gated && n % 2) || !aligned(tiles, 16)) return ALOFA_ERR_ARGUMENT;
+  const long long rows = gated ? 2ll * ((n / 2 + 15) / 16 * 16) : n, tall = (rows + MX_TILE_ROWS - 1) / MX_TILE_ROWS;
+  if (tall > 65535) return ALOFA_ERR_ARGUMENT;
+  const dim3 grid((unsigned)(padded(k) / MX_GROUP), (unsigned)tall);
+  const bool whole = k % 8 == 0 && aligned(w, 16);
+  if (bf16_w)
+    launch_whole(mx_pack_kernel<bf16>, grid, 256, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const bf16*)w, n, k, gated ? n / 2 : 0, whole);
+  else
+    launch_whole(mx_pack_kernel<float>, grid, 256, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const float*)w, n, k, gated ? n / 2 : 0, whole);
+  const int rc = launch_status();
+  return rc ? rc : alofa_mx_settle(stream);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) mx_weight_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ tiles, int n, int k, int features, bool whole) {
+  const uint8_t* tile = tiles + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * MX_TILE_BYTES;
+  const int c = (threadIdx.x & 15) * 8, kc = blockIdx.x * MX_GROUP + c;
+  pdl_wait();
+  pdl_launch();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 16 + (threadIdx.x >> 4), src = weight_source_row(blockIdx.y * MX_TILE_ROWS + r, n, features);
+    if (src < 0 || kc >= k) continue;
+    const uint32_t p = *reinterpret_cast<const uint32_t*>(tile + r * (MX_GROUP / 2) + c / 2);
+    const float by = mx_power(tile[MX_TILE_CODES + mx_scale_at(r, c / MX_BLOCK)]);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = mx_from_e2m1((p >> (4 * j)) & 15u) * by;
+    store8(out + (size_t)src * k + kc, v, k - kc, whole);
+  }
+}
+
+ALOFA_API int alofa_mx_weight_values(void* out, const void* tiles, int n, int k, int gated, int bf16_out, void* stream) {
+  if (n <= 0 || k <= 0 || k > (1 << 30) || (gated && n % 2) || !aligned(tiles, 16)) return ALOFA_ERR_ARGUMENT;
+  const long long rows = gated ? 2ll * ((n / 2 + 15) / 16 * 16) : n, tall = (rows + MX_TILE_ROWS - 1) / MX_TILE_ROWS;
+  if (tall > 65535) return ALOFA_ERR_ARGUMENT;
+  const dim3 grid((unsigned)(padded(k) / MX_GROUP), (unsigned)tall);
+  const bool whole = k % 8 == 0 && aligned(out, 16);
+  if (bf16_out)
+    launch_dep(mx_weight_values_kernel<bf16>, grid, 256, 0, (cudaStream_t)stream, (bf16*)out, (const uint8_t*)tiles, n, k, gated ? n / 2 : 0, whole);
+  else
+    launch_dep(mx_weight_values_kernel<float>, grid, 256, 0, (cudaStream_t)stream, (float*)out, (const uint8_t*)tiles, n, k, gated ? n / 2 : 0, whole);
+  return launch_status();
+}

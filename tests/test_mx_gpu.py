@@ -1,0 +1,271 @@
+"""Microscaled weights and rows on the GPU, against their definition in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import plain_mx as plain
+from alofa_b200 import mx
+from alofa_b200.csrc import ops
+from alofa_b200.errors import AlofaError
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+ROWS_SLACK = 2.0**-18  # what fp32 sums of a few thousand numbers and the hardware's exponential leave in a normed or gated number
+
+
+def numbers(t, k, seed, dtype=F32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(t, k, generator=g) * torch.exp(2 * torch.randn(t, 1, generator=g)) * scale
+    x[:, ::37] *= 30
+    return x.to(dtype)
+
+
+def host(t):
+    return t.cpu().numpy()
+
+
+def unpack(tiles, n, k, gated):
+    """Codes and scales of a weight's tiles, by rows of the product."""
+    tall, slices, _ = tiles.shape
+    raw = host(tiles)
+    c = raw[:, :, :8192].reshape(tall, slices, 128, 64).transpose(0, 2, 1, 3).reshape(tall * 128, -1)
+    codes = np.stack([c & 15, c >> 4], -1).reshape(tall * 128, -1)
+    s = raw[:, :, 8192:].reshape(tall, slices, 32, 4, 4).transpose(0, 3, 2, 1, 4).reshape(tall * 128, -1)
+    if gated:
+        f = np.arange(n // 2)
+        at = f // 16 * 32 + f % 16
+        at = np.concatenate([at, at + 16])
+    else:
+        at = np.arange(n)
+    rest = np.setdiff1d(np.arange(tall * 128), at)
+    return codes[at], s[at], codes[rest]
+
+
+# ---- rows ------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,k", [(1, 1), (1, 32), (3, 33), (2, 127), (5, 128), (7, 896), (1, 1000), (33, 1537), (300, 264)])
+def test_rows_are_the_nearest_codes(t, k, dtype):
+    x = numbers(t, k, 1, dtype)
+    rows = mx.quantize_rows(x.cuda())
+    codes, scales = plain.encode(x, False)
+    assert np.array_equal(host(rows.scales), scales) and np.array_equal(host(rows.codes), codes)
+    want = plain.decode(codes, scales, k, False)
+    assert np.array_equal(host(rows.dequantize(F32)), want)
+    assert np.array_equal(host(rows.dequantize().float()), want)  # four digits: bfloat16 has them all
+
+
+def test_rows_ties_borders_and_the_smallest_numbers():
+    steps = np.concatenate([plain.E4M3, (plain.E4M3[1:] + plain.E4M3[:-1]) / 2])  # every code and every tie
+    x = np.zeros((12, 32 * 12), np.float32)
+    for r, power in enumerate([-140, -133, -127, -120, -60, -1, 0, 1, 50, 100, 110, 118]):
+        block = np.concatenate([steps[:240], -steps[:144]])
+        x[r] = block * 2.0**power
+        x[r, ::32] = 448 * 2.0**power  # the block's largest: its scale is 2^power
+    x[6, 0::32] = np.float32(448.0)
+    x[6, 32] = np.nextafter(np.float32(448.0), np.float32(500))  # one step over: the next scale
+    rows = mx.quantize_rows(torch.from_numpy(x).cuda())
+    codes, scales = plain.encode(x, False)
+    assert np.array_equal(host(rows.scales), scales) and np.array_equal(host(rows.codes), codes)
+
+
+def test_rows_of_zeros_infinities_and_nan():
+    x = torch.randn(4, 160)
+    x[0] = 0
+    x[1, 5], x[1, 40], x[2, 159], x[3, 64] = float("inf"), float("nan"), float("-inf"), 3.0e38
+    rows = mx.quantize_rows(x.cuda())
+    codes, scales = plain.encode(x, False)
+    assert np.array_equal(host(rows.scales), scales) and np.array_equal(host(rows.codes), codes)
+    got = host(rows.dequantize(F32))
+    assert np.isnan(got[1, :64]).all() and np.isfinite(got[1, 64:]).all() and np.isnan(got[2, 128:]).all() and np.isfinite(got[3]).all() and (got[0] == 0).all()
+
+
+def test_rows_over_memory_off_its_alignment():
+    base = torch.randn(3 * 64 + 1).cuda()
+    x = base[1:].view(3, 64)  # 4 bytes off
+    codes, scales = plain.encode(x, False)
+    rows = mx.quantize_rows(x)
+    assert np.array_equal(host(rows.codes), codes) and np.array_equal(host(rows.scales), scales)
+
+
+# ---- weights ---------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n,k,gated", [(1, 1, False), (128, 128, False), (130, 257, False), (2, 32, True), (66, 100, True), (1152, 896, False), (512, 1000, True)])
+def test_weights_are_the_nearest_codes(n, k, gated, dtype):
+    w = numbers(n, k, 2, dtype, 0.02)
+    packed = mx.pack_weight(w.cuda(), gated)
+    codes, scales = plain.encode(w, True)
+    got_codes, got_scales, rest = unpack(packed.tiles, n, k, gated)
+    assert np.array_equal(got_codes, codes) and np.array_equal(got_scales, scales) and not rest.any()
+    want = plain.decode(codes, scales, k, True)
+    assert np.array_equal(host(packed.dequantize(F32)), want) and np.array_equal(host(packed.dequantize().float()), want)
+
+
+def test_weights_ties_and_what_is_clipped():
+    v = np.array([0, 0.25, 0.26, 0.5, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 5.01, 6, 6.5, 7.99, -0.25, -0.75, -5, -7, 4, 1, 2, 3] + [0.1] * 10, np.float32)
+    w = np.stack([v, v * 2.0**-20, v * 2.0**100, v * 2.0**-128])
+    packed = mx.pack_weight(torch.from_numpy(w.astype(np.float32)).cuda())
+    codes, scales = plain.encode(w.astype(np.float32), True)
+    got_codes, got_scales, _ = unpack(packed.tiles, 4, 32, False)
+    assert np.array_equal(got_codes, codes) and np.array_equal(got_scales, scales)
+
+
+@pytest.mark.parametrize("n,k,gated", [(130, 257, False), (66, 100, True), (256, 256, True)])
+def test_a_weight_from_codes_is_the_weight_packed(n, k, gated):
+    w = numbers(n, k, 3, F32, 0.02)
+    codes, scales = plain.encode(w, True)
+    dirty = codes.copy()
+    dirty[:, k:] = 5  # behind the depth: not read
+    made = mx.MxWeight.from_codes(torch.from_numpy(plain.nibbles(dirty)).cuda(), torch.from_numpy(scales.astype(np.uint8)).cuda(), k, gated)
+    assert torch.equal(made.tiles, mx.pack_weight(w.cuda(), gated).tiles)
+
+
+# ---- the norm --------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t,k,planes,bias,layer", [(1, 896, 4, False, False), (3, 100, 0, True, False), (5, 1537, 2, True, True), (37, 1536, 1, False, False), (2, 9000, 3, False, True), (300, 64, 8, True, False), (1, 1, 0, False, False)])
+def test_norm_rows(t, k, planes, bias, layer):
+    base, weight = numbers(t, k, 4), 1 + 0.1 * torch.randn(k)
+    owed = torch.randn(planes, t, k) if planes else None
+    b, shift = torch.randn(k) if bias else None, torch.randn(k) if layer else None
+    dev = lambda v: None if v is None else v.cuda()  # noqa: E731
+    h = base.cuda()
+    rows = mx.norm_rows(h, dev(weight), 1e-6, owed=dev(owed), bias=dev(b), shift=dev(shift))
+    want_h = base.double() + (owed.double().sum(0) if planes else 0) + (b.double() if bias else 0)
+    size = base.abs().double() + (owed.abs().double().sum(0) if planes else 0) + (b.abs().double() if bias else 0)
+    assert ((h.cpu().double() - want_h).abs() <= (planes + 1) * 2.0**-24 * size).all()  # a rounding an addition
+    y = plain.norm(h.cpu().double().numpy(), weight.double().numpy(), 1e-6, None if shift is None else shift.double().numpy())
+    if layer and k > 1:  # a difference from the mean, and a sum with the shift, may cancel: their roundings count by what went in
+        spread = np.abs(y) + np.abs(shift.double().numpy()) + 1
+        got = host(rows.dequantize(F32)).astype(np.float64)
+        unit = np.exp2(host(rows.scales).astype(np.float64) - 127).repeat(32, -1)[:, :k]
+        step = unit * np.exp2(np.maximum(np.frexp(np.maximum(np.abs(got), np.abs(y)) / unit)[1] - 1, -6) - 3.0)
+        assert (np.abs(got - y) <= step / 2 + ROWS_SLACK * spread).all()
+    else:
+        assert plain.near(host(rows.codes), host(rows.scales), y, ROWS_SLACK)
+    # into another tensor, the base left as it is
+    base_dev, h2 = base.cuda(), torch.full((t, k), float("nan"), device="cuda")
+    again = mx.norm_rows(h2, dev(weight), 1e-6, base=base_dev, owed=dev(owed), bias=dev(b), shift=dev(shift))
+    assert torch.equal(h2, h) and torch.equal(again.codes, rows.codes) and torch.equal(again.scales, rows.scales) and torch.equal(base_dev.cpu(), base)
+
+
+# ---- the product -----------------------------------------------------------------------------------------------------
+
+
+def product_operands(t, n, k, seed, gated=False):
+    x, w = numbers(t, k, seed), numbers(n, k, seed + 1, F32, 0.05)
+    xr, wp = mx.quantize_rows(x.cuda()), mx.pack_weight(w.cuda(), gated)
+    return xr, wp, plain.values(x), plain.values(w, True)
+
+
+def sum_bound(xv, wv):
+    """Each of a sum's additions may lose a step of fp32 at most (a truncating adder), of no more than the sum of sizes."""
+    k = xv.shape[1]
+    return (k + 8) * 2.0**-23 * (np.abs(xv) @ np.abs(wv).T)
+
+
+@pytest.mark.parametrize("t,n,k", [(1, 128, 128), (1, 1, 1), (3, 130, 257), (16, 128, 1024), (17, 300, 384), (33, 1152, 896), (64, 64, 2048), (65, 129, 640), (128, 256, 896), (200, 515, 1000), (257, 384, 512), (515, 200, 96)])
+def test_linear(t, n, k):
+    xr, wp, xv, wv = product_operands(t, n, k, 10)
+    want, loose = xv @ wv.T, sum_bound(xv, wv)
+    got = mx.linear(xr, wp, dtype=F32)
+    assert got.shape == (t, n) and (np.abs(host(got) - want) <= loose).all()
+    bias, add = torch.randn(n), torch.randn(t, n)
+    got = mx.linear(xr, wp, bias=bias.cuda())
+    assert got.dtype == BF16
+    full = want + bias.double().numpy()
+    assert (np.abs(host(got.float()) - full) <= loose * 1.01 + 2.0**-8 * np.abs(full) + 2.0**-22 * np.abs(bias.numpy())).all()
+    h = add.cuda()
+    got = mx.linear(xr, wp, bias=bias.cuda(), add=h, out=h)
+    full += add.double().numpy()
+    assert got is h and (np.abs(host(h) - full) <= loose + 2.0**-22 * (np.abs(want) + np.abs(bias.numpy()) + np.abs(add.numpy()))).all()
+
+
+@pytest.mark.parametrize("bn", mx.TOKEN_TILES)
+@pytest.mark.parametrize("asked", [1, 2, 3, 5, 100])
+def test_every_tile_and_part(bn, asked):
+    t, n, k = 70, 200, 1100
+    xr, wp, xv, wv = product_operands(t, n, k, 20)
+    splits = ops.mx_splits(k, asked)
+    partial = torch.full((splits, t, n), float("nan"), device="cuda")
+    out = torch.empty(t, n, device="cuda")
+    ops.mx_gemm(out, xr.codes, xr.scales, wp.tiles, n, k, bn, splits, partial)
+    assert (np.abs(host(out) - xv @ wv.T) <= sum_bound(xv, wv)).all()
+    ops.mx_gemm(None, xr.codes, xr.scales, wp.tiles, n, k, bn, splits, partial, leave=True)
+    assert (np.abs(host(partial).astype(np.float64).sum(0) - xv @ wv.T) <= sum_bound(xv, wv)).all()
+
+
+def test_every_pair_of_codes():
+    """Row t holds E4M3's code t in place t, feature f all of E2M1's codes in turn: each product stands alone in its sum."""
+    codes = torch.zeros(254, 256, dtype=torch.uint8)
+    every = torch.tensor([c for c in range(256) if c & 127 != 127], dtype=torch.uint8)
+    codes[torch.arange(254), torch.arange(254)] = every
+    scales = torch.full((254, 8), 127, dtype=torch.uint8)
+    w = ((torch.arange(256)[None, :] + torch.arange(16)[:, None]) % 16).numpy()
+    wp = mx.MxWeight.from_codes(torch.from_numpy(plain.nibbles(w)).cuda(), torch.full((16, 8), 127, dtype=torch.uint8).cuda(), 256)
+    got = mx.linear(mx.MxRows(codes.cuda(), scales.cuda(), 256), wp, dtype=F32)
+    want = plain.decode(codes, scales, 256, False) @ plain.decode(w, np.full((16, 8), 127), 256, True).T
+    assert np.array_equal(host(got), want)
+
+
+def test_scales_over_their_whole_range():
+    """One number a block, scales from both ends: the product of the two powers is taken without a rounding."""
+    codes = torch.zeros(20, 128, dtype=torch.uint8)
+    codes[:, 0] = 0x38  # 1
+    scales = torch.zeros(20, 4, dtype=torch.uint8)
+    scales[:, 0] = torch.tensor([0, 1, 2, 30, 60, 90, 100, 110, 120, 126, 127, 128, 130, 140, 160, 180, 200, 220, 240, 250])
+    ws = torch.zeros(20, 4, dtype=torch.uint8)
+    ws[:, 0] = torch.tensor([127, 126, 128, 100, 200, 247, 1, 3, 10, 20, 30, 40, 50, 60, 70, 80, 90, 110, 140, 254])
+    wc = np.zeros((20, 128), np.int64)
+    wc[:, 0] = 2  # 1
+    wp = mx.MxWeight.from_codes(torch.from_numpy(plain.nibbles(wc)).cuda(), ws.cuda(), 128)
+    got = host(mx.linear(mx.MxRows(codes.cuda(), scales.cuda(), 128), wp, dtype=F32)).astype(np.float64)
+    want = np.exp2(scales[:, :1].double().numpy() + ws[:, 0].double().numpy() - 254)
+    normal = (want >= 2.0**-126) & (want < 2.0**128)
+    assert np.array_equal(got[normal], want[normal])
+
+
+def test_a_block_of_nan_reaches_its_row_only():
+    xr, wp, xv, wv = product_operands(5, 140, 300, 30)
+    xr.scales[2, 1] = 255
+    got = host(mx.linear(xr, wp, dtype=F32))
+    assert np.isnan(got[2]).all() and np.isfinite(got[[0, 1, 3, 4]]).all()
+
+
+def test_rows_behind_the_last_are_left_alone():
+    xr, wp, xv, wv = product_operands(5, 140, 300, 31)
+    room = torch.full((20, 140), 7.0, device="cuda")
+    mx.linear(xr, wp, out=room[:5])
+    assert (room[5:] == 7).all() and (np.abs(host(room[:5]) - xv @ wv.T) <= sum_bound(xv, wv)).all()
+
+
+@pytest.mark.parametrize("t,f,k", [(1, 16, 128), (3, 33, 100), (16, 4864, 896), (70, 200, 384), (300, 260, 256)])
+@pytest.mark.parametrize("gate", [ops.SILU_GATE, (1.702, 7.0)])
+def test_gated_linear(t, f, k, gate):
+    xr, wp, xv, wv = product_operands(t, 2 * f, k, 40, gated=True)
+    rows = mx.gated_linear(xr, wp, gate)
+    g, u = xv @ wv[:f].T, xv @ wv[f:].T
+    eg, eu = sum_bound(xv, wv[:f]), sum_bound(xv, wv[f:])
+    if gate == ops.SILU_GATE:
+        want, slope = plain.silu(g) * u, 1.1 * np.abs(u) * eg + (np.abs(g) + eg) * eu
+    else:
+        a, top = gate
+        g, u = np.minimum(g, top), np.clip(u, -top, top)
+        want, slope = g / (1 + np.exp(-a * g)) * (u + 1), 1.1 * (np.abs(u) + 1) * eg + (np.abs(g) + eg) * eu
+    got = host(rows.dequantize(F32)).astype(np.float64)
+    assert rows.shape == (t, f) and not host(rows.codes)[:, f:].any()
+    unit = np.exp2(host(rows.scales).astype(np.float64) - 127).repeat(32, -1)[:, :f]
+    step = unit * np.exp2(np.maximum(np.frexp(np.maximum(np.abs(got), np.abs(want)) / unit)[1] - 1, -6) - 3.0)
+    assert (np.abs(got - want) <= step / 2 + slope + ROWS_SLACK * np.abs(want)).all()
+    # the scales are those of the numbers' own sizes
+    full = np.zeros((t, plain.padded(f)))
+    full[:, :f] = want
+    pad = np.zeros_like(full)
+    pad[:, :f] = slope + ROWS_SLACK * np.abs(want)
+    sizes, room = np.abs(full).reshape(t, -1, 32), pad.reshape(t, -1, 32)
+    scales = host(rows.scales)
+    assert (scales >= plain.scale_bytes(np.maximum(sizes - room, 0).max(-1), False)).all() and (scales <= plain.scale_bytes((sizes + room).max(-1), False)).all()
