@@ -19,6 +19,8 @@
 #include "tcgen05.cuh"
 #include "tma.cuh"
 
+#include <atomic>
+
 constexpr int MX_THREADS = 192;  // warps 0-3 weights, then the epilogue; warp 4 tokens; warp 5 products
 
 struct MxArgs {
@@ -255,11 +257,23 @@ static bool make_rows_map(CUtensorMap* map, const void* base, uint64_t rows, uin
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A kernel's shared memory is asked for once a device (a bit of `done` each; asking takes as long as a launch).
+static bool allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+template <int BN> static std::atomic<uint64_t> configured{0};
+
 template <int BN>
 static int launch_mx(const CUtensorMap& map, const MxArgs& args, int splits, cudaStream_t stream) {
   const long long tall = ((long long)args.N + MX_TILE_ROWS - 1) / MX_TILE_ROWS, wide = ((long long)args.T + BN - 1) / BN;
   if (tall > 0x7fffffffll || wide > 65535 || splits > 65535) return ALOFA_ERR_ARGUMENT;
-  if (cudaFuncSetAttribute((const void*)mx_gemm_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MxTile<BN>::SMEM) != cudaSuccess) return ALOFA_ERR_LAUNCH;
+  if (!allow_shared((const void*)mx_gemm_kernel<BN>, (int)MxTile<BN>::SMEM, configured<BN>)) return ALOFA_ERR_LAUNCH;
   launch_dep(mx_gemm_kernel<BN>, dim3((unsigned)tall, (unsigned)wide, (unsigned)splits), MX_THREADS, MxTile<BN>::SMEM, stream, map, args);
   return launch_status();
 }

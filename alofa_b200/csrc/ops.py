@@ -1599,7 +1599,8 @@ def decode_stack(table, n_layers: int, ctas: int, sizes: tuple, page: int, scale
     count_launches(-(-n_layers // DECODE_STACK_LAYERS) - 1)
 
 
-def _mx():
+def mx_library():
+    """The library of the microscaled operators (:mod:`alofa_b200.mx` is its Python face)."""
     lib = _libs.get("mx")
     if lib is None:
         lib = load_library("alofa_mx", ["kernels/mx_rows.cu", "kernels/mx_gemm.cu"])
@@ -1622,125 +1623,14 @@ def _mx():
     return lib
 
 
-MX_BLOCK, MX_GROUP, MX_TILE_ROWS, MX_TILE_BYTES, MX_GATE_ROWS = 32, 128, 128, 8704, 16  # as in kernels/mx.cuh
-MX_MOST_WIDTH = 32768  # numbers of a row that the norm takes
+def mx_launched(rc: int, launches: int, what: str, detail) -> None:
+    """Counts what an operator launched, or raises its error; ``detail()`` says what sizes it had."""
+    global _launches
+    if rc:
+        _done(rc, what, detail())
+    _launches += launches
 
 
-def mx_padded(k: int) -> int:
-    """A depth rounded up to whole groups: the width of rows in 8 bits."""
-    return -(-k // MX_GROUP) * MX_GROUP
-
-
-def mx_weight_rows(n: int, gated: bool) -> int:
-    """Rows of a product with a weight of ``n`` rows: of a gated one the gate's and the up projection's features in turns of 16."""
-    return 2 * (-(-(n // 2) // MX_GATE_ROWS) * MX_GATE_ROWS) if gated else n
-
-
-def _mx_rows(codes, scales, t: int, k: int, what: str) -> tuple:
-    kp = mx_padded(k)
-    if tuple(codes.shape) != (t, kp) or tuple(scales.shape) != (t, kp // MX_BLOCK):
-        raise AlofaError("invalid_argument", f"{what}: rows in 8 bits have the wrong size", f"codes={tuple(codes.shape)} scales={tuple(scales.shape)} rows={t} depth={k}")
-    return _dev(codes, "codes", torch.uint8), _dev(scales, "scales", torch.uint8)
-
-
-def _mx_tiles(tiles, n: int, k: int, gated: bool, what: str) -> int:
-    want = (-(-mx_weight_rows(n, gated) // MX_TILE_ROWS), mx_padded(k) // MX_GROUP, MX_TILE_BYTES)
-    if tuple(tiles.shape) != want:
-        raise AlofaError("invalid_argument", f"{what}: a weight's tiles have the wrong size", f"tiles={tuple(tiles.shape)} want={want}")
-    return _dev(tiles, "tiles", torch.uint8)
-
-
-def mx_rows(codes, scales, x) -> None:
-    """Rows ``x [T, K]`` (bfloat16 or float32) in 8 bits: ``codes [T, Kp]``
-    (E4M3) and ``scales [T, Kp / 32]``, Kp being K in whole groups of 128."""
-    t, k = x.shape
-    c, s = _mx_rows(codes, scales, t, k, "mx_rows")
-    _done(_mx().alofa_mx_rows(c, s, _dev(x, "x"), t, k, _is_bf16(x, "x"), _stream()), "mx_rows", f"rows={t} depth={k}")
-
-
-def mx_rows_values(out, codes, scales) -> None:
-    """The numbers that rows in 8 bits stand for."""
-    t, k = out.shape
-    c, s = _mx_rows(codes, scales, t, k, "mx_rows_values")
-    _done(_mx().alofa_mx_rows_values(_dev(out, "out"), c, s, t, k, _is_bf16(out, "out"), _stream()), "mx_rows_values", f"rows={t} depth={k}")
-
-
-def mx_norm(codes, scales, h, weight, eps: float, base=None, owed=None, bias=None, shift=None) -> None:
-    """``h = base (h itself unless given) + sum_z owed[z] + bias`` in fp32, and
-    the RMSNorm of its rows in 8 bits; with ``shift`` the layer norm.  ``owed
-    [splits, T, K]``: the sums a product left for parts of its depth."""
-    t, k = h.shape
-    c, s = _mx_rows(codes, scales, t, k, "mx_norm")
-    f32 = torch.float32
-    if weight.shape != (k,) or any(v is not None and v.shape != (k,) for v in (bias, shift)) or (base is not None and base.shape != h.shape) or (owed is not None and (owed.dim() != 3 or owed.shape[1:] != h.shape)):
-        raise AlofaError("invalid_argument", "mx_norm sizes disagree", f"h={tuple(h.shape)} weight={tuple(weight.shape)} owed={None if owed is None else tuple(owed.shape)}")
-    _done(
-        _mx().alofa_mx_norm(
-            c, s, _dev(h, "h", f32), _dev(base if base is not None else h, "base", f32), _dev(owed, "owed", f32) if owed is not None else None, 0 if owed is None else owed.shape[0],
-            _dev(bias, "bias", f32) if bias is not None else None, _dev(weight, "weight", f32), _dev(shift, "shift", f32) if shift is not None else None, t, k, float(eps), _stream(),
-        ),
-        "mx_norm", f"rows={t} width={k}",
-    )
-
-
-def mx_gate(codes, scales, sums, features: int, gate=SILU_GATE) -> None:
-    """Rows of ``silu(g) * u`` (or the clamped form, see :func:`gemm_generic`)
-    in 8 bits from the sums ``[splits, T, rows]`` of a gated weight."""
-    splits, t, rows = sums.shape
-    c, s = _mx_rows(codes, scales, t, features, "mx_gate")
-    if rows != mx_weight_rows(2 * features, True):
-        raise AlofaError("invalid_argument", "mx_gate sizes disagree", f"sums={tuple(sums.shape)} features={features}")
-    _done(_mx().alofa_mx_gate(c, s, _dev(sums, "sums", torch.float32), splits, t, features, float(gate[0]), float(gate[1]), _stream()), "mx_gate", f"rows={t} features={features}")
-
-
-def mx_pack(tiles, w, gated: bool = False) -> None:
-    """A weight ``w [N, K]`` (bfloat16 or float32) in 4 bits, laid out for the
-    product; ``gated``: the gate's N / 2 rows, then the up projection's."""
-    n, k = w.shape
-    at = _mx_tiles(tiles, n, k, gated, "mx_pack")
-    _done(_mx().alofa_mx_pack(at, _dev(w, "w"), n, k, int(gated), _is_bf16(w, "w"), _stream()), "mx_pack", f"rows={n} depth={k}")
-    count_launches(1)
-
-
-def mx_settle() -> None:
-    """To be called behind kernels that wrote a weight's tiles in another way
-    than :func:`mx_pack`: the product reads tiles ahead of the kernel before it."""
-    _done(_mx().alofa_mx_settle(_stream()), "mx_settle")
-
-
-def mx_weight_values(out, tiles, gated: bool = False) -> None:
-    """The numbers that a weight's tiles stand for."""
-    n, k = out.shape
-    at = _mx_tiles(tiles, n, k, gated, "mx_weight_values")
-    _done(_mx().alofa_mx_weight_values(_dev(out, "out"), at, n, k, int(gated), _is_bf16(out, "out"), _stream()), "mx_weight_values", f"rows={n} depth={k}")
-
-
-def mx_splits(k: int, splits: int) -> int:
-    """The number of parts that a depth of ``k`` really goes in."""
-    return _mx().alofa_mx_splits(k, splits)
-
-
-def mx_gemm(out, codes, scales, tiles, n: int, k: int, bn: int, splits: int = 1, partial=None, leave: bool = False, bias=None, add=None, gated: bool = False, status=None) -> None:
-    """Rows in 8 bits times a weight in 4: ``out = x w^T (+ bias) (+ add)``,
-    bfloat16 or float32.  ``bn`` tokens a tile (16, 32, 64, 128, 256).
-    ``splits`` parts of the depth (:func:`mx_splits`) go through ``partial
-    [splits, T, N]``; with ``leave`` they stay there for their reader to add
-    and ``out`` is not written.  A ``gated`` weight's rows come in turns of 16."""
-    t = codes.shape[0]
-    c, s = _mx_rows(codes, scales, t, k, "mx_gemm")
-    at = _mx_tiles(tiles, n, k, gated, "mx_gemm")
-    rows, f32 = mx_weight_rows(n, gated), torch.float32
-    if (out is None) != leave or (out is not None and tuple(out.shape) != (t, rows)) or (bias is not None and tuple(bias.shape) != (rows,)) or (add is not None and tuple(add.shape) != (t, rows)):
-        raise AlofaError("invalid_argument", "mx_gemm sizes disagree", f"tokens={t} rows={rows} out={None if out is None else tuple(out.shape)}")
-    if (splits > 1 or leave) and (partial is None or tuple(partial.shape) != (splits, t, rows)):
-        raise AlofaError("invalid_argument", "mx_gemm: split sums need [splits, tokens, rows]", f"partial={None if partial is None else tuple(partial.shape)} splits={splits}")
-    _done(
-        _mx().alofa_mx_gemm(
-            _dev(out, "out") if out is not None else None, _dev(partial, "partial", f32) if partial is not None else None, c, s, at, _dev(bias, "bias", f32) if bias is not None else None,
-            _dev(add, "add", f32) if add is not None else None, t, rows, k, bn, splits, int(leave), _is_bf16(out, "out") if out is not None else 0,
-            _dev(status, "status", torch.int32) if status is not None else None, _stream(),
-        ),
-        "mx_gemm", f"tokens={t} rows={rows} depth={k} bn={bn} splits={splits}",
-    )
-    if splits > 1 and not leave:
-        count_launches(1)
+def current_stream_handle(device: int) -> int:
+    """The handle of the device's current stream (the step's, inside a step), without the object around it that takes longer to make than a launch."""
+    return _bound_stream if _bound_stream is not None else torch._C._cuda_getCurrentRawStream(device)

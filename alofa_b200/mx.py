@@ -14,11 +14,14 @@ round to nearest, ties to the even code.  A weight so takes 4.25 bits a number.
 through a gate and an up projection (``pack_weight(..., gated=True)``) and gives
 rows again.  Everything runs on the current stream of the device that the
 tensors are on, which has to be the current one; what is returned belongs to
-that stream.  The engine uses these operators where it is given
-``weight_format="mxfp4"``."""
+that stream.  Operands are contiguous.  The engine uses these operators where it
+is given ``weight_format="mxfp4"``.
+
+A call of the smallest sizes is a few microseconds of launching and checking
+beside as much of the GPU's time: operands are checked once each, in one pass
+over what a launch goes by, and rows are one allocation."""
 from __future__ import annotations
 
-from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -26,132 +29,196 @@ import torch
 from .csrc import ops
 from .errors import AlofaError
 
-TOKEN_TILES = (16, 32, 64, 128, 256)  # tokens a CTA of the product may take
+BLOCK, GROUP, TILE_ROWS, TILE_BYTES, GATE_ROWS = 32, 128, 128, 8704, 16  # as in kernels/mx.cuh
+TOKEN_TILES = (16, 32, 64, 128, 256)  # tokens that a CTA of the product may take
+MOST_WIDTH = 32768  # numbers of a row that the norm takes
+
+_BF16, _F32, _U8, _I32 = torch.bfloat16, torch.float32, torch.uint8, torch.int32
 
 
-def _check(t, name: str, dims: int, dtypes: tuple) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dim() != dims or t.dtype not in dtypes:
-        got = f"{t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise AlofaError("invalid_argument", f"{name} must be a tensor of {dims} dimensions", f"got {got}, want one of {[str(d) for d in dtypes]}")
+def _refuse(t, name: str, want: str, here: int):
+    if not isinstance(t, torch.Tensor):
+        raise AlofaError("invalid_argument", f"{name} must be a tensor", f"got {type(t).__name__}")
     if not t.is_cuda:
         raise AlofaError("unsupported", "kernels run on CUDA tensors only", f"{name} is on {t.device}")
-    if t.device.index != torch.cuda.current_device():
-        raise AlofaError("invalid_argument", "kernels run on the current device only", f"{name} is on {t.device}, current is {torch.cuda.current_device()}")
+    if t.get_device() != here:
+        raise AlofaError("invalid_argument", "kernels run on the current device only", f"{name} is on {t.device}, current is {here}")
     if not t.is_contiguous():
         raise AlofaError("invalid_argument", "kernel operand must be contiguous", name)
-    return t
+    raise AlofaError("invalid_argument", "kernel operand has the wrong type or size", f"{name} is {t.dtype} {tuple(t.shape)}, want {want}")
 
 
-_NUMBERS, _F32, _BYTES = (torch.bfloat16, torch.float32), (torch.float32,), (torch.uint8,)
+def _at(t, name: str, dtype, shape, here: int) -> int:
+    """The address of an operand of this type and shape on the current device."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != here or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        _refuse(t, name, f"{dtype} {tuple(shape)}", here)
+    return t.data_ptr()
 
 
-@dataclass
+def _matrix(t, name: str, here: int) -> tuple:
+    """(address, rows, columns, whether bfloat16) of a matrix in one of the compute types."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.get_device() != here or not t.is_contiguous() or (t.dtype is not _BF16 and t.dtype is not _F32):
+        _refuse(t, name, "bfloat16 or float32 of two dimensions", here)
+    rows, columns = t.shape
+    return t.data_ptr(), rows, columns, t.dtype is _BF16
+
+
+def _here() -> int:
+    try:
+        return torch.cuda.current_device()
+    except (RuntimeError, AssertionError) as err:
+        raise AlofaError("unsupported", "kernels run on CUDA tensors only", str(err)) from err
+
+
+_stream = ops.current_stream_handle
+
+
+def padded(k: int) -> int:
+    """A depth rounded up to whole groups: the width of the codes of rows."""
+    return -(-k // GROUP) * GROUP
+
+
 class MxRows:
     """Rows ``[T, width]`` in 8 bits: ``codes`` uint8 ``[T, Kp]`` (E4M3) and
     ``scales`` uint8 ``[T, Kp / 32]``, Kp being the width rounded up to 128;
     the codes behind the width are zeros."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    width: int
+    __slots__ = ("_data", "_codes", "_scales", "rows", "width", "device", "codes_at", "scales_at")
 
-    def __post_init__(self):
-        t, kp = self.codes.shape[0], ops.mx_padded(self.width)
-        if self.width <= 0 or tuple(self.codes.shape) != (t, kp) or tuple(self.scales.shape) != (t, kp // ops.MX_BLOCK):
-            raise AlofaError("invalid_argument", "rows in 8 bits have the wrong size", f"codes={tuple(self.codes.shape)} scales={tuple(self.scales.shape)} width={self.width}")
-        _check(self.codes, "codes", 2, _BYTES), _check(self.scales, "scales", 2, _BYTES)
+    def __init__(self, codes, scales, width: int):
+        here = _here()
+        if width <= 0 or not isinstance(codes, torch.Tensor) or codes.dim() != 2:
+            raise AlofaError("invalid_argument", "rows in 8 bits are a matrix of codes", f"width={width}")
+        self._data, self._codes, self._scales = None, codes, scales
+        self.rows, self.width, self.device, kp = codes.shape[0], width, here, padded(width)
+        self.codes_at = _at(codes, "codes", _U8, (self.rows, kp), here)
+        self.scales_at = _at(scales, "scales", _U8, (self.rows, kp // BLOCK), here)
+        if self.codes_at % 16 or self.scales_at % 4:
+            raise AlofaError("unsupported", "codes must start on a 16-byte boundary, scales on one of 4", f"codes={self.codes_at % 16} scales={self.scales_at % 4}")
 
     @classmethod
-    def empty(cls, rows: int, width: int, device=None, buf=None) -> "MxRows":
+    def _empty(cls, rows: int, width: int, here: int, buf) -> "MxRows":
         """Room for rows, from ``buf(shape, dtype)`` (a step's scratch) or new."""
-        kp = ops.mx_padded(width)
-        make = buf or (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=device or "cuda"))
-        return cls(make((rows, kp), torch.uint8), make((rows, kp // ops.MX_BLOCK), torch.uint8), width)
+        self = cls.__new__(cls)
+        kp = -(-width // GROUP) * GROUP
+        size = rows * (kp + kp // BLOCK)
+        self._data = torch.empty(size, dtype=_U8, device=here) if buf is None else buf((size,), _U8)
+        self._codes = self._scales = None
+        self.rows, self.width, self.device = rows, width, here
+        self.codes_at = self._data.data_ptr()
+        self.scales_at = self.codes_at + rows * kp
+        return self
 
     @property
     def shape(self) -> tuple:
-        return self.codes.shape[0], self.width
+        return self.rows, self.width
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes if self._data is None else self._data[: self.rows * padded(self.width)].view(self.rows, -1)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales if self._data is None else self._data[self.rows * padded(self.width) :].view(self.rows, -1)
 
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
         """The numbers that the rows stand for (bfloat16 has them all, but for some below 2^-133)."""
-        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
-        ops.mx_rows_values(_check(out, "out", 2, _NUMBERS), self.codes, self.scales)
+        here = _on(self, "rows", _here())
+        if dtype is not _BF16 and dtype is not _F32:
+            raise AlofaError("unsupported", "numbers come in bfloat16 or float32", f"dtype={dtype}")
+        out = torch.empty((self.rows, self.width), dtype=dtype, device=here)
+        rc = ops.mx_library().alofa_mx_rows_values(out.data_ptr(), self.codes_at, self.scales_at, self.rows, self.width, dtype is _BF16, _stream(here))
+        ops.mx_launched(rc, 1, "mx rows' values", lambda: f"rows={self.rows} width={self.width}")
         return out
 
 
-@dataclass
+def _on(v, name: str, here: int) -> int:
+    if v.device != here:
+        raise AlofaError("invalid_argument", "kernels run on the current device only", f"{name} is on cuda:{v.device}, current is {here}")
+    return here
+
+
 class MxWeight:
     """A weight ``[n, k]`` in 4 bits, laid out in tiles of 128 rows and 128
     numbers as the product reads them.  ``gated``: the first half of the rows
-    are a gate's, the second an up projection's."""
+    are a gate's, the second an up projection's.  Made by :func:`pack_weight`
+    or :meth:`from_codes`."""
 
-    tiles: torch.Tensor
-    n: int
-    k: int
-    gated: bool = False
+    __slots__ = ("tiles", "n", "k", "gated", "rows", "device", "at")
 
-    @classmethod
-    def empty(cls, n: int, k: int, gated: bool, device) -> "MxWeight":
+    def __init__(self, n: int, k: int, gated: bool, here: int):
         if n <= 0 or k <= 0 or (gated and n % 2):
             raise AlofaError("invalid_argument", "a weight has rows and a depth, a gated one an even number of rows", f"rows={n} depth={k} gated={gated}")
-        shape = (-(-ops.mx_weight_rows(n, gated) // ops.MX_TILE_ROWS), ops.mx_padded(k) // ops.MX_GROUP, ops.MX_TILE_BYTES)
-        return cls(torch.empty(shape, dtype=torch.uint8, device=device), n, k, gated)
+        self.n, self.k, self.gated, self.device = n, k, bool(gated), here
+        #: rows of the product: a gated weight's features stand in turns of 16, padded to whole turns
+        self.rows = 2 * (-(-(n // 2) // GATE_ROWS) * GATE_ROWS) if gated else n
+        self.tiles = torch.empty((-(-self.rows // TILE_ROWS), padded(k) // GROUP, TILE_BYTES), dtype=_U8, device=here)
+        self.at = self.tiles.data_ptr()
 
     @classmethod
     def from_codes(cls, codes, scales, k: int, gated: bool = False) -> "MxWeight":
         """A weight that is in 4 bits already: ``codes`` uint8 ``[n, >= k / 2]``,
         two numbers a byte with the first in its low half, and ``scales`` uint8
         ``[n, >= k / 32]``; what they hold behind ``k`` is not read."""
-        _check(codes, "codes", 2, _BYTES), _check(scales, "scales", 2, _BYTES)
+        here = _here()
+        for t, name in ((codes, "codes"), (scales, "scales")):
+            if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype is not _U8 or t.get_device() != here:
+                _refuse(t, name, "uint8 of two dimensions", here)
         n = codes.shape[0]
-        if scales.shape[0] != n or codes.shape[1] < -(-k // 2) or scales.shape[1] < -(-k // ops.MX_BLOCK):
+        if scales.shape[0] != n or codes.shape[1] < -(-k // 2) or scales.shape[1] < -(-k // BLOCK):
             raise AlofaError("invalid_argument", "a weight's codes and scales disagree", f"codes={tuple(codes.shape)} scales={tuple(scales.shape)} depth={k}")
-        w = cls.empty(n, k, gated, codes.device)
+        w = cls(n, k, gated, here)
         tall, slices, _ = w.tiles.shape
-        c = codes.new_zeros((tall * ops.MX_TILE_ROWS, slices * ops.MX_GROUP // 2))
-        s = codes.new_zeros((tall * ops.MX_TILE_ROWS, slices * ops.MX_GROUP // ops.MX_BLOCK))
-        half, blocks = -(-k // 2), -(-k // ops.MX_BLOCK)
+        c = codes.new_zeros((tall * TILE_ROWS, slices * GROUP // 2))
+        s = codes.new_zeros((tall * TILE_ROWS, slices * GROUP // BLOCK))
+        half, blocks = -(-k // 2), -(-k // BLOCK)
         if gated:  # the gate's and the up projection's features in turns of 16
             f = torch.arange(n // 2, device=codes.device)
-            at = f // ops.MX_GATE_ROWS * (2 * ops.MX_GATE_ROWS) + f % ops.MX_GATE_ROWS
-            at = torch.cat([at, at + ops.MX_GATE_ROWS])
+            at = f // GATE_ROWS * (2 * GATE_ROWS) + f % GATE_ROWS
+            at = torch.cat([at, at + GATE_ROWS])
         else:
             at = torch.arange(n, device=codes.device)
         c[at, :half], s[at, :blocks] = codes[:, :half], scales[:, :blocks]
         if k % 2:
             c[:, k // 2] &= 15
-        size = ops.MX_TILE_ROWS * ops.MX_GROUP // 2
-        w.tiles[:, :, :size] = c.view(tall, ops.MX_TILE_ROWS, slices, ops.MX_GROUP // 2).permute(0, 2, 1, 3).reshape(tall, slices, size)
-        w.tiles[:, :, size:] = s.view(tall, 4, 32, slices, 4).permute(0, 3, 2, 1, 4).reshape(tall, slices, ops.MX_TILE_BYTES - size)
-        ops.mx_settle()
+        size = TILE_ROWS * GROUP // 2
+        w.tiles[:, :, :size] = c.view(tall, TILE_ROWS, slices, GROUP // 2).permute(0, 2, 1, 3).reshape(tall, slices, size)
+        w.tiles[:, :, size:] = s.view(tall, 4, 32, slices, 4).permute(0, 3, 2, 1, 4).reshape(tall, slices, TILE_BYTES - size)
+        # the product reads tiles ahead of the kernel before it
+        ops.mx_launched(ops.mx_library().alofa_mx_settle(_stream(here)), 1, "mx weight", str)
         return w
-
-    @property
-    def rows(self) -> int:
-        """Rows of the product: a gated weight's features are padded to whole turns of 16."""
-        return ops.mx_weight_rows(self.n, self.gated)
 
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
         """The numbers ``[n, k]`` that the weight stands for."""
-        out = torch.empty((self.n, self.k), dtype=dtype, device=self.tiles.device)
-        ops.mx_weight_values(_check(out, "out", 2, _NUMBERS), self.tiles, self.gated)
+        here = _on(self, "weight", _here())
+        if dtype is not _BF16 and dtype is not _F32:
+            raise AlofaError("unsupported", "numbers come in bfloat16 or float32", f"dtype={dtype}")
+        out = torch.empty((self.n, self.k), dtype=dtype, device=here)
+        rc = ops.mx_library().alofa_mx_weight_values(out.data_ptr(), self.at, self.n, self.k, self.gated, dtype is _BF16, _stream(here))
+        ops.mx_launched(rc, 1, "mx weight's values", lambda: f"rows={self.n} depth={self.k}")
         return out
 
 
 def pack_weight(w: torch.Tensor, gated: bool = False) -> MxWeight:
     """``w [N, K]`` (bfloat16 or float32) in 4 bits; ``gated``: a gate's N / 2
     rows above an up projection's, for :func:`gated_linear`."""
-    _check(w, "w", 2, _NUMBERS)
-    out = MxWeight.empty(w.shape[0], w.shape[1], gated, w.device)
-    ops.mx_pack(out.tiles, w, gated)
+    here = _here()
+    at, n, k, bf16 = _matrix(w, "w", here)
+    out = MxWeight(n, k, gated, here)
+    rc = ops.mx_library().alofa_mx_pack(out.at, at, n, k, out.gated, bf16, _stream(here))
+    ops.mx_launched(rc, 2, "pack_weight", lambda: f"rows={n} depth={k}")
     return out
 
 
 def quantize_rows(x: torch.Tensor, buf=None) -> MxRows:
     """``x [T, K]`` (bfloat16 or float32) as rows in 8 bits."""
-    _check(x, "x", 2, _NUMBERS)
-    rows = MxRows.empty(x.shape[0], x.shape[1], x.device, buf)
-    ops.mx_rows(rows.codes, rows.scales, x)
+    here = _here()
+    at, t, k, bf16 = _matrix(x, "x", here)
+    if not k:
+        raise AlofaError("invalid_argument", "rows have a width", "width=0")
+    rows = MxRows._empty(t, k, here, buf)
+    rc = ops.mx_library().alofa_mx_rows(rows.codes_at, rows.scales_at, at, t, k, bf16, _stream(here))
+    ops.mx_launched(rc, 1, "quantize_rows", lambda: f"rows={t} width={k}")
     return rows
 
 
@@ -161,78 +228,103 @@ def norm_rows(h: torch.Tensor, weight: torch.Tensor, eps: float, base=None, owed
     bits: ``h / sqrt(mean(h^2) + eps) * weight``.  With ``shift`` the layer
     norm, ``(h - mean) / sqrt(variance + eps) * weight + shift``.  ``owed
     [splits, T, K]`` are the sums that a product left (:func:`linear_parts`)."""
-    _check(h, "h", 2, _F32), _check(weight, "weight", 1, _F32)
-    for t, name, dims in ((base, "base", 2), (owed, "owed", 3), (bias, "bias", 1), (shift, "shift", 1)):
-        if t is not None:
-            _check(t, name, dims, _F32)
-    rows = MxRows.empty(h.shape[0], h.shape[1], h.device, buf)
-    ops.mx_norm(rows.codes, rows.scales, h, weight, eps, base, owed, bias, shift)
+    here = _here()
+    at, t, k, bf16 = _matrix(h, "h", here)
+    if bf16 or not k:
+        _refuse(h, "h", "float32 of two dimensions", here)
+    splits = owed.shape[0] if isinstance(owed, torch.Tensor) and owed.dim() else 0
+    rows = MxRows._empty(t, k, here, buf)
+    rc = ops.mx_library().alofa_mx_norm(
+        rows.codes_at, rows.scales_at, at, at if base is None else _at(base, "base", _F32, (t, k), here), None if owed is None else _at(owed, "owed", _F32, (splits, t, k), here), splits,
+        None if bias is None else _at(bias, "bias", _F32, (k,), here), _at(weight, "weight", _F32, (k,), here), None if shift is None else _at(shift, "shift", _F32, (k,), here), t, k, eps, _stream(here),
+    )
+    ops.mx_launched(rc, 1, "norm_rows", lambda: f"rows={t} width={k} most={MOST_WIDTH}")
     return rows
 
 
-def _operands(x, w, what: str, gated: bool, buf):
+def _operands(x, w, what: str, gated: bool, here: int, buf) -> MxRows:
     if not isinstance(w, MxWeight) or w.gated != gated:
-        raise AlofaError("invalid_argument", f"{what} takes a weight that was packed for it", f"gated={getattr(w, 'gated', None)} want={gated}")
-    _check(w.tiles, "w", 3, _BYTES)
+        raise AlofaError("invalid_argument", f"{what} takes a weight that was packed for it", f"weight={type(w).__name__} gated={getattr(w, 'gated', None)}")
     if not isinstance(x, MxRows):
         x = quantize_rows(x, buf)
     if x.width != w.k:
         raise AlofaError("invalid_argument", f"{what}: rows and weight differ in depth", f"rows={x.width} weight={w.k}")
-    _check(x.codes, "x", 2, _BYTES)
+    _on(x, "x", _on(w, "w", here))
     return x
+
+
+_plans: dict = {}
 
 
 def plan(tokens: int, rows: int, depth: int) -> tuple:
     """(tokens a tile, parts of the depth) of a product."""
-    bn = next((b for b in TOKEN_TILES if tokens <= b), TOKEN_TILES[-1])
-    ctas = -(-rows // ops.MX_TILE_ROWS) * -(-tokens // bn)
-    slices = ops.mx_padded(depth) // ops.MX_GROUP
-    room = 148 * (1 if bn == 256 else 2)
-    return bn, ops.mx_splits(depth, max(1, min(slices, room // ctas)))
+    key = (tokens, rows, depth)
+    found = _plans.get(key)
+    if found is None:
+        bn = next((b for b in TOKEN_TILES if tokens <= b), TOKEN_TILES[-1])
+        ctas = -(-rows // TILE_ROWS) * -(-tokens // bn)
+        room = 148 * (1 if bn == 256 else 2)
+        if len(_plans) >= 4096:
+            _plans.clear()
+        found = _plans[key] = (bn, ops.mx_library().alofa_mx_splits(depth, max(1, min(padded(depth) // GROUP, room // max(1, ctas)))))
+    return found
 
 
-def _room(shape, device, buf):
-    return buf(shape, torch.float32) if buf is not None else torch.empty(shape, dtype=torch.float32, device=device)
+def _sums(parts: int, t: int, rows: int, here: int, buf) -> torch.Tensor:
+    return torch.empty((parts, t, rows), dtype=_F32, device=here) if buf is None else buf((parts, t, rows), _F32)
 
 
-def linear(x, w: MxWeight, bias=None, add=None, out=None, dtype=None, buf=None, status=None) -> torch.Tensor:
+def linear(x, w: MxWeight, bias=None, add=None, out=None, dtype=None, buf=None, status=None, how: Optional[tuple] = None) -> torch.Tensor:
     """``out = x w^T (+ bias) (+ add)``.  ``x``: rows in 8 bits, or a tensor
     that is made such rows first; ``bias [N]``, ``add [T, N]`` float32
     (``add`` may be ``out``).  ``out`` (or ``dtype``): bfloat16 unless ``add``
-    is given, else float32."""
-    x = _operands(x, w, "linear", False, buf)
-    t = x.shape[0]
-    for v, name, dims in ((bias, "bias", 1), (add, "add", 2)):
-        if v is not None:
-            _check(v, name, dims, _F32)
+    is given, else float32.  ``status`` (int32): raised where a kernel gave up.
+    ``how``: another answer than :func:`plan`'s."""
+    here = _here()
+    x = _operands(x, w, "linear", False, here, buf)
+    t, n = x.rows, w.n
     if out is None:
-        out = torch.empty((t, w.n), dtype=dtype or (torch.bfloat16 if add is None else torch.float32), device=w.tiles.device)
-    _check(out, "out", 2, _NUMBERS)
-    bn, splits = plan(t, w.rows, w.k)
-    partial = _room((splits, t, w.rows), w.tiles.device, buf) if splits > 1 else None
-    ops.mx_gemm(out, x.codes, x.scales, w.tiles, w.n, w.k, bn, splits, partial, bias=bias, add=add, status=status)
+        dtype = dtype or (_BF16 if add is None else _F32)
+        if dtype is not _BF16 and dtype is not _F32:
+            raise AlofaError("unsupported", "a product is stored in bfloat16 or float32", f"dtype={dtype}")
+        out = torch.empty((t, n), dtype=dtype, device=here)
+        out_at, out_bf16 = out.data_ptr(), dtype is _BF16
+    else:
+        out_at, rows, columns, out_bf16 = _matrix(out, "out", here)
+        if rows != t or columns != n:
+            _refuse(out, "out", f"({t}, {n})", here)
+    bn, parts = how or plan(t, w.rows, w.k)
+    partial = _sums(parts, t, n, here, buf) if parts > 1 else None
+    rc = ops.mx_library().alofa_mx_gemm(
+        out_at, None if partial is None else partial.data_ptr(), x.codes_at, x.scales_at, w.at, None if bias is None else _at(bias, "bias", _F32, (n,), here),
+        None if add is None else _at(add, "add", _F32, (t, n), here), t, n, w.k, bn, parts, 0, out_bf16, None if status is None else _at(status, "status", _I32, status.shape, here), _stream(here),
+    )
+    ops.mx_launched(rc, 1 if parts == 1 else 2, "linear", lambda: f"tokens={t} rows={n} depth={w.k} how={(bn, parts)}")
     return out
 
 
-def linear_parts(x, w: MxWeight, buf=None, status=None) -> torch.Tensor:
+def linear_parts(x, w: MxWeight, buf=None, status=None, how: Optional[tuple] = None, gated: bool = False) -> torch.Tensor:
     """The sums of ``x w^T`` for each part of the depth, ``[parts, T, N]``
-    float32, for a reader that adds them (:func:`norm_rows`)."""
-    x = _operands(x, w, "linear_parts", False, buf)
-    bn, splits = plan(x.shape[0], w.rows, w.k)
-    sums = _room((splits, x.shape[0], w.rows), w.tiles.device, buf)
-    ops.mx_gemm(None, x.codes, x.scales, w.tiles, w.n, w.k, bn, splits, sums, leave=True, status=status)
+    float32, for a reader that adds them (:func:`norm_rows`).  Of a ``gated``
+    weight: a column for each of its ``rows``."""
+    here = _here()
+    x = _operands(x, w, "linear_parts", gated, here, buf)
+    bn, parts = how or plan(x.rows, w.rows, w.k)
+    sums = _sums(parts, x.rows, w.rows, here, buf)
+    rc = ops.mx_library().alofa_mx_gemm(
+        None, sums.data_ptr(), x.codes_at, x.scales_at, w.at, None, None, x.rows, w.rows, w.k, bn, parts, 1, 0, None if status is None else _at(status, "status", _I32, status.shape, here), _stream(here),
+    )
+    ops.mx_launched(rc, 1, "linear_parts", lambda: f"tokens={x.rows} rows={w.rows} depth={w.k} how={(bn, parts)}")
     return sums
 
 
-def gated_linear(x, w: MxWeight, gate=ops.SILU_GATE, buf=None, status=None) -> MxRows:
+def gated_linear(x, w: MxWeight, gate=ops.SILU_GATE, buf=None, status=None, how: Optional[tuple] = None) -> MxRows:
     """``silu(x Wg^T) * (x Wu^T)`` as rows in 8 bits; ``gate`` = (alpha,
     limit): the clamped form ``g = min(g, limit), u = clamp(u, -limit, limit):
     g sigmoid(alpha g) (u + 1)``."""
-    x = _operands(x, w, "gated_linear", True, buf)
-    t = x.shape[0]
-    rows = MxRows.empty(t, w.n // 2, w.tiles.device, buf)
-    bn, splits = plan(t, w.rows, w.k)
-    sums = _room((splits, t, w.rows), w.tiles.device, buf)
-    ops.mx_gemm(None, x.codes, x.scales, w.tiles, w.n, w.k, bn, splits, sums, leave=True, gated=True, status=status)
-    ops.mx_gate(rows.codes, rows.scales, sums, w.n // 2, gate)
+    sums = linear_parts(x, w, buf, status, how, gated=True)
+    here, (parts, t, _), f = w.device, sums.shape, w.n // 2
+    rows = MxRows._empty(t, f, here, buf)
+    rc = ops.mx_library().alofa_mx_gate(rows.codes_at, rows.scales_at, sums.data_ptr(), parts, t, f, gate[0], gate[1], _stream(here))
+    ops.mx_launched(rc, 1, "gated_linear", lambda: f"tokens={t} features={f}")
     return rows

@@ -190,13 +190,11 @@ def test_linear(t, n, k):
 def test_every_tile_and_part(bn, asked):
     t, n, k = 70, 200, 1100
     xr, wp, xv, wv = product_operands(t, n, k, 20)
-    splits = ops.mx_splits(k, asked)
-    partial = torch.full((splits, t, n), float("nan"), device="cuda")
-    out = torch.empty(t, n, device="cuda")
-    ops.mx_gemm(out, xr.codes, xr.scales, wp.tiles, n, k, bn, splits, partial)
+    parts = ops.mx_library().alofa_mx_splits(k, min(asked, mx.padded(k) // 128))
+    out = mx.linear(xr, wp, dtype=F32, how=(bn, parts))
     assert (np.abs(host(out) - xv @ wv.T) <= sum_bound(xv, wv)).all()
-    ops.mx_gemm(None, xr.codes, xr.scales, wp.tiles, n, k, bn, splits, partial, leave=True)
-    assert (np.abs(host(partial).astype(np.float64).sum(0) - xv @ wv.T) <= sum_bound(xv, wv)).all()
+    left = mx.linear_parts(xr, wp, how=(bn, parts))
+    assert left.shape == (parts, t, n) and (np.abs(host(left).astype(np.float64).sum(0) - xv @ wv.T) <= sum_bound(xv, wv)).all()
 
 
 def test_every_pair_of_codes():
@@ -231,7 +229,7 @@ def test_scales_over_their_whole_range():
 
 def test_a_block_of_nan_reaches_its_row_only():
     xr, wp, xv, wv = product_operands(5, 140, 300, 30)
-    xr.scales[2, 1] = 255
+    xr.scales[2, 1] = 255  # a view of the rows' own memory
     got = host(mx.linear(xr, wp, dtype=F32))
     assert np.isnan(got[2]).all() and np.isfinite(got[[0, 1, 3, 4]]).all()
 
