@@ -58,6 +58,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--num-prompts", type=int, default=1, help="how many random prompts with --prompt-len")
     ap.add_argument("--max-new-tokens", type=int, default=DEFAULT_NEW)
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    ap.add_argument("--weight-format", choices=["mxfp4"], default=None, help="keep the layers' weights in 4 bits with a scale for each 32 numbers")
     # sampling: the reference's SampleParams (src/alofa/runtime/sampler.mojo:93-118)
     ap.add_argument("--temperature", type=float, default=0.0, help="0 = greedy")
     ap.add_argument("--top-k", type=int, default=0)
@@ -117,7 +118,7 @@ def main(argv=None) -> int:
     from alofa_b200.sampling.params import SamplingParams
 
     settings = dict(
-        dtype=args.dtype, max_tokens=args.max_tokens, token_budget=args.token_budget, max_chunk=args.max_chunk,
+        dtype=args.dtype, weight_format=args.weight_format, max_tokens=args.max_tokens, token_budget=args.token_budget, max_chunk=args.max_chunk,
         block_size=args.block_size, capacity_blocks=args.capacity_blocks, watermark_permille=args.watermark_permille,
         max_wait_ticks=args.max_wait_ticks, max_batch=args.max_batch, admission=args.admission, trace_out=args.trace_out,
     )

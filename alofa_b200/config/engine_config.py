@@ -9,6 +9,7 @@ size at compile time (8 requests, 64 rows per step) the size is a field."""
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
 
 from ..errors import AlofaError
 
@@ -16,6 +17,7 @@ from ..errors import AlofaError
 @dataclass
 class EngineConfig:
     dtype: str = "bfloat16"  # "bfloat16" or "float32"
+    weight_format: Optional[str] = None  # None: the layers' weights in that dtype; "mxfp4": in 4 bits with a scale for each 32 (bfloat16 only)
     block_size: int = 64  # tokens per cache page
     capacity_blocks: int = 0  # pages per cache group; 0 = derive from max_batch * max_tokens
     max_batch: int = 64  # live requests
@@ -34,6 +36,8 @@ class EngineConfig:
                 raise AlofaError("invalid_argument", what, detail)
 
         need(self.dtype in ("bfloat16", "float32"), "dtype must be bfloat16 or float32", f"dtype={self.dtype}")
+        need(self.weight_format in (None, "mxfp4"), "weight_format must be mxfp4 or None", f"weight_format={self.weight_format}")
+        need(self.weight_format is None or self.dtype == "bfloat16", "weight_format mxfp4 needs dtype bfloat16", f"dtype={self.dtype}")
         need(self.block_size > 0 and self.block_size % 16 == 0, "block_size must be a positive multiple of 16", f"block_size={self.block_size}")
         need(self.capacity_blocks >= 0, "capacity_blocks must not be negative", f"capacity_blocks={self.capacity_blocks}")
         need(self.max_batch > 0, "max_batch must be positive", f"max_batch={self.max_batch}")

@@ -82,7 +82,7 @@ class Engine:
         else:
             if model is None:
                 raise AlofaError("invalid_argument", "Engine needs a model folder")
-            self.model, self.model_config, self.architecture = load_model(model, cfg.dtype, device)
+            self.model, self.model_config, self.architecture = load_model(model, cfg.dtype, device, cfg.weight_format)
         spec = self.model.spec
         self.max_tokens = min(cfg.max_tokens, spec.max_position)
         blocks_per_request = -(-self.max_tokens // cfg.block_size)
@@ -122,7 +122,8 @@ class Engine:
     @classmethod
     def from_random(cls, architecture: str, model_config, seed: int, dtype: str = "bfloat16", device=None, generate_on_device: bool = False, **kwargs):
         """An engine over seeded random weights of a typed model configuration."""
-        loaded = random_model(architecture, model_config, seed, dtype, device, generate_on_device)
+        weight_format = kwargs.get("weight_format", kwargs["config"].weight_format if kwargs.get("config") is not None else None)
+        loaded = random_model(architecture, model_config, seed, dtype, device, generate_on_device, weight_format)
         return cls(dtype=dtype, _loaded=loaded, **kwargs)
 
     # -- requests -----------------------------------------------------------

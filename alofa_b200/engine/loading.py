@@ -36,26 +36,27 @@ def require_cuda(device=None) -> torch.device:
     return dev
 
 
-def load_model(folder, dtype="bfloat16", device=None):
+def load_model(folder, dtype="bfloat16", device=None, weight_format=None):
     """(model, typed config, architecture) of a folder with config.json and
-    model.safetensors; the model class is chosen by config.json."""
+    model.safetensors; the model class is chosen by config.json.
+    ``weight_format`` "mxfp4": the layers' weights are kept in 4 bits."""
     dev = require_cuda(device)
     arch, cfg = read_model_config(folder)
     spec = arch.build_spec(cfg)
-    model = Model(spec, Runtime(dev, compute_dtype(dtype)))
+    model = Model(spec, Runtime(dev, compute_dtype(dtype), weight_format))
     state = load_state(model.tensors(), folder, model.rt.dtype, dev)
     model.load(state)
     return model, cfg, arch
 
 
-def random_model(architecture: str, config, seed: int, dtype="bfloat16", device=None, generate_on_device: bool = False):
+def random_model(architecture: str, config, seed: int, dtype="bfloat16", device=None, generate_on_device: bool = False, weight_format=None):
     """A model with seeded random weights, without a folder on disk.  With
     ``generate_on_device`` the numbers are drawn by the device's generator
     (fast for large shapes; a different stream than the CPU's)."""
     dev = require_cuda(device)
     arch = get_architecture(architecture)
     spec = arch.build_spec(config)
-    model = Model(spec, Runtime(dev, compute_dtype(dtype)))
+    model = Model(spec, Runtime(dev, compute_dtype(dtype), weight_format))
     state = random_state(model.tensors(), seed, torch.bfloat16, dev if generate_on_device else "cpu")
     model.load(load_state(model.tensors(), state, model.rt.dtype, dev))
     return model, config, arch

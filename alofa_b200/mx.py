@@ -188,6 +188,15 @@ class MxWeight:
         ops.mx_launched(ops.mx_library().alofa_mx_settle(_stream(here)), 1, "mx weight", str)
         return w
 
+    def first_rows(self, n: int) -> "MxWeight":
+        """The weight's first ``n`` rows, in the same memory."""
+        if self.gated or not 0 < n <= self.n:
+            raise AlofaError("invalid_argument", "the first rows of a weight that is not gated", f"rows={n} of {self.n} gated={self.gated}")
+        part = MxWeight.__new__(MxWeight)
+        part.n, part.rows, part.k, part.gated, part.device = n, n, self.k, False, self.device
+        part.tiles, part.at = self.tiles[: -(-n // TILE_ROWS)], self.at
+        return part
+
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
         """The numbers ``[n, k]`` that the weight stands for."""
         here = _on(self, "weight", _here())

@@ -21,7 +21,8 @@ from ..csrc import ops
 from ..errors import AlofaError
 from . import fast_linear
 from .base import PagedKV, Part, TensorSpec, as_float32_vector, build_part, register_part
-from .linear import RESIDUAL, STORE, Linear, MergedSplits, add_into_stream
+from .linear import RESIDUAL, STORE, MergedSplits, add_into_stream
+from .mx_linear import make_linear
 
 
 class PagedAttend:
@@ -204,13 +205,15 @@ class GQAttention(PagedAttend, Part):
         b = None
         if self.qkv_bias:
             b = as_float32_vector(torch.cat([state[pre + f"{n}_proj.bias"] for n in "qkv"], dim=0))
-        self.qkv = Linear(w, b, STORE)
+        self.qkv = make_linear(self.rt, w, b, STORE)
         # a run of this layer that reads another run's cache needs q only
-        self.q_only = Linear(w[: self.q_dim], b[: self.q_dim] if b is not None else None, STORE)
+        q_weight = self.qkv.weight.first_rows(self.q_dim) if self.rt.weight_format is not None else w[: self.q_dim]
+        self.q_only = make_linear(self.rt, q_weight, b[: self.q_dim] if b is not None else None, STORE)
         ob = as_float32_vector(state[pre + "o_proj.bias"]) if self.out_bias else None
-        self.out = Linear(state[pre + "o_proj.weight"], ob, RESIDUAL)
+        self.out = make_linear(self.rt, state[pre + "o_proj.weight"], ob, RESIDUAL)
         self.position.load(state)
 
+    takes_weight_formats = True
     takes_normed_rows = True  # ``x`` may be rows still to be made: the q/k/v kernel of a few tokens folds the norm in
 
     def forward(self, ctx, x, h, cache, writes=True):
@@ -225,6 +228,10 @@ class GQAttention(PagedAttend, Part):
         vectorised = dt == torch.bfloat16 and custom is None and rot == self.hd and self.hd % 16 == 0
         lin = self.qkv if writes else self.q_only
         q = ctx.buf((n, self.q_dim), dt)
+        if self.rt.weight_format is not None:
+            self._project(ctx, lin, x, q, cache, group, table, rot, custom, vectorised, nkv_in, writes)
+            add_into_stream(ctx, self.out, h, self.attend(ctx, q, cache, group))
+            return
         # a handful of tokens: product, bias, rotation and the cache write in one kernel
         # (its depth split over a cluster of up to eight CTAs: the largest for which every tile's cluster is
         # resident at once - a GPC holds whole clusters only, 16 clusters of 8 ran in two waves where 16 of 6 run
@@ -252,11 +259,14 @@ class GQAttention(PagedAttend, Part):
             done = ops.gemm_tc_rope(x, lin.weight, lin.bias, q, cache.k, cache.v, group.slot_map, ctx.positions, table, self.nh, nkv_in, self.hd,
                                     depth_splits, ctx.status)
         if not done:
-            qkv = ctx.buf((n, (self.nh + 2 * nkv_in) * self.hd), dt)
-            owed = lin(qkv, x, defer=vectorised, buf=ctx.buf)
-            self._rotate_and_store(ctx, q, qkv, owed, cache, group, table, rot, custom, vectorised, nkv_in, writes)
+            self._project(ctx, lin, x, q, cache, group, table, rot, custom, vectorised, nkv_in, writes)
         attn = self.attend(ctx, q, cache, group)
         add_into_stream(ctx, self.out, h, attn)
+
+    def _project(self, ctx, lin, x, q, cache, group, table, rot, custom, vectorised, nkv_in, writes):
+        qkv = ctx.buf((q.shape[0], (self.nh + 2 * nkv_in) * self.hd), self.rt.dtype)
+        owed = lin(qkv, x, defer=vectorised, buf=ctx.buf)
+        self._rotate_and_store(ctx, q, qkv, owed, cache, group, table, rot, custom, vectorised, nkv_in, writes)
 
     def _rotate_and_store(self, ctx, q, qkv, owed, cache, group, table, rot, custom, vectorised, nkv_in, writes):
         n = q.shape[0]

@@ -85,10 +85,12 @@ class SlotState:
 
 @dataclass
 class Runtime:
-    """What parts share: the device and the compute dtype."""
+    """What parts share: the device, the compute dtype, and the form that the
+    layers' weights are kept in."""
 
     device: torch.device
     dtype: torch.dtype  # torch.float32 (true 32-bit path) or torch.bfloat16
+    weight_format: Optional[str] = None  # None: the compute dtype; "mxfp4": 4 bits with a scale for each 32 (parts that say takes_weight_formats)
 
 
 class Part:
@@ -100,6 +102,8 @@ class Part:
     # host-side dependence on device data: such a part can be recorded in a
     # CUDA graph.  Parts must opt in.
     graph_safe = False
+    # True for a mixer or feed-forward that keeps its weights as rt.weight_format says.
+    takes_weight_formats = False
 
     def __init__(self, spec: PartSpec, rt: Runtime):
         self.spec = spec

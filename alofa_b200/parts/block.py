@@ -74,6 +74,8 @@ class PrenormResidual(Part):
         if not getattr(norm, "absorbs_pending", False):
             ctx.flush_pending()
             return norm.forward(ctx, h)
+        if self.rt.weight_format is not None and getattr(reader, "takes_weight_formats", False) and getattr(norm, "gives_mx_rows", False):
+            return norm.mx_rows(ctx, h)  # the rows in 8 bits that the reader's products take
         # a reader that says so may get rows still to be made (the norm folded into its own product)
         if getattr(reader, "takes_normed_rows", False) and getattr(norm, "gives_normed_rows", False):
             return norm.forward(ctx, h, lazy=True)

@@ -83,7 +83,7 @@ class DecodeStack:
         form the kernel has (or not loaded).  Looked at anew for every step
         that is not a replay: a model may be loaded again."""
         model, caches = self.model, self.caches
-        if model.rt.dtype != torch.bfloat16 or model.stream_copies or model.keeps_embedding or model.shared_value_width:
+        if model.rt.dtype != torch.bfloat16 or model.rt.weight_format is not None or model.stream_copies or model.keeps_embedding or model.shared_value_width:
             return None
         shapes, layers, bf16, fp32, cuda = set(), [], torch.bfloat16, torch.float32, model.rt.device.type == "cuda"
         for i, (layer, cache) in enumerate(model.run):

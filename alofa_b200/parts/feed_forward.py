@@ -12,6 +12,7 @@ from ..errors import AlofaError
 from . import fast_linear
 from .base import Part, TensorSpec, as_float32_vector, register_part
 from .linear import GATED, RESIDUAL, STORE, Linear, add_into_stream
+from .mx_linear import make_linear
 
 
 class GatedMLP(Part):
@@ -37,15 +38,19 @@ class GatedMLP(Part):
 
     def load(self, state):
         pre = self.prefix
-        self.gate_up = Linear(torch.cat([state[pre + "gate_proj.weight"], state[pre + "up_proj.weight"]], dim=0), None, GATED)
-        self.down = Linear(state[pre + "down_proj.weight"], None, RESIDUAL)
+        self.gate_up = make_linear(self.rt, torch.cat([state[pre + "gate_proj.weight"], state[pre + "up_proj.weight"]], dim=0), None, GATED)
+        self.down = make_linear(self.rt, state[pre + "down_proj.weight"], None, RESIDUAL)
 
     def scratch_row_bytes(self) -> int:
         return 4 * self.inter + fast_linear.owed_row_bytes(self.hidden, self.inter)  # the activation, and the down product's sums where they are left to the consumer
 
     takes_normed_rows = True  # ``x`` may be rows still to be made: the gate/up product folds the norm in
+    takes_weight_formats = True
 
     def forward(self, ctx, x, h):
+        if self.rt.weight_format is not None:
+            add_into_stream(ctx, self.down, h, self.gate_up.gated_rows(x, ctx.buf))
+            return
         act = ctx.buf((x.shape[0], self.inter), self.rt.dtype)
         self.gate_up(act, x, buf=ctx.buf)
         add_into_stream(ctx, self.down, h, act)

@@ -13,6 +13,8 @@ from ..config.spec import ModelSpec
 from ..csrc import ops
 from ..errors import AlofaError
 from .base import Runtime, build_part
+from .block import PrenormResidual
+from .mx_linear import WEIGHT_FORMATS
 
 
 class Model:
@@ -22,6 +24,8 @@ class Model:
         self.rt = rt
         self.embedding = build_part("embedding", spec.embedding, rt)
         self.layers = [build_part("block", layer.block, rt) for layer in spec.layers]
+        if rt.weight_format is not None:
+            self._check_weight_format()
         self.final_norm = build_part("norm", spec.final_norm, rt)
         self.head = build_part("head", spec.head, rt)
         self.run = [(e.layer, i if e.cache is None else e.cache) for i, e in enumerate(spec.run)]
@@ -43,6 +47,17 @@ class Model:
             raise AlofaError("unsupported", "blocks over several residual streams cannot be mixed with others", f"stream_copies={sorted(copies)}")
         self.stream_copies = copies.pop() if copies else 0
         self.loads = 0  # how often weights were loaded: what was recorded of earlier ones is not run again
+
+    def _check_weight_format(self) -> None:
+        """Weights in another form than the compute dtype: where every layer's mixer and feed-forward keep theirs so."""
+        if self.rt.weight_format not in WEIGHT_FORMATS:
+            raise AlofaError("unsupported", "unknown weight format", f"weight_format={self.rt.weight_format} known={WEIGHT_FORMATS}")
+        if self.rt.dtype != torch.bfloat16:
+            raise AlofaError("unsupported", "weights in 4 bits are for the bfloat16 path", f"dtype={self.rt.dtype}")
+        for block in self.layers:
+            others = [p.spec.kind for p in (getattr(block, "mixer", None), getattr(block, "feed_forward", None)) if p is not None and not p.takes_weight_formats]
+            if others or not isinstance(block, PrenormResidual):
+                raise AlofaError("unsupported", "a layer of this model does not take a weight format", f"weight_format={self.rt.weight_format} block={block.spec.kind} parts={others}")
 
     def parts(self):
         return [self.embedding, *self.layers, self.final_norm, self.head]

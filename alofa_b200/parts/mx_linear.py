@@ -1,0 +1,57 @@
+"""Matrix products of the parts with weights in 4 bits and rows in 8
+(``weight_format="mxfp4"``; the formats and kernels: :mod:`alofa_b200.mx`).
+
+A :class:`MxLinear` is called as a :class:`~alofa_b200.parts.linear.Linear` is.
+The weight is packed when the part loads.  Rows come in 8 bits from the norm in
+front (:class:`~alofa_b200.mx.MxRows`); any other rows are made so first.  A
+product in parts of its depth leaves their sums to a consumer that asks
+(``defer``), as the bfloat16 products do."""
+from __future__ import annotations
+
+import torch
+
+from .. import mx
+from ..csrc import ops
+from ..errors import AlofaError
+from .linear import GATED, RESIDUAL, STORE, Linear, Partial
+
+MXFP4 = "mxfp4"
+WEIGHT_FORMATS = (None, MXFP4)
+
+
+class MxLinear:
+    """``epi`` STORE: out = x W^T + b.  RESIDUAL: out (fp32) += x W^T + b.
+    GATED: W = [gate; up]; :meth:`gated_rows` instead of a call."""
+
+    def __init__(self, weight, bias, epi: int = STORE, gate=ops.SILU_GATE):
+        self.weight = weight if isinstance(weight, mx.MxWeight) else mx.pack_weight(weight.contiguous(), gated=epi == GATED)
+        self.bias, self.epi, self.gate, self.act = bias, epi, gate, 0
+        self.in_features, self.out_features = self.weight.k, self.weight.n // 2 if epi == GATED else self.weight.n
+        if bias is not None and epi == GATED:
+            raise AlofaError("unsupported", "a gated product with weights in 4 bits takes no bias")
+
+    def can_accumulate(self, tokens: int) -> bool:
+        return False  # its parts are added by the norm that reads the stream next
+
+    def _rows(self, x, buf):
+        if isinstance(x, mx.MxRows):
+            return x
+        return mx.quantize_rows(x if isinstance(x, torch.Tensor) else x.rows(), buf)
+
+    def __call__(self, out, x, defer: bool = False, buf=None):
+        x = self._rows(x, buf)
+        if defer and (self.epi == RESIDUAL or mx.plan(x.rows, self.weight.rows, self.weight.k)[1] > 1):
+            sums = mx.linear_parts(x, self.weight, buf)
+            return Partial(sums, sums.shape[0], self.bias)
+        mx.linear(x, self.weight, bias=self.bias, add=out if self.epi == RESIDUAL else None, out=out, buf=buf)
+        return None
+
+    def gated_rows(self, x, buf=None) -> mx.MxRows:
+        return mx.gated_linear(self._rows(x, buf), self.weight, self.gate, buf)
+
+
+def make_linear(rt, weight, bias, epi: int = STORE, gate=ops.SILU_GATE):
+    """A product of a part's: in the model's compute dtype, or with its weight in 4 bits."""
+    if rt.weight_format == MXFP4:
+        return MxLinear(weight, bias, epi, gate)
+    return Linear(weight, bias, epi, gate=gate)

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import torch
 
+from .. import mx
 from ..csrc import ops
 from .base import Part, TensorSpec, as_float32_vector, register_part
 from .linear import NormedRows
@@ -49,6 +50,20 @@ class RMSNorm(Part):
         if lazy and rows is None and ctx.stream_of(h) is not None and h.shape[1] == self.size:
             return NormedRows(ctx, h, self)
         return self.rows_now(ctx, h, rows)
+
+    gives_mx_rows = True
+
+    def mx_rows(self, ctx, h):
+        """Every normalised row of the stream in 8 bits (:class:`~alofa_b200.mx.MxRows`);
+        sums that a product left are added on the way."""
+        pend = ctx.pending
+        if pend is not None and pend.h is h and (pend.partial is None or pend.base is not h):
+            ctx.flush_pending()  # kept as base + accumulator: nothing here reads that
+        pend = ctx.take_pending(h)
+        owed = pend.partial if pend is not None else None
+        if owed is None:
+            return mx.norm_rows(h, self.weight, self.eps, shift=self.shift, buf=ctx.buf)
+        return mx.norm_rows(h, self.weight, self.eps, owed=owed.sums[: owed.splits], bias=owed.bias, shift=self.shift, buf=ctx.buf)
 
     def rows_now(self, ctx, h, rows=None):
         n = h.shape[0] if rows is None else rows.shape[0]
