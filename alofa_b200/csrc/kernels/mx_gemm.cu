@@ -1,7 +1,9 @@
 // Product of rows in 8 bits and a weight in 4 (mx.cuh) on the 5th-generation tensor cores:
-//   y[t, f] = sum_b 2^(sx[t, b] + sw[f, b] - 254) sum_{k in block b} x[t, k] w[f, k]   (+ bias[f]) (+ add[t, f])
-// One tcgen05.mma.kind::mxf8f6f4.block_scale takes 128 weight rows, BN tokens and one block of 32 numbers;
-// the scales are its operands too, in tensor memory, so sums are of the numbers themselves and in fp32.
+//   y[t, f] = sum_b 2^(sx[t, b] + sw[f, b] - 254) sum_{k in block b} x[t, k] w[f, k]
+// and out = y (+ bias[f]) (+ add[t, f]) in bf16 or fp32, or, for a gated weight, rows in 8 bits of
+// silu(y of the gate) * (y of the up projection)  (src/alofa/kernels/cpu/scalar.mojo:132-231).
+// One tcgen05.mma.kind::mxf8f6f4.block_scale takes one block of 32 numbers of its rows; the scales are its
+// operands too, in tensor memory, so sums are of the numbers themselves and in fp32.
 //
 // A k-slice is 128 numbers: four blocks.  A weight's tile of a slice is 8,704 contiguous bytes of memory
 // (8,192 of codes, 512 of scales).  Shared memory holds 4-bit operands as 16 numbers in 8 bytes and 8 bytes
@@ -10,27 +12,29 @@
 // (fence.proxy.async) when they have landed.  Tokens come by TMA, their scales 4 bytes a row.  The weights
 // depend on no earlier kernel of the stream: the first ring of them is asked for before the dependency wait.
 //
-// Scales in tensor memory have as many places as the ring has stages, so those of a slice are written
-// only when the products that read the slice before them in that place are complete.
+// Two kernels: mx_few_kernel, the weight's rows on the M side, for a few tokens or few tiles, whose time is
+// the weight's bytes or a launch's latency; mx_pair_kernel, the tokens on the M side and a pair of CTAs to a
+// tile, for prompts, whose time is the tensor cores'.
 //
 // Every wait on an mbarrier is bounded: after the limit the CTA raises the status word, lets its copies
-// land, frees its tensor memory and returns.
+// and products end, frees its tensor memory and returns; what it should have written is NaN.
 #include "mx.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
 
 #include <atomic>
 
-constexpr int MX_THREADS = 192;  // warps 0-3 weights, then the epilogue; warp 4 tokens; warp 5 products
-
 struct MxArgs {
   const uint8_t* tiles;     // the weight: [ceil(N / 128), slices, MX_TILE_BYTES]
   const uint8_t* x_scales;  // [T, 4 * slices]
-  void* out;                // [T, N] bf16 or fp32
+  void* out;                // [T, N] bf16 or fp32; gated: codes [T, padded(F)]
+  uint8_t* out_scales;      // gated: [T, padded(F) / 32]
   const float* bias;        // [N] or null
   const float* add;         // [T, N] or null
-  float* partial;           // [splits, T, N]: the sums of each part of the depth are left here, and nothing else done
-  int T, N, slices, per_split, out_bf16;
+  int T, N, slices;         // tokens, rows of the weight, k-slices
+  int F;                    // gated: features
+  int out_bf16, wide;       // wide: four numbers of a row are stored (and bias and add read) at once
+  float gate_alpha, gate_limit;
   int* status;
 };
 
@@ -51,11 +55,27 @@ __device__ __forceinline__ void copies_wait_but(int n) {  // all of this thread'
   }
 }
 __device__ __forceinline__ void fence_to_tensor_core() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void load_tokens(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+// A weight's tile: thread i of 128 copies 8 bytes of every sixteenth row (the same place in their groups of 8), the first 32 the scales.
+__device__ __forceinline__ void load_weight_tile(uint32_t dst, const uint8_t* from, int i) {
+  const int row = i >> 3, chunk = i & 7;
+  const uint32_t to = dst + (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) copy8(to + j * 16 * 128, from + j * 1024 + i * 8);
+}
+// Ends early: what is still in flight lands in a bounded time.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+  for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(bar, parity); ++w) {
+  }
+}
 
+// Shared memory seen as rows of 16 bytes, groups of 8 rows 128 bytes apart, no swizzle.
+__device__ __forceinline__ uint64_t scales_desc(uint32_t smem) { return (uint64_t)((smem & 0x3FFFFu) >> 4) | (8ull << 16) | (8ull << 32) | (1ull << 46); }
 // 512 bytes of scales (32 rows of 16) to four columns of tensor memory, the same in all four quarters of its lanes.
 __device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t smem) {
-  const uint64_t desc = (uint64_t)((smem & 0x3FFFFu) >> 4) | (8ull << 16) | (8ull << 32) | (1ull << 46);  // rows of 16 bytes, groups of 8 rows 128 bytes apart, no swizzle
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scales_desc(smem)) : "memory");
 }
 __device__ __forceinline__ void umma_mx(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
   asm volatile(
@@ -65,24 +85,118 @@ __device__ __forceinline__ void umma_mx(uint32_t tmem_d, uint64_t desc_a, uint64
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
       : "memory");
 }
-// Instruction: E2M1 (5) times E4M3 (0), scales E8M0, M = 128, N, the scales' byte `block` of their column.
-constexpr uint32_t mx_idesc(int n, int block) { return (5u << 7) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (1u << 27) | ((uint32_t)block << 29) | ((uint32_t)block << 4); }
+// The same for a pair of CTAs: each CTA's own shared memory to its own tensor memory.
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t tmem, uint32_t smem) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scales_desc(smem)) : "memory");
+}
+__device__ __forceinline__ void umma_mx_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+      : "memory");
+}
+constexpr uint32_t E4M3 = 0, E2M1 = 5;
+// The instruction: types of A and B, scales E8M0, M and N, the scales' byte `block` of their column.
+constexpr uint32_t mx_idesc(uint32_t a, uint32_t b, int m, int n, int block) {
+  return (a << 7) | (b << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27) | ((uint32_t)block << 29) | ((uint32_t)block << 4);
+}
+
+__device__ __forceinline__ uint32_t cta_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {  // every thread of every CTA of the cluster
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------
+// A few tokens.  A CTA has 128 of the weight's rows, BN tokens and a part of the depth; the CTAs of a tile's
+// parts are a cluster.  Each leaves its sums in its shared memory as [token][row]; the cluster's CTAs share
+// out the tokens, add the parts in order out of one another's shared memory and write whole rows: no sums go
+// through memory, nothing is launched to add them, and the last step is spread over as many SMs as the first.
+// ---------------------------------------------------------------------------
+constexpr int FEW_THREADS = 192;  // warps 0-3 weights, then the sums; warp 4 tokens; warp 5 products
+constexpr int FEW_PARTS = 8;      // of a depth, at most: a portable cluster
+constexpr int SUM_PITCH = MX_TILE_ROWS + 4;
 
 template <int BN>
-struct MxTile {
-  static constexpr int STAGES = BN <= 32 ? 5 : BN == 64 ? 4 : BN == 128 ? 3 : 4;
-  static constexpr int B_ATOMS = BN > 128 ? 2 : 1;
+struct FewTile {
+  static constexpr int STAGES = BN <= 32 ? 5 : BN == 64 ? 4 : 3;  // two CTAs an SM
   static constexpr uint32_t A_BYTES = MX_TILE_ROWS * MX_GROUP, B_BYTES = BN * MX_GROUP;
-  static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES + (BN > 128 ? 2048 : 1024);  // tiles, 512 bytes of the weight's scales, the tokens'
+  static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES + 1024;  // tiles, 512 bytes of the weight's scales, 512 of the tokens'
   static constexpr uint32_t SMEM = STAGES * STAGE_BYTES + 1024;
-  static constexpr int SCALE_COLS = 4 + 4 * B_ATOMS;
-  static constexpr int COLS = BN + STAGES * SCALE_COLS;
-  static constexpr uint32_t TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static constexpr int COLS = BN + STAGES * 8;  // the scales have as many places as the ring has stages: those of a slice are written when the products of the slice before them there are complete
+  static constexpr uint32_t TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+  static_assert(BN * SUM_PITCH * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's room");
 };
 
+// Four neighbouring rows' sums of one token, as a gated weight has them (16 rows of the gate, the same 16 of the up
+// projection): the warp's 64 features as codes and two scales.  f0: the first of the tile's features.
+__device__ __forceinline__ void few_gated_token(const MxArgs& args, float4 v, int t, int f0, int lane) {
+  const int f = f0 + (lane >> 3) * 16 + (lane & 3) * 4;  // lanes with bit 2 clear have the gate's rows, those with it set the up projection's
+  float g[4] = {v.x, v.y, v.z, v.w};
+  uint32_t largest = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float u = __shfl_xor_sync(0xffffffffu, g[j], 4);
+    g[j] = f + j < args.F ? mx_gate_times(g[j], u, args.gate_alpha, args.gate_limit) : 0.f;
+  }
+  if ((lane & 4) == 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) largest = max(largest, mx_size(g[j]));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));  // a block: half the warp
+  const uint32_t s = mx_row_scale(largest);
+  const float over = mx_over(s);
+  const int fp = (args.F + MX_GROUP - 1) / MX_GROUP * MX_GROUP;
+  uint8_t* codes = reinterpret_cast<uint8_t*>(args.out) + (size_t)t * fp;
+  uint8_t* scales = args.out_scales + (size_t)t * (fp / MX_BLOCK);
+  if ((lane & 4) == 0) *reinterpret_cast<uint32_t*>(codes + f) = s == 255u ? 0u : mx_e4m3(g[0] * over, g[1] * over, g[2] * over, g[3] * over);
+  if ((lane & 15) == 0) scales[f / MX_BLOCK] = (uint8_t)s;
+  if (f0 + 64 < fp && f0 + 64 >= (args.N + 1) / 2) {  // the last tile fills half a group: the other half is zeros
+    if (lane < 16) *reinterpret_cast<uint32_t*>(codes + f0 + 64 + lane * 4) = 0u;
+    if (lane < 2) scales[(f0 + 64) / MX_BLOCK + lane] = 0;
+  }
+}
+
+// The same four rows of a product that is stored.
+__device__ __forceinline__ void few_stored_token(const MxArgs& args, float4 v, int t, int f) {
+  const size_t at = (size_t)t * args.N + f;
+  if (args.wide && f + 4 <= args.N) {
+    if (args.bias) {
+      const float4 b = *reinterpret_cast<const float4*>(args.bias + f);
+      v.x += b.x, v.y += b.y, v.z += b.z, v.w += b.w;
+    }
+    if (args.add) {
+      const float4 a = *reinterpret_cast<const float4*>(args.add + at);
+      v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+    }
+    if (args.out_bf16) {
+      __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+      *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(args.out) + at) = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+    } else {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(args.out) + at) = v;
+    }
+    return;
+  }
+  const float y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (f + j >= args.N) break;
+    float z = y[j] + (args.bias ? args.bias[f + j] : 0.f);
+    if (args.add) z += args.add[at + j];
+    if (args.out_bf16) reinterpret_cast<bf16*>(args.out)[at + j] = __float2bfloat16_rn(z);
+    else reinterpret_cast<float*>(args.out)[at + j] = z;
+  }
+}
+
 template <int BN>
-__global__ void __launch_bounds__(MX_THREADS, BN == 256 ? 1 : 2) mx_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const MxArgs args) {
-  using Tile = MxTile<BN>;
+__global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_constant__ CUtensorMap map_x, const MxArgs args, const int parts) {
+  using Tile = FewTile<BN>;
   constexpr int STAGES = Tile::STAGES, AHEAD = STAGES - 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -91,8 +205,10 @@ __global__ void __launch_bounds__(MX_THREADS, BN == 256 ? 1 : 2) mx_gemm_kernel(
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int f0 = blockIdx.x * MX_TILE_ROWS, t0 = blockIdx.y * BN;
-  const int first = blockIdx.z * args.per_split, n = min(args.slices, first + args.per_split) - first;
+  const int part = blockIdx.x % parts, f_tile = blockIdx.x / parts;  // a cluster: the parts of one tile's depth
+  const int f0 = f_tile * MX_TILE_ROWS, t0 = blockIdx.y * BN;
+  // parts that differ by one slice at most
+  const int first = (int)((long long)args.slices * part / parts), n = (int)((long long)args.slices * (part + 1) / parts) - first;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
@@ -110,17 +226,14 @@ __global__ void __launch_bounds__(MX_THREADS, BN == 256 ? 1 : 2) mx_gemm_kernel(
   const uint32_t tmem = tmem_base_smem;
 
   if (warp < 4) {
-    const uint8_t* src = args.tiles + ((size_t)blockIdx.x * args.slices + first) * MX_TILE_BYTES;
-    const int row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
-    const uint32_t to = (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));  // rows 16 apart: the same place in their groups of 8
+    const uint8_t* src = args.tiles + ((size_t)f_tile * args.slices + first) * MX_TILE_BYTES;
     int i = 0;
     for (; i < n; ++i) {
       const int s = i % STAGES;
       if (i >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(i / STAGES - 1) & 1u, &abort_flag)) break;
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES;
       const uint8_t* from = src + (size_t)i * MX_TILE_BYTES;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) copy8(stage + to + j * 16 * 128, from + j * 1024 + threadIdx.x * 8);
+      load_weight_tile(stage, from, threadIdx.x);
       if (threadIdx.x < 32) copy16(stage + Tile::A_BYTES + Tile::B_BYTES + threadIdx.x * 16, from + MX_TILE_CODES + threadIdx.x * 16);
       copies_end_group();
       if (i >= AHEAD) {
@@ -135,7 +248,7 @@ __global__ void __launch_bounds__(MX_THREADS, BN == 256 ? 1 : 2) mx_gemm_kernel(
       mbar_arrive(&weights_in[j % STAGES]);
     }
   } else if (warp == 4) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_wait();
     pdl_launch();
     const int row_bytes = 4 * args.slices;
     int i = 0;
@@ -145,14 +258,12 @@ __global__ void __launch_bounds__(MX_THREADS, BN == 256 ? 1 : 2) mx_gemm_kernel(
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES + 512;
       if (lane == 0) {
         mbar_expect_tx(&tokens_in[s], Tile::B_BYTES);
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(stage + Tile::A_BYTES), "l"(&map_x),
-                     "r"(smem_u32(&tokens_in[s])), "r"((first + i) * MX_GROUP), "r"(t0)
-                     : "memory");
+        load_tokens(stage + Tile::A_BYTES, &map_x, &tokens_in[s], (first + i) * MX_GROUP, t0);
       }
 #pragma unroll
       for (int r = 0; r < BN; r += 32) {
         const int t = r + lane;
-        if (t < BN && t0 + t < args.T) copy4(scales + (uint32_t)((t >> 7) * 512 + mx_scale_at(t & 127, 0)), args.x_scales + (size_t)(t0 + t) * row_bytes + 4 * (first + i));
+        if (t < BN && t0 + t < args.T) copy4(scales + (uint32_t)mx_scale_at(t, 0), args.x_scales + (size_t)(t0 + t) * row_bytes + 4 * (first + i));
       }
       copies_end_group();
       if (i >= AHEAD) {
@@ -166,87 +277,367 @@ __global__ void __launch_bounds__(MX_THREADS, BN == 256 ? 1 : 2) mx_gemm_kernel(
       fence_to_tensor_core();
       mbar_arrive(&tokens_in[j % STAGES]);
     }
-    // every slice asked for has its arrivals now: what is still in flight lands in a bounded time
     if (*(volatile int*)&abort_flag)
-      for (int j = max(0, i - STAGES); j < i; ++j)
-        for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(&tokens_in[j % STAGES], (uint32_t)(j / STAGES) & 1u); ++w) {
-        }
+      for (int j = max(0, i - STAGES); j < i; ++j) drain(&tokens_in[j % STAGES], (uint32_t)(j / STAGES) & 1u);
   } else if (lane == 0) {
     bool ok = true;
-    for (int i = 0; i < n && ok; ++i) {
+    for (int i = 0; i < n; ++i) {
       const int s = i % STAGES;
       const uint32_t parity = (uint32_t)(i / STAGES) & 1u;
       ok = mbar_wait(&weights_in[s], parity, &abort_flag) && mbar_wait(&tokens_in[s], parity, &abort_flag);
       if (!ok) break;
       tc_fence_after();
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES;
-      const uint32_t scale_a = tmem + BN + s * Tile::SCALE_COLS, scale_b = scale_a + 4;
+      const uint32_t scale_a = tmem + BN + s * 8, scale_b = scale_a + 4;
       scales_to_tmem(scale_a, scales);
-#pragma unroll
-      for (int a = 0; a < Tile::B_ATOMS; ++a) scales_to_tmem(scale_b + 4 * a, scales + 512 + 512 * a);
+      scales_to_tmem(scale_b, scales + 512);
       const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + Tile::A_BYTES);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) umma_mx(tmem, a + 2 * j, b + 2 * j, mx_idesc(BN, j), scale_a, scale_b, (i | j) ? 1u : 0u);
+      for (int j = 0; j < 4; ++j) umma_mx(tmem, a + 2 * j, b + 2 * j, mx_idesc(E2M1, E4M3, 128, BN, j), scale_a, scale_b, (i | j) ? 1u : 0u);
       umma_commit(&stage_free[s]);
     }
     umma_commit(&sums_done);
-    if (!ok)  // the products issued so far end before tensor memory is given back
-      for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(&sums_done, 0); ++w) {
-      }
+    if (!ok) drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
   }
   __syncwarp();
 
+  const int live = min(BN, args.T - t0);
   if (warp < 4) {
-    if (mbar_wait(&sums_done, 0, &abort_flag) && !*(volatile int*)&abort_flag) {
-      tc_fence_after();
-      const int f = f0 + warp * 32 + lane;
-      const bool live = f < args.N;
-      asm volatile("griddepcontrol.wait;" ::: "memory");  // what is written here, an earlier kernel may still read
-      const float bias = live && args.bias ? args.bias[f] : 0.f;
-      for (int c = 0; c < BN && t0 + c < args.T; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c, r);
-        tmem_ld_wait();
-        if (!live) continue;
+    const bool good = mbar_wait(&sums_done, 0, &abort_flag) && !*(volatile int*)&abort_flag;
+    tc_fence_after();
+    if (!good && threadIdx.x == 0 && args.status) atomicExch(args.status, 2);
+    const uint32_t mine = tiles + (uint32_t)(warp * 32 + lane) * 4;
+    for (int c = 0; c < live; c += 16) {
+      uint32_t r[16];
+      tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c, r);
+      tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int t = t0 + c + j;
-          if (t >= args.T) break;
-          const size_t at = (size_t)t * args.N + f;
-          float v = __uint_as_float(r[j]);
-          if (args.partial) {
-            args.partial[(size_t)blockIdx.z * args.T * args.N + at] = v;
-            continue;
-          }
-          v += bias;
-          if (args.add) v += args.add[at];
-          if (args.out_bf16) reinterpret_cast<bf16*>(args.out)[at] = __float2bfloat16_rn(v);
-          else reinterpret_cast<float*>(args.out)[at] = v;
-        }
-      }
-    } else if (threadIdx.x == 0 && args.status) {
-      atomicExch(args.status, 1);
+      for (int j = 0; j < 16; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + (uint32_t)((c + j) * SUM_PITCH * 4)), "f"(good ? __uint_as_float(r[j]) : __uint_as_float(0x7fc00000u)) : "memory");
     }
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == 5) tmem_dealloc(tmem, Tile::TMEM_COLS);
+  __syncwarp();
+  if (parts > 1) cluster_sync_all();
+  else __syncthreads();
+  pdl_wait();  // what is written now, an earlier kernel may have been reading
+  for (int t = part + parts * warp; t < live; t += parts * (FEW_THREADS / 32)) {
+    const uint32_t local = tiles + (uint32_t)(t * SUM_PITCH + lane * 4) * 4;
+    float4 v[FEW_PARTS];
+#pragma unroll
+    for (int z = 0; z < FEW_PARTS; ++z) {
+      v[z] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (z < parts) {
+        if (parts > 1) {
+          uint32_t there;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(local), "r"(z));
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[z].x), "=f"(v[z].y), "=f"(v[z].z), "=f"(v[z].w) : "r"(there) : "memory");
+        } else {
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[z].x), "=f"(v[z].y), "=f"(v[z].z), "=f"(v[z].w) : "r"(local) : "memory");
+        }
+      }
+    }
+#pragma unroll
+    for (int z = 1; z < FEW_PARTS; ++z)
+      if (z < parts) v[0].x += v[z].x, v[0].y += v[z].y, v[0].z += v[z].z, v[0].w += v[z].w;
+    if (args.F) few_gated_token(args, v[0], t0 + t, f_tile * (MX_TILE_ROWS / 2), lane);
+    else few_stored_token(args, v[0], t0 + t, f0 + lane * 4);
+  }
+  if (parts > 1) cluster_sync_all();  // nobody leaves while its sums are read
+  else __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Tile::TMEM_COLS);
+  }
 }
 
-// The sums of a depth's parts, in their order.
-template <typename T>
-__global__ void __launch_bounds__(256) mx_join_kernel(T* __restrict__ out, const float* __restrict__ partial, const float* __restrict__ bias, const float* __restrict__ add, long long count, int n, int splits) {
-  pdl_wait();
-  pdl_launch();
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= count) return;
-  float v = 0.f;
-  for (int z = 0; z < splits; ++z) v += partial[z * count + i];
-  if (bias) v += bias[i % n];
-  if (add) v += add[i];
-  out[i] = from_f<T>(v);
+// ---------------------------------------------------------------------------
+// Prompts.  A pair of CTAs (a cluster of two, one CTA an SM) works through tiles of 256 tokens and 256 rows of
+// the weight with products of M = 256 that the first CTA issues for both: each CTA fetches its own 128 tokens and
+// its own 128 rows, 25 KB a k-slice for 512 clocks of the tensor cores, about what an SM can pull out of L2.  The
+// scales of all 256 rows stand in both CTAs' tensor memory, those of its own tokens in each.
+//
+// Tensor memory holds 512 columns: two accumulators of 256 and the scales do not fit.  The accumulators therefore
+// share 32 columns (0-255 and 224-479), and the epilogue takes the block that holds them first: the next tile's
+// products begin when it has those in registers, and run beside the rest of the epilogue.
+// ---------------------------------------------------------------------------
+constexpr int PAIR_THREADS = 448;  // warps 0-3 weights, 4 tokens, 5 products (second CTA: tells the first what has landed), 6-13 epilogue
+constexpr int PAIR_STAGES = 6;
+constexpr uint32_t PAIR_STAGE_BYTES = 2 * 128 * MX_GROUP + 2048;  // tokens, weight rows, 512 bytes of the tokens' scales, 1,024 of the weight's
+constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 1024;
+constexpr uint32_t PAIR_SECOND = 224, PAIR_SCALES = 480;  // columns of the second accumulator, of two places of 12 for scales
+
+__device__ __forceinline__ void pair_load64(uint32_t tmem, uint32_t (&r)[64]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t q[16];
+    tmem_ld16(tmem + j * 16, q);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[j * 16 + i] = q[i];
+  }
+  tmem_ld_wait();
 }
 
+// 64 rows' sums of one token: stored, or (two features' rows for each) one block of codes and its scale.
+__device__ __forceinline__ void pair_finish64(const MxArgs& args, const uint32_t (&r)[64], int t, int row, bool good) {
+  const float nan = __uint_as_float(0x7fc00000u);
+  if (args.F) {
+    const int f = row / 2, fp = (args.F + MX_GROUP - 1) / MX_GROUP * MX_GROUP;
+    if (f >= fp) return;
+    float v[32];
+    uint32_t largest = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const int at = (j / 16) * 32 + j % 16;
+      float y = mx_gate_times(__uint_as_float(r[at]), __uint_as_float(r[at + 16]), args.gate_alpha, args.gate_limit);
+      y = good ? y : nan;
+      v[j] = f + j < args.F ? y : 0.f;
+      largest = max(largest, mx_size(v[j]));
+    }
+    const uint32_t s = mx_row_scale(largest);
+    const float over = mx_over(s);
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = s == 255u ? 0u : mx_e4m3(v[4 * j] * over, v[4 * j + 1] * over, v[4 * j + 2] * over, v[4 * j + 3] * over);
+    uint4* codes = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(args.out) + (size_t)t * fp + f);
+    codes[0] = make_uint4(c[0], c[1], c[2], c[3]);
+    codes[1] = make_uint4(c[4], c[5], c[6], c[7]);
+    args.out_scales[(size_t)t * (fp / MX_BLOCK) + f / MX_BLOCK] = (uint8_t)s;
+    return;
+  }
+  const size_t at = (size_t)t * args.N + row;
+#pragma unroll
+  for (int j = 0; j < 64; j += 8) {
+    const int f = row + j;
+    if (f >= args.N) break;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = good ? __uint_as_float(r[j + i]) : nan;
+    if (args.wide && f + 8 <= args.N) {
+      if (args.bias) {
+        const float4 a = *reinterpret_cast<const float4*>(args.bias + f), b = *reinterpret_cast<const float4*>(args.bias + f + 4);
+        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+      }
+      if (args.add) {
+        const float4 a = *reinterpret_cast<const float4*>(args.add + at + j), b = *reinterpret_cast<const float4*>(args.add + at + j + 4);
+        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+      }
+      if (args.out_bf16) {
+        uint4 p;
+        __nv_bfloat162 h0 = __floats2bfloat162_rn(v[0], v[1]), h1 = __floats2bfloat162_rn(v[2], v[3]), h2 = __floats2bfloat162_rn(v[4], v[5]), h3 = __floats2bfloat162_rn(v[6], v[7]);
+        p.x = *reinterpret_cast<uint32_t*>(&h0), p.y = *reinterpret_cast<uint32_t*>(&h1), p.z = *reinterpret_cast<uint32_t*>(&h2), p.w = *reinterpret_cast<uint32_t*>(&h3);
+        bf16* dst = reinterpret_cast<bf16*>(args.out) + at + j;
+        if (args.N % 8 == 0) {
+          *reinterpret_cast<uint4*>(dst) = p;
+        } else {
+          reinterpret_cast<uint2*>(dst)[0] = make_uint2(p.x, p.y);
+          reinterpret_cast<uint2*>(dst)[1] = make_uint2(p.z, p.w);
+        }
+      } else {
+        float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(args.out) + at + j);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (f + i >= args.N) break;
+      float z = v[i] + (args.bias ? args.bias[f + i] : 0.f);
+      if (args.add) z += args.add[at + j + i];
+      if (args.out_bf16) reinterpret_cast<bf16*>(args.out)[at + j + i] = __float2bfloat16_rn(z);
+      else reinterpret_cast<float*>(args.out)[at + j + i] = z;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const MxArgs args) {
+  constexpr int STAGES = PAIR_STAGES, AHEAD = STAGES - 1;
+  constexpr uint32_t A_BYTES = 128 * MX_GROUP, B_BYTES = 128 * MX_GROUP;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  // landed: this CTA's own copies of a slice; peer_landed (first CTA): the second one's; sums_ready, sums_taken: a tile's accumulator
+  __shared__ uint64_t landed[STAGES], peer_landed[STAGES], stage_free[STAGES], sums_ready, sums_taken, gave_up;
+  __shared__ uint32_t tmem_base_smem;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_in_cluster();
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, slices = args.slices;
+  const int f_tiles = (args.N + 255) / 256, n_tiles = f_tiles * ((args.T + 255) / 256);  // the weight's tiles innermost
+  const int last_weight_tile = (args.N + MX_TILE_ROWS - 1) / MX_TILE_ROWS - 1;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&landed[s], 128 + 32 + 1);
+      mbar_init(&peer_landed[s], 1);
+      mbar_init(&stage_free[s], 1);
+    }
+    mbar_init(&sums_ready, 1);
+    mbar_init(&sums_taken, 16);  // the epilogue warps of both CTAs
+    mbar_init(&gave_up, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 5) tmem_alloc_pair(&tmem_base_smem, 512);
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers stand before either signals the other's
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_smem;
+
+  if (warp < 4) {
+    int it = 0;  // slices asked for so far, over all tiles
+    auto tell = [&](int j) {
+      fence_to_tensor_core();
+      mbar_arrive(&landed[j % STAGES]);
+    };
+    bool ok = true;
+    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+      const int first_tile = (tile % f_tiles) * 2;
+      // a row count that is no multiple of 256 leaves the second CTA without rows: it reads the last ones, and what comes of them is not stored
+      const uint8_t* mine = args.tiles + (size_t)min(first_tile + (int)rank, last_weight_tile) * slices * MX_TILE_BYTES;
+      const uint8_t* scales = args.tiles + (size_t)min(first_tile + (int)(threadIdx.x >> 5 & 1), last_weight_tile) * slices * MX_TILE_BYTES + MX_TILE_CODES + lane * 16;
+      for (int i = 0; i < slices; ++i, ++it) {
+        const int s = it % STAGES;
+        if (it >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(it / STAGES - 1) & 1u, &abort_flag)) {
+          ok = false;
+          break;
+        }
+        const uint32_t stage = tiles + s * PAIR_STAGE_BYTES;
+        load_weight_tile(stage + A_BYTES, mine + (size_t)i * MX_TILE_BYTES, threadIdx.x);
+        if (threadIdx.x < 64) copy16(stage + A_BYTES + B_BYTES + 512 + threadIdx.x * 16, scales + (size_t)i * MX_TILE_BYTES);
+        copies_end_group();
+        if (it >= AHEAD) {
+          copies_wait<AHEAD>();
+          tell(it - AHEAD);
+        }
+      }
+    }
+    for (int j = max(0, it - AHEAD); j < it; ++j) {
+      copies_wait_but(it - 1 - j);
+      tell(j);
+    }
+  } else if (warp == 4) {
+    pdl_wait();
+    pdl_launch();
+    const int row_bytes = 4 * slices;
+    int it = 0;
+    bool ok = true;
+    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+      const int t0 = tile / f_tiles * 256 + (int)rank * 128;
+      for (int i = 0; i < slices; ++i, ++it) {
+        const int s = it % STAGES;
+        if (it >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(it / STAGES - 1) & 1u, &abort_flag)) {
+          ok = false;
+          break;
+        }
+        const uint32_t stage = tiles + s * PAIR_STAGE_BYTES;
+        if (lane == 0) {
+          mbar_expect_tx(&landed[s], A_BYTES);
+          load_tokens(stage, &map_x, &landed[s], i * MX_GROUP, t0);
+        }
+#pragma unroll
+        for (int r = 0; r < 128; r += 32)
+          if (t0 + r + lane < args.T) copy4(stage + A_BYTES + B_BYTES + (uint32_t)mx_scale_at(r + lane, 0), args.x_scales + (size_t)(t0 + r + lane) * row_bytes + 4 * i);
+        copies_end_group();
+        if (it >= AHEAD) {
+          copies_wait<AHEAD>();
+          fence_to_tensor_core();
+          mbar_arrive(&landed[(it - AHEAD) % STAGES]);
+        }
+      }
+    }
+    for (int j = max(0, it - AHEAD); j < it; ++j) {
+      copies_wait_but(it - 1 - j);
+      fence_to_tensor_core();
+      mbar_arrive(&landed[j % STAGES]);
+    }
+    if (*(volatile int*)&abort_flag)
+      for (int j = max(0, it - STAGES); j < it; ++j) drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+  } else if (warp == 5) {
+    if (lane == 0 && rank == 1) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs)
+        for (int i = 0; i < slices; ++i, ++it) {
+          ok = mbar_wait(&landed[it % STAGES], (uint32_t)(it / STAGES) & 1u, &abort_flag);
+          if (!ok) break;
+          mbar_arrive_in_cluster(in_cluster_cta(&peer_landed[it % STAGES], 0));
+        }
+    } else if (lane == 0) {
+      int it = 0, done = 0;  // slices consumed, tiles begun
+      bool ok = true;
+      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs, ++done) {
+        if (done) ok = mbar_wait_in_cluster(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sums = tmem + (done & 1 ? PAIR_SECOND : 0);
+        for (int i = 0; i < slices; ++i, ++it) {
+          const int s = it % STAGES;
+          const uint32_t parity = (uint32_t)(it / STAGES) & 1u;
+          ok = mbar_wait(&landed[s], parity, &abort_flag) && mbar_wait_in_cluster(&peer_landed[s], parity, &abort_flag);
+          // the scales' two places take turns: the products of the slice before last are complete
+          if (ok && it >= 2) ok = mbar_wait(&stage_free[(it - 2) % STAGES], (uint32_t)((it - 2) / STAGES) & 1u, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES;
+          const uint32_t scale_a = tmem + PAIR_SCALES + (it & 1) * 12, scale_b = scale_a + 4;
+          scales_to_tmem_pair(scale_a, scales);
+          scales_to_tmem_pair(scale_b, scales + 512);
+          scales_to_tmem_pair(scale_b + 4, scales + 1024);
+          const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + A_BYTES);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) umma_mx_pair(sums, a + 2 * j, b + 2 * j, mx_idesc(E4M3, E2M1, 256, 256, j), scale_a, scale_b, (i | j) ? 1u : 0u);
+          umma_commit_pair(&stage_free[s], 3);
+        }
+        if (ok) umma_commit_pair(&sums_ready, 3);
+      }
+      if (!ok) {  // the products issued so far end before tensor memory is given back
+        umma_commit_pair(&gave_up, 3);
+        drain(&gave_up, 0);
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 6) >> 2;  // a quarter of the lanes (warps read 32 (w % 4) and on), half of the columns
+    pdl_wait();  // what is written here, an earlier kernel may have been reading
+    const uint32_t taken = in_cluster_cta(&sums_taken, 0);
+    bool good = true;
+    int done = 0;
+    for (int tile = pair; tile < n_tiles; tile += n_pairs, ++done) {
+      const int row0 = (tile % f_tiles) * 256 + half * 128, t = tile / f_tiles * 256 + (int)rank * 128 + q * 32 + lane;
+      good = good && __all_sync(0xffffffffu, mbar_wait(&sums_ready, (uint32_t)done & 1u, &abort_flag));
+      tc_fence_after();
+      const bool second = done & 1, shared_half = half == (second ? 0 : 1);  // the shared columns: the first tile's last, the second's first
+      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (second ? PAIR_SECOND : 0) + half * 128;
+      if (!shared_half) {  // this half's columns are no part of the next tile's accumulator
+        if (lane == 0) mbar_arrive_in_cluster(taken);
+      }
+#pragma unroll 1
+      for (int k = 0; k < 2; ++k) {
+        const int block = second ? k : 1 - k;  // the block with the shared columns first
+        uint32_t r[64];
+        pair_load64(at + block * 64, r);
+        if (k == 0 && shared_half) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_in_cluster(taken);
+        }
+        if (t < args.T) pair_finish64(args, r, t, row0 + block * 64, good);
+      }
+      tc_fence_before();
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA leaves, or frees tensor memory, while the other may still signal or read it
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+  if (threadIdx.x == 0 && abort_flag && args.status) atomicExch(args.status, 2);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
 static bool make_rows_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t bytes, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
@@ -264,52 +655,51 @@ static bool allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& d
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   if (done.load(std::memory_order_relaxed) & bit) return true;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
   done.fetch_or(bit, std::memory_order_relaxed);
   return true;
 }
-template <int BN> static std::atomic<uint64_t> configured{0};
+template <int BN> static std::atomic<uint64_t> few_allowed{0};
+static std::atomic<uint64_t> pair_allowed{0};
 
 template <int BN>
-static int launch_mx(const CUtensorMap& map, const MxArgs& args, int splits, cudaStream_t stream) {
-  const long long tall = ((long long)args.N + MX_TILE_ROWS - 1) / MX_TILE_ROWS, wide = ((long long)args.T + BN - 1) / BN;
-  if (tall > 0x7fffffffll || wide > 65535 || splits > 65535) return ALOFA_ERR_ARGUMENT;
-  if (!allow_shared((const void*)mx_gemm_kernel<BN>, (int)MxTile<BN>::SMEM, configured<BN>)) return ALOFA_ERR_LAUNCH;
-  launch_dep(mx_gemm_kernel<BN>, dim3((unsigned)tall, (unsigned)wide, (unsigned)splits), MX_THREADS, MxTile<BN>::SMEM, stream, map, args);
+static int launch_few(const CUtensorMap& map, const MxArgs& args, int parts, cudaStream_t stream) {
+  const long long wide = (((long long)args.N + MX_TILE_ROWS - 1) / MX_TILE_ROWS) * parts, tall = ((long long)args.T + BN - 1) / BN;
+  if (wide > 0x7fffffffll || tall > 65535) return ALOFA_ERR_ARGUMENT;
+  if (!allow_shared((const void*)mx_few_kernel<BN>, (int)FewTile<BN>::SMEM, few_allowed<BN>)) return ALOFA_ERR_LAUNCH;
+  launch_dep_cluster(mx_few_kernel<BN>, dim3((unsigned)wide, (unsigned)tall), FEW_THREADS, FewTile<BN>::SMEM, stream, parts, map, args, parts);
   return launch_status();
 }
 
-// How many parts a depth of k really goes in when `splits` are asked for (every part has a slice).
-ALOFA_API int alofa_mx_splits(int k, int splits) {
-  const int slices = (k + MX_GROUP - 1) / MX_GROUP, per = (slices + splits - 1) / splits;
-  return (slices + per - 1) / per;
-}
-
-// partial: [splits, T, N] for splits > 1; leave: the sums of the parts are the result, nothing is joined.
-ALOFA_API int alofa_mx_gemm(void* out, float* partial, const void* x_codes, const void* x_scales, const void* tiles, const float* bias, const float* add, int t, int n, int k, int bn, int splits,
-                            int leave, int out_bf16, int* status, void* stream) {
-  if (t < 0 || n <= 0 || k <= 0 || k > (1 << 30) || splits < 1 || (uintptr_t)x_codes % 16 || (uintptr_t)x_scales % 4 || (uintptr_t)tiles % 16) return ALOFA_ERR_ARGUMENT;
+// bn: 256: pairs of CTAs (`parts` 1, a grid of `ctas` of them); 16, 32, 64 or 128 tokens a CTA, the depth in `parts` parts.
+// features > 0: out are the codes and out_scales the scales of that many gated features, n the rows of the gated weight.
+ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, const void* x_scales, const void* tiles, const float* bias, const float* add, int t, int n, int k, int features,
+                            float gate_alpha, float gate_limit, int bn, int parts, int ctas, int out_bf16, int* status, void* stream) {
+  if (t < 0 || n <= 0 || k <= 0 || k > (1 << 30) || n > (1 << 30) || (uintptr_t)x_codes % 16 || (uintptr_t)x_scales % 4 || (uintptr_t)tiles % 16) return ALOFA_ERR_ARGUMENT;
+  if (features < 0 || (features && (n != 2 * ((features + 15) / 16 * 16) || !out_scales || (uintptr_t)out % 16))) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
-  const int slices = (k + MX_GROUP - 1) / MX_GROUP;
-  if (splits > slices || alofa_mx_splits(k, splits) != splits || ((splits > 1 || leave) && !partial)) return ALOFA_ERR_ARGUMENT;
   MxArgs args = {};
   args.tiles = (const uint8_t*)tiles, args.x_scales = (const uint8_t*)x_scales;
-  args.out = out, args.bias = bias, args.add = add, args.partial = splits > 1 || leave ? partial : nullptr;
-  args.T = t, args.N = n, args.slices = slices, args.per_split = (slices + splits - 1) / splits, args.out_bf16 = out_bf16, args.status = status;
+  args.out = out, args.out_scales = (uint8_t*)out_scales, args.bias = bias, args.add = add;
+  args.T = t, args.N = n, args.slices = (k + MX_GROUP - 1) / MX_GROUP, args.F = features, args.out_bf16 = out_bf16, args.status = status;
+  args.gate_alpha = gate_alpha, args.gate_limit = gate_limit;
+  args.wide = n % 4 == 0 && ((uintptr_t)out | (uintptr_t)bias | (uintptr_t)add) % 16 == 0;
+  const bool few = bn == 16 || bn == 32 || bn == 64 || bn == 128;
+  if (!few && bn != 256) return ALOFA_ERR_ARGUMENT;
+  if (parts < 1 || parts > args.slices || parts > (few ? FEW_PARTS : 1)) return ALOFA_ERR_ARGUMENT;
   CUtensorMap map;
-  if (!make_rows_map(&map, x_codes, (uint64_t)t, (uint64_t)slices * MX_GROUP, bn)) return ALOFA_ERR_ARGUMENT;
+  if (!make_rows_map(&map, x_codes, (uint64_t)t, (uint64_t)args.slices * MX_GROUP, few ? bn : 128)) return ALOFA_ERR_ARGUMENT;
   cudaStream_t s = (cudaStream_t)stream;
-  int rc = ALOFA_ERR_ARGUMENT;
   switch (bn) {
-    case 16: rc = launch_mx<16>(map, args, splits, s); break;
-    case 32: rc = launch_mx<32>(map, args, splits, s); break;
-    case 64: rc = launch_mx<64>(map, args, splits, s); break;
-    case 128: rc = launch_mx<128>(map, args, splits, s); break;
-    case 256: rc = launch_mx<256>(map, args, splits, s); break;
+    case 16: return launch_few<16>(map, args, parts, s);
+    case 32: return launch_few<32>(map, args, parts, s);
+    case 64: return launch_few<64>(map, args, parts, s);
+    case 128: return launch_few<128>(map, args, parts, s);
   }
-  if (rc || leave || splits == 1) return rc;
-  const long long count = (long long)t * n, blocks = (count + 255) / 256;
-  if (blocks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
-  if (out_bf16) launch_dep(mx_join_kernel<bf16>, (unsigned)blocks, 256, 0, s, (bf16*)out, (const float*)partial, bias, add, count, n, splits);
-  else launch_dep(mx_join_kernel<float>, (unsigned)blocks, 256, 0, s, (float*)out, (const float*)partial, bias, add, count, n, splits);
+  const long long pair_tiles = (((long long)n + 255) / 256) * (((long long)t + 255) / 256);
+  if (ctas < 2 || pair_tiles > 0x3fffffffll) return ALOFA_ERR_ARGUMENT;
+  if (!allow_shared((const void*)mx_pair_kernel, (int)PAIR_SMEM, pair_allowed)) return ALOFA_ERR_LAUNCH;
+  const long long grid = 2 * pair_tiles < ctas ? 2 * pair_tiles : ctas / 2 * 2;
+  launch_dep_cluster(mx_pair_kernel, dim3((unsigned)grid), PAIR_THREADS, PAIR_SMEM, s, 2, map, args);
   return launch_status();
 }

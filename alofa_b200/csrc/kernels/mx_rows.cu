@@ -1,7 +1,6 @@
 // What makes microscaled numbers (mx.cuh), and what turns them back:
 //   alofa_mx_rows        rows [T, K] in bf16 or fp32 -> E4M3 codes [T, Kp], scales [T, Kp / 32]
 //   alofa_mx_norm        h = base + sum_z owed[z] (+ bias); the RMSNorm (or layer norm) of h's rows as such rows
-//   alofa_mx_gate        the sums of a gated product, one per part of its depth, as rows of silu(g) * u
 //   alofa_mx_pack        a weight [N, K] in bf16 or fp32 -> tiles of E2M1 codes and scales
 //   alofa_mx_rows_values, alofa_mx_weight_values   the numbers that rows, or a weight, stand for
 // Kp is K rounded up to whole groups of 128; the codes behind K are zeros.
@@ -209,48 +208,6 @@ ALOFA_API int alofa_mx_norm(void* codes, void* scales, float* h, const float* ba
   else if (per <= 4) GO(4);
   else GO(8);
 #undef GO
-  return launch_status();
-}
-
-// ---------------------------------------------------------------------------
-// The gate: sums [splits, T, 2 F16] of a gated weight's rows (16 of the gate, the same 16 of the up
-// projection, and so on; F16 is F rounded up to 16), added in split order
-// (silu(gate) * up: src/alofa/kernels/cpu/scalar.mojo:208-231).
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) mx_gate_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const float* __restrict__ sums, int splits, int t, int f, int fp, float alpha, float limit) {
-  pdl_wait();
-  pdl_launch();
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int per_row = fp >> 3, f16 = (f + 15) / 16 * 16;
-  const bool live = i < (long long)t * per_row;
-  const long long row = live ? i / per_row : 0;
-  const int c = live ? (int)(i - row * per_row) * 8 : 0;
-  float g[8], u[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) g[j] = u[j] = 0.f;
-  if (live && c < f16) {
-    const float* src = sums + row * (2 * f16) + mx_gated_row(c, 0);
-    const size_t plane = (size_t)t * 2 * f16;
-    for (int z = 0; z < splits; ++z) {
-      float a[8], b[8];
-      load8(a, src + z * plane, 8, true);
-      load8(b, src + z * plane + MX_GATE_ROWS, 8, true);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] += a[j], u[j] += b[j];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) g[j] = c + j < f ? fast_gate_times(g[j], u[j], alpha, limit) : 0.f;
-  mx_put8(g, codes + row * fp + c, scales + row * (fp / MX_BLOCK) + c / MX_BLOCK, live);
-}
-
-ALOFA_API int alofa_mx_gate(void* codes, void* scales, const float* sums, int splits, int t, int f, float alpha, float limit, void* stream) {
-  if (t < 0 || f <= 0 || f > (1 << 29) || splits < 1 || !aligned(codes, 8) || !aligned(sums, 16)) return ALOFA_ERR_ARGUMENT;
-  if (t == 0) return ALOFA_OK;
-  const int fp = padded(f);
-  const long long blocks = ((long long)t * (fp / 8) + 255) / 256;
-  if (blocks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
-  launch_dep(mx_gate_kernel, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, sums, splits, t, f, fp, alpha, limit);
   return launch_status();
 }
 

@@ -1608,12 +1608,10 @@ def mx_library():
             "alofa_mx_rows": [_P, _P, _P, _I, _I, _I, _P],
             "alofa_mx_rows_values": [_P, _P, _P, _I, _I, _I, _P],
             "alofa_mx_norm": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _F, _P],
-            "alofa_mx_gate": [_P, _P, _P, _I, _I, _I, _F, _F, _P],
             "alofa_mx_pack": [_P, _P, _I, _I, _I, _I, _P],
             "alofa_mx_settle": [_P],
             "alofa_mx_weight_values": [_P, _P, _I, _I, _I, _I, _P],
-            "alofa_mx_splits": [_I, _I],
-            "alofa_mx_gemm": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+            "alofa_mx_gemm": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _I, _I, _I, _I, _P, _P],
         }
         for name, args in sigs.items():
             fn = getattr(lib, name)

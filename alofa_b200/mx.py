@@ -30,7 +30,8 @@ from .csrc import ops
 from .errors import AlofaError
 
 BLOCK, GROUP, TILE_ROWS, TILE_BYTES, GATE_ROWS = 32, 128, 128, 8704, 16  # as in kernels/mx.cuh
-TOKEN_TILES = (16, 32, 64, 128, 256)  # tokens that a CTA of the product may take
+TOKEN_TILES = (16, 32, 64, 128, 256)  # tokens that a CTA of the product may take, the last a pair of CTAs
+MOST_PARTS = 8  # of a depth
 MOST_WIDTH = 32768  # numbers of a row that the norm takes
 
 _BF16, _F32, _U8, _I32 = torch.bfloat16, torch.float32, torch.uint8, torch.int32
@@ -236,7 +237,7 @@ def norm_rows(h: torch.Tensor, weight: torch.Tensor, eps: float, base=None, owed
     all float32), in place, and the RMSNorm of its rows times ``weight`` in 8
     bits: ``h / sqrt(mean(h^2) + eps) * weight``.  With ``shift`` the layer
     norm, ``(h - mean) / sqrt(variance + eps) * weight + shift``.  ``owed
-    [splits, T, K]`` are the sums that a product left (:func:`linear_parts`)."""
+    [splits, T, K]`` are sums that products left, for parts of their depth or whole."""
     here = _here()
     at, t, k, bf16 = _matrix(h, "h", here)
     if bf16 or not k:
@@ -263,24 +264,40 @@ def _operands(x, w, what: str, gated: bool, here: int, buf) -> MxRows:
 
 
 _plans: dict = {}
+_SMS: dict = {}  # of a device
+
+
+def _sms(here: int) -> int:
+    if here not in _SMS:
+        _SMS[here] = torch.cuda.get_device_properties(here).multi_processor_count
+    return _SMS[here]
 
 
 def plan(tokens: int, rows: int, depth: int) -> tuple:
-    """(tokens a tile, parts of the depth) of a product."""
+    """(tokens a tile, parts of the depth) of a product; 256 tokens: pairs of CTAs."""
     key = (tokens, rows, depth)
     found = _plans.get(key)
     if found is None:
-        bn = next((b for b in TOKEN_TILES if tokens <= b), TOKEN_TILES[-1])
-        ctas = -(-rows // TILE_ROWS) * -(-tokens // bn)
-        room = 148 * (1 if bn == 256 else 2)
+        slices, sms = padded(depth) // GROUP, _sms(_here())
+        if tokens > 128:
+            found = (256, 1)
+        else:
+            bn = next(b for b in TOKEN_TILES if tokens <= b)
+            ctas = -(-rows // TILE_ROWS) * -(-tokens // bn)
+            found = (bn, max(1, min(MOST_PARTS, slices, 2 * sms // max(1, ctas))))
         if len(_plans) >= 4096:
             _plans.clear()
-        found = _plans[key] = (bn, ops.mx_library().alofa_mx_splits(depth, max(1, min(padded(depth) // GROUP, room // max(1, ctas)))))
+        _plans[key] = found
     return found
 
 
-def _sums(parts: int, t: int, rows: int, here: int, buf) -> torch.Tensor:
-    return torch.empty((parts, t, rows), dtype=_F32, device=here) if buf is None else buf((parts, t, rows), _F32)
+def _product(x: MxRows, w: MxWeight, out_at, scales_at, bias_at, add_at, features: int, gate, out_bf16, status, how, here: int, what: str) -> None:
+    bn, parts = how or plan(x.rows, w.rows, w.k)
+    status_at = None if status is None else _at(status, "status", _I32, status.shape, here)
+    rc = ops.mx_library().alofa_mx_gemm(
+        out_at, scales_at, x.codes_at, x.scales_at, w.at, bias_at, add_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16, status_at, _stream(here)
+    )
+    ops.mx_launched(rc, 1, what, lambda: f"tokens={x.rows} rows={w.rows} depth={w.k} how={(bn, parts)}")
 
 
 def linear(x, w: MxWeight, bias=None, add=None, out=None, dtype=None, buf=None, status=None, how: Optional[tuple] = None) -> torch.Tensor:
@@ -296,44 +313,25 @@ def linear(x, w: MxWeight, bias=None, add=None, out=None, dtype=None, buf=None, 
         dtype = dtype or (_BF16 if add is None else _F32)
         if dtype is not _BF16 and dtype is not _F32:
             raise AlofaError("unsupported", "a product is stored in bfloat16 or float32", f"dtype={dtype}")
-        out = torch.empty((t, n), dtype=dtype, device=here)
+        out = torch.empty((t, n), dtype=dtype, device=here) if buf is None else buf((t, n), dtype)
         out_at, out_bf16 = out.data_ptr(), dtype is _BF16
     else:
         out_at, rows, columns, out_bf16 = _matrix(out, "out", here)
         if rows != t or columns != n:
             _refuse(out, "out", f"({t}, {n})", here)
-    bn, parts = how or plan(t, w.rows, w.k)
-    partial = _sums(parts, t, n, here, buf) if parts > 1 else None
-    rc = ops.mx_library().alofa_mx_gemm(
-        out_at, None if partial is None else partial.data_ptr(), x.codes_at, x.scales_at, w.at, None if bias is None else _at(bias, "bias", _F32, (n,), here),
-        None if add is None else _at(add, "add", _F32, (t, n), here), t, n, w.k, bn, parts, 0, out_bf16, None if status is None else _at(status, "status", _I32, status.shape, here), _stream(here),
-    )
-    ops.mx_launched(rc, 1 if parts == 1 else 2, "linear", lambda: f"tokens={t} rows={n} depth={w.k} how={(bn, parts)}")
+    bias_at = None if bias is None else _at(bias, "bias", _F32, (n,), here)
+    add_at = None if add is None else _at(add, "add", _F32, (t, n), here)
+    _product(x, w, out_at, None, bias_at, add_at, 0, ops.SILU_GATE, out_bf16, status, how, here, "linear")
     return out
-
-
-def linear_parts(x, w: MxWeight, buf=None, status=None, how: Optional[tuple] = None, gated: bool = False) -> torch.Tensor:
-    """The sums of ``x w^T`` for each part of the depth, ``[parts, T, N]``
-    float32, for a reader that adds them (:func:`norm_rows`).  Of a ``gated``
-    weight: a column for each of its ``rows``."""
-    here = _here()
-    x = _operands(x, w, "linear_parts", gated, here, buf)
-    bn, parts = how or plan(x.rows, w.rows, w.k)
-    sums = _sums(parts, x.rows, w.rows, here, buf)
-    rc = ops.mx_library().alofa_mx_gemm(
-        None, sums.data_ptr(), x.codes_at, x.scales_at, w.at, None, None, x.rows, w.rows, w.k, bn, parts, 1, 0, None if status is None else _at(status, "status", _I32, status.shape, here), _stream(here),
-    )
-    ops.mx_launched(rc, 1, "linear_parts", lambda: f"tokens={x.rows} rows={w.rows} depth={w.k} how={(bn, parts)}")
-    return sums
 
 
 def gated_linear(x, w: MxWeight, gate=ops.SILU_GATE, buf=None, status=None, how: Optional[tuple] = None) -> MxRows:
     """``silu(x Wg^T) * (x Wu^T)`` as rows in 8 bits; ``gate`` = (alpha,
     limit): the clamped form ``g = min(g, limit), u = clamp(u, -limit, limit):
     g sigmoid(alpha g) (u + 1)``."""
-    sums = linear_parts(x, w, buf, status, how, gated=True)
-    here, (parts, t, _), f = w.device, sums.shape, w.n // 2
-    rows = MxRows._empty(t, f, here, buf)
-    rc = ops.mx_library().alofa_mx_gate(rows.codes_at, rows.scales_at, sums.data_ptr(), parts, t, f, gate[0], gate[1], _stream(here))
-    ops.mx_launched(rc, 1, "gated_linear", lambda: f"tokens={t} features={f}")
+    here = _here()
+    x = _operands(x, w, "gated_linear", True, here, buf)
+    features = w.n // 2
+    rows = MxRows._empty(x.rows, features, here, buf)
+    _product(x, w, rows.codes_at, rows.scales_at, None, None, features, gate, False, status, how, here, "gated_linear")
     return rows

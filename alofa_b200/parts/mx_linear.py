@@ -4,7 +4,7 @@
 A :class:`MxLinear` is called as a :class:`~alofa_b200.parts.linear.Linear` is.
 The weight is packed when the part loads.  Rows come in 8 bits from the norm in
 front (:class:`~alofa_b200.mx.MxRows`); any other rows are made so first.  A
-product in parts of its depth leaves their sums to a consumer that asks
+product into the residual stream leaves its sums to a consumer that asks
 (``defer``), as the bfloat16 products do."""
 from __future__ import annotations
 
@@ -31,7 +31,7 @@ class MxLinear:
             raise AlofaError("unsupported", "a gated product with weights in 4 bits takes no bias")
 
     def can_accumulate(self, tokens: int) -> bool:
-        return False  # its parts are added by the norm that reads the stream next
+        return False  # its sums are added by the norm that reads the stream next
 
     def _rows(self, x, buf):
         if isinstance(x, mx.MxRows):
@@ -40,9 +40,9 @@ class MxLinear:
 
     def __call__(self, out, x, defer: bool = False, buf=None):
         x = self._rows(x, buf)
-        if defer and (self.epi == RESIDUAL or mx.plan(x.rows, self.weight.rows, self.weight.k)[1] > 1):
-            sums = mx.linear_parts(x, self.weight, buf)
-            return Partial(sums, sums.shape[0], self.bias)
+        if defer and self.epi == RESIDUAL:
+            y = mx.linear(x, self.weight, dtype=torch.float32, buf=buf)
+            return Partial(y.view(1, *y.shape), 1, self.bias)  # the norm that reads the stream next adds it
         mx.linear(x, self.weight, bias=self.bias, add=out if self.epi == RESIDUAL else None, out=out, buf=buf)
         return None
 

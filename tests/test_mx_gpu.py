@@ -185,16 +185,35 @@ def test_linear(t, n, k):
     assert got is h and (np.abs(host(h) - full) <= loose + 2.0**-22 * (np.abs(want) + np.abs(bias.numpy()) + np.abs(add.numpy()))).all()
 
 
-@pytest.mark.parametrize("bn", mx.TOKEN_TILES)
-@pytest.mark.parametrize("asked", [1, 2, 3, 5, 100])
-def test_every_tile_and_part(bn, asked):
-    t, n, k = 70, 200, 1100
+HOWS = [(bn, parts) for bn in (16, 32, 64, 128) for parts in (1, 2, 3, 5, 8)] + [(256, 1)]
+
+
+@pytest.mark.parametrize("how", HOWS)
+@pytest.mark.parametrize("t,n,k", [(70, 200, 1100), (300, 520, 1024), (9, 640, 2000)])
+def test_every_tile_and_part(how, t, n, k):
     xr, wp, xv, wv = product_operands(t, n, k, 20)
-    parts = ops.mx_library().alofa_mx_splits(k, min(asked, mx.padded(k) // 128))
-    out = mx.linear(xr, wp, dtype=F32, how=(bn, parts))
-    assert (np.abs(host(out) - xv @ wv.T) <= sum_bound(xv, wv)).all()
-    left = mx.linear_parts(xr, wp, how=(bn, parts))
-    assert left.shape == (parts, t, n) and (np.abs(host(left).astype(np.float64).sum(0) - xv @ wv.T) <= sum_bound(xv, wv)).all()
+    want, loose = xv @ wv.T, sum_bound(xv, wv)
+    assert (np.abs(host(mx.linear(xr, wp, dtype=F32, how=how)) - want) <= loose).all()
+    bias, add = torch.randn(n), torch.randn(t, n)
+    full, size = want + bias.double().numpy() + add.double().numpy(), np.abs(want) + np.abs(bias.numpy()) + np.abs(add.numpy())
+    got = mx.linear(xr, wp, bias=bias.cuda(), add=add.cuda(), dtype=BF16, how=how)
+    assert (np.abs(host(got.float()) - full) <= 1.01 * loose + 2.0**-8 * np.abs(full) + 2.0**-22 * size).all()
+
+
+@pytest.mark.parametrize("t,n,k", [(2100, 8000, 128), (1030, 10500, 384)])
+def test_many_tiles_a_pair(t, n, k):
+    """More tiles than pairs of CTAs: accumulators that share columns, a ring that runs on from tile to tile."""
+    xr, wp, xv, wv = product_operands(t, n, k, 50)
+    assert (np.abs(host(mx.linear(xr, wp, dtype=F32, how=(256, 1))) - xv @ wv.T) <= sum_bound(xv, wv)).all()
+    f = n // 2
+    xr, wp, xv, wv = product_operands(t, n, k, 52, gated=True)
+    got = host(mx.gated_linear(xr, wp, how=(256, 1)).dequantize(F32)).astype(np.float64)
+    g, u = xv @ wv[:f].T, xv @ wv[f:].T
+    slope = 1.1 * np.abs(u) * sum_bound(xv, wv[:f]) + (np.abs(g) + 1) * sum_bound(xv, wv[f:])
+    want = plain.silu(g) * u
+    largest = np.abs(np.pad(want, ((0, 0), (0, -f % 32)))).reshape(t, -1, 32).max(-1).repeat(32, -1)[:, :f]
+    # half a step of E4M3: 2^-4 of the number, or of the smallest normal number by a scale that is at most 2^-7 of the block's largest
+    assert (np.abs(got - want) <= np.maximum(2.0**-4 * np.abs(want), 2.0**-17 * largest) * (1 + 2.0**-10) + slope).all()
 
 
 def test_every_pair_of_codes():
@@ -241,11 +260,12 @@ def test_rows_behind_the_last_are_left_alone():
     assert (room[5:] == 7).all() and (np.abs(host(room[:5]) - xv @ wv.T) <= sum_bound(xv, wv)).all()
 
 
-@pytest.mark.parametrize("t,f,k", [(1, 16, 128), (3, 33, 100), (16, 4864, 896), (70, 200, 384), (300, 260, 256)])
+@pytest.mark.parametrize("t,f,k,how", [(1, 16, 128, None), (3, 33, 100, None), (16, 4864, 896, None), (70, 200, 384, None), (300, 260, 256, None), (20, 64, 1024, (16, 8)), (33, 70, 700, (32, 3)), (40, 130, 640, (64, 2)), (130, 96, 640, (128, 5)),
+                                       (7, 193, 512, (256, 1)), (513, 64, 256, (256, 1))])
 @pytest.mark.parametrize("gate", [ops.SILU_GATE, (1.702, 7.0)])
-def test_gated_linear(t, f, k, gate):
+def test_gated_linear(t, f, k, how, gate):
     xr, wp, xv, wv = product_operands(t, 2 * f, k, 40, gated=True)
-    rows = mx.gated_linear(xr, wp, gate)
+    rows = mx.gated_linear(xr, wp, gate, how=how)
     g, u = xv @ wv[:f].T, xv @ wv[f:].T
     eg, eu = sum_bound(xv, wv[:f]), sum_bound(xv, wv[f:])
     if gate == ops.SILU_GATE:
