@@ -8,8 +8,11 @@
 // A k-slice is 128 numbers: four blocks.  A weight's tile of a slice is 8,704 contiguous bytes of memory
 // (8,192 of codes, 512 of scales).  Shared memory holds 4-bit operands as 16 numbers in 8 bytes and 8 bytes
 // of room, rows of 128 bytes with 128-byte swizzle: four warps copy them there 8 bytes at a time with
-// cp.async, which spreads them on the way; each thread makes its own copies visible to the tensor core
-// (fence.proxy.async) when they have landed.  Tokens come by TMA, their scales 4 bytes a row.  The weights
+// cp.async, which spreads them on the way.  A slice's barrier counts the threads whose copies have landed; the
+// thread that issues the products then makes them visible to the tensor core (fence.proxy.async).  It is that
+// thread's fence because the fence waits for all its thread's own copies: made by the threads that copy, it let
+// one slice be on its way where the ring has room for five (7B's gate and up projections, one token: 25.0 us).
+// Tokens come by TMA, their scales 4 bytes a row.  The weights
 // depend on no earlier kernel of the stream: the first ring of them is asked for before the dependency wait.
 //
 // Two kernels: mx_few_kernel, the weight's rows on the M side, for a few tokens or few tiles, whose time is
@@ -41,19 +44,9 @@ struct MxArgs {
 __device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void copies_wait_but(int n) {  // all of this thread's groups but the last n
-  switch (n) {
-    case 0: copies_wait<0>(); break;
-    case 1: copies_wait<1>(); break;
-    case 2: copies_wait<2>(); break;
-    case 3: copies_wait<3>(); break;
-    case 4: copies_wait<4>(); break;
-    case 5: copies_wait<5>(); break;
-    default: copies_wait<6>(); break;
-  }
-}
+// The barrier counts one arrival of this thread when all its copies so far have landed.
+__device__ __forceinline__ void arrive_when_landed(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void fence_to_tensor_core() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void load_tokens(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
@@ -197,7 +190,7 @@ __device__ __forceinline__ void few_stored_token(const MxArgs& args, float4 v, i
 template <int BN>
 __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_constant__ CUtensorMap map_x, const MxArgs args, const int parts) {
   using Tile = FewTile<BN>;
-  constexpr int STAGES = Tile::STAGES, AHEAD = STAGES - 1;
+  constexpr int STAGES = Tile::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
   __shared__ uint64_t weights_in[STAGES], tokens_in[STAGES], stage_free[STAGES], sums_done;
@@ -227,25 +220,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
 
   if (warp < 4) {
     const uint8_t* src = args.tiles + ((size_t)f_tile * args.slices + first) * MX_TILE_BYTES;
-    int i = 0;
-    for (; i < n; ++i) {
+    for (int i = 0; i < n; ++i) {
       const int s = i % STAGES;
       if (i >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(i / STAGES - 1) & 1u, &abort_flag)) break;
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES;
       const uint8_t* from = src + (size_t)i * MX_TILE_BYTES;
       load_weight_tile(stage, from, threadIdx.x);
       if (threadIdx.x < 32) copy16(stage + Tile::A_BYTES + Tile::B_BYTES + threadIdx.x * 16, from + MX_TILE_CODES + threadIdx.x * 16);
-      copies_end_group();
-      if (i >= AHEAD) {
-        copies_wait<AHEAD>();
-        fence_to_tensor_core();
-        mbar_arrive(&weights_in[(i - AHEAD) % STAGES]);
-      }
-    }
-    for (int j = max(0, i - AHEAD); j < i; ++j) {
-      copies_wait_but(i - 1 - j);
-      fence_to_tensor_core();
-      mbar_arrive(&weights_in[j % STAGES]);
+      arrive_when_landed(&weights_in[s]);
     }
   } else if (warp == 4) {
     pdl_wait();
@@ -265,17 +247,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
         const int t = r + lane;
         if (t < BN && t0 + t < args.T) copy4(scales + (uint32_t)mx_scale_at(t, 0), args.x_scales + (size_t)(t0 + t) * row_bytes + 4 * (first + i));
       }
-      copies_end_group();
-      if (i >= AHEAD) {
-        copies_wait<AHEAD>();
-        fence_to_tensor_core();
-        mbar_arrive(&tokens_in[(i - AHEAD) % STAGES]);
-      }
-    }
-    for (int j = max(0, i - AHEAD); j < i; ++j) {
-      copies_wait_but(i - 1 - j);
-      fence_to_tensor_core();
-      mbar_arrive(&tokens_in[j % STAGES]);
+      arrive_when_landed(&tokens_in[s]);
     }
     if (*(volatile int*)&abort_flag)
       for (int j = max(0, i - STAGES); j < i; ++j) drain(&tokens_in[j % STAGES], (uint32_t)(j / STAGES) & 1u);
@@ -286,6 +258,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
       const uint32_t parity = (uint32_t)(i / STAGES) & 1u;
       ok = mbar_wait(&weights_in[s], parity, &abort_flag) && mbar_wait(&tokens_in[s], parity, &abort_flag);
       if (!ok) break;
+      fence_to_tensor_core();
       tc_fence_after();
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES;
       const uint32_t scale_a = tmem + BN + s * 8, scale_b = scale_a + 4;
@@ -299,6 +272,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
     umma_commit(&sums_done);
     if (!ok) drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
   }
+  if (warp < 5) copies_wait();  // landed long ago, unless a wait ran out
   __syncwarp();
 
   const int live = min(BN, args.T - t0);
@@ -451,7 +425,7 @@ __device__ __forceinline__ void pair_finish64(const MxArgs& args, const uint32_t
 }
 
 __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const MxArgs args) {
-  constexpr int STAGES = PAIR_STAGES, AHEAD = STAGES - 1;
+  constexpr int STAGES = PAIR_STAGES;
   constexpr uint32_t A_BYTES = 128 * MX_GROUP, B_BYTES = 128 * MX_GROUP;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -485,10 +459,6 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
 
   if (warp < 4) {
     int it = 0;  // slices asked for so far, over all tiles
-    auto tell = [&](int j) {
-      fence_to_tensor_core();
-      mbar_arrive(&landed[j % STAGES]);
-    };
     bool ok = true;
     for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
       const int first_tile = (tile % f_tiles) * 2;
@@ -504,16 +474,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
         const uint32_t stage = tiles + s * PAIR_STAGE_BYTES;
         load_weight_tile(stage + A_BYTES, mine + (size_t)i * MX_TILE_BYTES, threadIdx.x);
         if (threadIdx.x < 64) copy16(stage + A_BYTES + B_BYTES + 512 + threadIdx.x * 16, scales + (size_t)i * MX_TILE_BYTES);
-        copies_end_group();
-        if (it >= AHEAD) {
-          copies_wait<AHEAD>();
-          tell(it - AHEAD);
-        }
+        arrive_when_landed(&landed[s]);
       }
-    }
-    for (int j = max(0, it - AHEAD); j < it; ++j) {
-      copies_wait_but(it - 1 - j);
-      tell(j);
     }
   } else if (warp == 4) {
     pdl_wait();
@@ -537,18 +499,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
 #pragma unroll
         for (int r = 0; r < 128; r += 32)
           if (t0 + r + lane < args.T) copy4(stage + A_BYTES + B_BYTES + (uint32_t)mx_scale_at(r + lane, 0), args.x_scales + (size_t)(t0 + r + lane) * row_bytes + 4 * i);
-        copies_end_group();
-        if (it >= AHEAD) {
-          copies_wait<AHEAD>();
-          fence_to_tensor_core();
-          mbar_arrive(&landed[(it - AHEAD) % STAGES]);
-        }
+        arrive_when_landed(&landed[s]);
       }
-    }
-    for (int j = max(0, it - AHEAD); j < it; ++j) {
-      copies_wait_but(it - 1 - j);
-      fence_to_tensor_core();
-      mbar_arrive(&landed[j % STAGES]);
     }
     if (*(volatile int*)&abort_flag)
       for (int j = max(0, it - STAGES); j < it; ++j) drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
@@ -560,6 +512,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
         for (int i = 0; i < slices; ++i, ++it) {
           ok = mbar_wait(&landed[it % STAGES], (uint32_t)(it / STAGES) & 1u, &abort_flag);
           if (!ok) break;
+          fence_to_tensor_core();
           mbar_arrive_in_cluster(in_cluster_cta(&peer_landed[it % STAGES], 0));
         }
     } else if (lane == 0) {
@@ -577,6 +530,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
           // the scales' two places take turns: the products of the slice before last are complete
           if (ok && it >= 2) ok = mbar_wait(&stage_free[(it - 2) % STAGES], (uint32_t)((it - 2) / STAGES) & 1u, &abort_flag);
           if (!ok) break;
+          fence_to_tensor_core();
           tc_fence_after();
           const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES;
           const uint32_t scale_a = tmem + PAIR_SCALES + (it & 1) * 12, scale_b = scale_a + 4;
@@ -625,6 +579,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
       tc_fence_before();
     }
   }
+  if (warp < 5) copies_wait();  // landed long ago, unless a wait ran out
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves, or frees tensor memory, while the other may still signal or read it
