@@ -20,6 +20,7 @@ constexpr int MX_TILE_ROWS = 128;  // rows of a weight's tile
 // the tensor core reads them: 32 rows of 16 bytes, byte 4 j + b of row i the scale of row 32 j + i, block b.
 constexpr int MX_TILE_CODES = MX_TILE_ROWS * MX_GROUP / 2;
 constexpr int MX_TILE_BYTES = MX_TILE_CODES + MX_TILE_ROWS * (MX_GROUP / MX_BLOCK);
+constexpr int MX_TILE_MAP_ROWS = MX_TILE_BYTES / (MX_GROUP / 2);  // a tile as rows of 64 bytes
 constexpr int MX_GATE_ROWS = 16;   // a gated weight's rows: 16 of the gate, the same 16 of the up projection, and so on
 
 __host__ __device__ __forceinline__ int mx_scale_at(int row, int block) { return (row & 31) * 16 + (row >> 5) * 4 + block; }

@@ -6,14 +6,12 @@
 // operands too, in tensor memory, so sums are of the numbers themselves and in fp32.
 //
 // A k-slice is 128 numbers: four blocks.  A weight's tile of a slice is 8,704 contiguous bytes of memory
-// (8,192 of codes, 512 of scales).  Shared memory holds 4-bit operands as 16 numbers in 8 bytes and 8 bytes
-// of room, rows of 128 bytes with 128-byte swizzle: four warps copy them there 8 bytes at a time with
-// cp.async, which spreads them on the way.  A slice's barrier counts the threads whose copies have landed; the
-// thread that issues the products then makes them visible to the tensor core (fence.proxy.async).  It is that
-// thread's fence because the fence waits for all its thread's own copies: made by the threads that copy, it let
-// one slice be on its way where the ring has room for five (7B's gate and up projections, one token: 25.0 us).
-// Tokens come by TMA, their scales 4 bytes a row.  The weights
-// depend on no earlier kernel of the stream: the first ring of them is asked for before the dependency wait.
+// (8,192 of codes, 512 of scales), fetched by one thread with two copies: TMA, which unpacks 4-bit numbers on
+// the way (shared memory holds them as 16 in 8 bytes and 8 bytes of room, rows of 128 bytes with 128-byte
+// swizzle), and a plain bulk copy.  Spreading them with cp.async, 8 bytes at a time, was bound by the copies'
+// instructions: 7B's gate and up projections, one token, 21.9 us and 2,048 tokens 419 us.  Tokens come by TMA,
+// their scales 4 bytes a row.  The weights depend on no earlier kernel of the stream: the first ring of them is
+// asked for before the dependency wait.
 //
 // Two kernels: mx_few_kernel, the weight's rows on the M side, for a few tokens or few tiles, whose time is
 // the weight's bytes or a launch's latency; mx_pair_kernel, the tokens on the M side and a pair of CTAs to a
@@ -24,6 +22,8 @@
 #include "mx.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
+
+#include <string.h>
 
 #include <atomic>
 
@@ -41,22 +41,17 @@ struct MxArgs {
   int* status;
 };
 
-__device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 // The barrier counts one arrival of this thread when all its copies so far have landed.
 __device__ __forceinline__ void arrive_when_landed(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void fence_to_tensor_core() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void load_tokens(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
 }
-// A weight's tile: thread i of 128 copies 8 bytes of every sixteenth row (the same place in their groups of 8), the first 32 the scales.
-__device__ __forceinline__ void load_weight_tile(uint32_t dst, const uint8_t* from, int i) {
-  const int row = i >> 3, chunk = i & 7;
-  const uint32_t to = dst + (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
-#pragma unroll
-  for (int j = 0; j < 8; ++j) copy8(to + j * 16 * 128, from + j * 1024 + i * 8);
+// A weight's tile: 128 rows of codes (a tile is 136 rows of 64 bytes, the last eight its scales); 8,192 bytes are counted.
+__device__ __forceinline__ void load_bytes(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 // Ends early: what is still in flight lands in a bounded time.
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
@@ -112,7 +107,7 @@ __device__ __forceinline__ void cluster_sync_all() {  // every thread of every C
 // out the tokens, add the parts in order out of one another's shared memory and write whole rows: no sums go
 // through memory, nothing is launched to add them, and the last step is spread over as many SMs as the first.
 // ---------------------------------------------------------------------------
-constexpr int FEW_THREADS = 192;  // warps 0-3 weights, then the sums; warp 4 tokens; warp 5 products
+constexpr int FEW_THREADS = 192;  // warp 0 weights, 4 tokens, 5 products; then warps 0-3 read the sums and all write rows
 constexpr int FEW_PARTS = 8;      // of a depth, at most: a portable cluster
 constexpr int SUM_PITCH = MX_TILE_ROWS + 4;
 
@@ -188,7 +183,7 @@ __device__ __forceinline__ void few_stored_token(const MxArgs& args, float4 v, i
 }
 
 template <int BN>
-__global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_constant__ CUtensorMap map_x, const MxArgs args, const int parts) {
+__global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MxArgs args, const int parts) {
   using Tile = FewTile<BN>;
   constexpr int STAGES = Tile::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -205,7 +200,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&weights_in[s], 128);
+      mbar_init(&weights_in[s], 1);
       mbar_init(&tokens_in[s], 32 + 1);
       mbar_init(&stage_free[s], 1);
     }
@@ -218,16 +213,19 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tmem = tmem_base_smem;
 
-  if (warp < 4) {
-    const uint8_t* src = args.tiles + ((size_t)f_tile * args.slices + first) * MX_TILE_BYTES;
-    for (int i = 0; i < n; ++i) {
-      const int s = i % STAGES;
-      if (i >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(i / STAGES - 1) & 1u, &abort_flag)) break;
-      const uint32_t stage = tiles + s * Tile::STAGE_BYTES;
-      const uint8_t* from = src + (size_t)i * MX_TILE_BYTES;
-      load_weight_tile(stage, from, threadIdx.x);
-      if (threadIdx.x < 32) copy16(stage + Tile::A_BYTES + Tile::B_BYTES + threadIdx.x * 16, from + MX_TILE_CODES + threadIdx.x * 16);
-      arrive_when_landed(&weights_in[s]);
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;
+      for (; i < n; ++i) {
+        const int s = i % STAGES, tile = f_tile * args.slices + first + i;
+        if (i >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(i / STAGES - 1) & 1u, &abort_flag)) break;
+        const uint32_t stage = tiles + s * Tile::STAGE_BYTES;
+        mbar_expect_tx(&weights_in[s], MX_TILE_BYTES);
+        load_tile(stage, &map_w, &weights_in[s], 0, tile * MX_TILE_MAP_ROWS);
+        load_bytes(stage + Tile::A_BYTES + Tile::B_BYTES, args.tiles + (size_t)tile * MX_TILE_BYTES + MX_TILE_CODES, MX_TILE_BYTES - MX_TILE_CODES, &weights_in[s]);
+      }
+      if (*(volatile int*)&abort_flag)
+        for (int j = max(0, i - STAGES); j < i; ++j) drain(&weights_in[j % STAGES], (uint32_t)(j / STAGES) & 1u);
     }
   } else if (warp == 4) {
     pdl_wait();
@@ -240,7 +238,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES + 512;
       if (lane == 0) {
         mbar_expect_tx(&tokens_in[s], Tile::B_BYTES);
-        load_tokens(stage + Tile::A_BYTES, &map_x, &tokens_in[s], (first + i) * MX_GROUP, t0);
+        load_tile(stage + Tile::A_BYTES, &map_x, &tokens_in[s], (first + i) * MX_GROUP, t0);
       }
 #pragma unroll
       for (int r = 0; r < BN; r += 32) {
@@ -251,7 +249,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
     }
     if (*(volatile int*)&abort_flag)
       for (int j = max(0, i - STAGES); j < i; ++j) drain(&tokens_in[j % STAGES], (uint32_t)(j / STAGES) & 1u);
-  } else if (lane == 0) {
+  } else if (warp == 5 && lane == 0) {
     bool ok = true;
     for (int i = 0; i < n; ++i) {
       const int s = i % STAGES;
@@ -272,7 +270,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
     umma_commit(&sums_done);
     if (!ok) drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
   }
-  if (warp < 5) copies_wait();  // landed long ago, unless a wait ran out
+  if (warp == 4) copies_wait();  // landed long ago, unless a wait ran out
   __syncwarp();
 
   const int live = min(BN, args.T - t0);
@@ -334,7 +332,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
 // share 32 columns (0-255 and 224-479), and the epilogue takes the block that holds them first: the next tile's
 // products begin when it has those in registers, and run beside the rest of the epilogue.
 // ---------------------------------------------------------------------------
-constexpr int PAIR_THREADS = 448;  // warps 0-3 weights, 4 tokens, 5 products (second CTA: tells the first what has landed), 6-13 epilogue
+constexpr int PAIR_THREADS = 384;  // warp 0 weights, 1 tokens, 2 products (second CTA: tells the first what has landed), 4-11 epilogue
 constexpr int PAIR_STAGES = 6;
 constexpr uint32_t PAIR_STAGE_BYTES = 2 * 128 * MX_GROUP + 2048;  // tokens, weight rows, 512 bytes of the tokens' scales, 1,024 of the weight's
 constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 1024;
@@ -424,7 +422,7 @@ __device__ __forceinline__ void pair_finish64(const MxArgs& args, const uint32_t
   }
 }
 
-__global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const MxArgs args) {
+__global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MxArgs args) {
   constexpr int STAGES = PAIR_STAGES;
   constexpr uint32_t A_BYTES = 128 * MX_GROUP, B_BYTES = 128 * MX_GROUP;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -442,7 +440,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&landed[s], 128 + 32 + 1);
+      mbar_init(&landed[s], 1 + 32 + 1);
       mbar_init(&peer_landed[s], 1);
       mbar_init(&stage_free[s], 1);
     }
@@ -451,33 +449,34 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
     mbar_init(&gave_up, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 5) tmem_alloc_pair(&tmem_base_smem, 512);
+  if (warp == 2) tmem_alloc_pair(&tmem_base_smem, 512);
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers stand before either signals the other's
   tc_fence_after();
   const uint32_t tmem = tmem_base_smem;
 
-  if (warp < 4) {
-    int it = 0;  // slices asked for so far, over all tiles
-    bool ok = true;
-    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
-      const int first_tile = (tile % f_tiles) * 2;
-      // a row count that is no multiple of 256 leaves the second CTA without rows: it reads the last ones, and what comes of them is not stored
-      const uint8_t* mine = args.tiles + (size_t)min(first_tile + (int)rank, last_weight_tile) * slices * MX_TILE_BYTES;
-      const uint8_t* scales = args.tiles + (size_t)min(first_tile + (int)(threadIdx.x >> 5 & 1), last_weight_tile) * slices * MX_TILE_BYTES + MX_TILE_CODES + lane * 16;
-      for (int i = 0; i < slices; ++i, ++it) {
-        const int s = it % STAGES;
-        if (it >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(it / STAGES - 1) & 1u, &abort_flag)) {
-          ok = false;
-          break;
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;  // slices asked for so far, over all tiles
+      bool ok = true;
+      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+        // a number of rows that is no multiple of 256 leaves the second CTA without any: it reads the last ones, and what comes of them is not stored
+        const int even = tile % f_tiles * 2 * slices, odd = min(tile % f_tiles * 2 + 1, last_weight_tile) * slices;
+        for (int i = 0; i < slices; ++i, ++it) {
+          const int s = it % STAGES;
+          if (it >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(it / STAGES - 1) & 1u, &abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES + 512;
+          mbar_expect_tx(&landed[s], MX_TILE_CODES + 1024);
+          load_tile(stage + A_BYTES, &map_w, &landed[s], 0, ((rank ? odd : even) + i) * MX_TILE_MAP_ROWS);
+          load_bytes(scales, args.tiles + (size_t)(even + i) * MX_TILE_BYTES + MX_TILE_CODES, 512, &landed[s]);
+          load_bytes(scales + 512, args.tiles + (size_t)(odd + i) * MX_TILE_BYTES + MX_TILE_CODES, 512, &landed[s]);
         }
-        const uint32_t stage = tiles + s * PAIR_STAGE_BYTES;
-        load_weight_tile(stage + A_BYTES, mine + (size_t)i * MX_TILE_BYTES, threadIdx.x);
-        if (threadIdx.x < 64) copy16(stage + A_BYTES + B_BYTES + 512 + threadIdx.x * 16, scales + (size_t)i * MX_TILE_BYTES);
-        arrive_when_landed(&landed[s]);
       }
     }
-  } else if (warp == 4) {
+  } else if (warp == 1) {
     pdl_wait();
     pdl_launch();
     const int row_bytes = 4 * slices;
@@ -494,7 +493,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
         const uint32_t stage = tiles + s * PAIR_STAGE_BYTES;
         if (lane == 0) {
           mbar_expect_tx(&landed[s], A_BYTES);
-          load_tokens(stage, &map_x, &landed[s], i * MX_GROUP, t0);
+          load_tile(stage, &map_x, &landed[s], i * MX_GROUP, t0);
         }
 #pragma unroll
         for (int r = 0; r < 128; r += 32)
@@ -504,7 +503,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
     }
     if (*(volatile int*)&abort_flag)
       for (int j = max(0, it - STAGES); j < it; ++j) drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
-  } else if (warp == 5) {
+  } else if (warp == 2) {
     if (lane == 0 && rank == 1) {
       int it = 0;
       bool ok = true;
@@ -549,8 +548,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
         drain(&gave_up, 0);
       }
     }
-  } else {
-    const int q = warp & 3, half = (warp - 6) >> 2;  // a quarter of the lanes (warps read 32 (w % 4) and on), half of the columns
+  } else if (warp >= 4) {
+    const int q = warp & 3, half = (warp - 4) >> 2;  // a quarter of the lanes (warps read 32 (w % 4) and on), half of the columns
     pdl_wait();  // what is written here, an earlier kernel may have been reading
     const uint32_t taken = in_cluster_cta(&sums_taken, 0);
     bool good = true;
@@ -579,11 +578,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
       tc_fence_before();
     }
   }
-  if (warp < 5) copies_wait();  // landed long ago, unless a wait ran out
+  if (warp == 1) copies_wait();  // landed long ago, unless a wait ran out
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves, or frees tensor memory, while the other may still signal or read it
-  if (warp == 5) {
+  if (warp == 2) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);
   }
@@ -603,6 +602,20 @@ static bool make_rows_map(CUtensorMap* map, const void* base, uint64_t rows, uin
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A weight's tiles as rows of 64 bytes, 128 numbers of 4 bits, seen as boxes of 128 rows; 128 bytes at `map`.
+ALOFA_API int alofa_mx_weight_map(void* map, const void* tiles, long long n_tiles) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || (uintptr_t)tiles % 32 || n_tiles <= 0 || n_tiles * MX_TILE_MAP_ROWS > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  cuuint64_t dims[2] = {MX_GROUP, (cuuint64_t)(n_tiles * MX_TILE_MAP_ROWS)}, strides[1] = {MX_GROUP / 2};
+  cuuint32_t box[2] = {MX_GROUP, MX_TILE_ROWS}, elem[2] = {1, 1};
+  CUtensorMap m;
+  if (fn(&m, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(tiles), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return ALOFA_ERR_ARGUMENT;
+  memcpy(map, &m, sizeof(m));
+  return ALOFA_OK;
+}
+
 // A kernel's shared memory is asked for once a device (a bit of `done` each; asking takes as long as a launch).
 static bool allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
   int device = 0;
@@ -618,19 +631,20 @@ template <int BN> static std::atomic<uint64_t> few_allowed{0};
 static std::atomic<uint64_t> pair_allowed{0};
 
 template <int BN>
-static int launch_few(const CUtensorMap& map, const MxArgs& args, int parts, cudaStream_t stream) {
+static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const MxArgs& args, int parts, cudaStream_t stream) {
   const long long wide = (((long long)args.N + MX_TILE_ROWS - 1) / MX_TILE_ROWS) * parts, tall = ((long long)args.T + BN - 1) / BN;
   if (wide > 0x7fffffffll || tall > 65535) return ALOFA_ERR_ARGUMENT;
   if (!allow_shared((const void*)mx_few_kernel<BN>, (int)FewTile<BN>::SMEM, few_allowed<BN>)) return ALOFA_ERR_LAUNCH;
-  launch_dep_cluster(mx_few_kernel<BN>, dim3((unsigned)wide, (unsigned)tall), FEW_THREADS, FewTile<BN>::SMEM, stream, parts, map, args, parts);
+  launch_dep_cluster(mx_few_kernel<BN>, dim3((unsigned)wide, (unsigned)tall), FEW_THREADS, FewTile<BN>::SMEM, stream, parts, map_w, map_x, args, parts);
   return launch_status();
 }
 
 // bn: 256: pairs of CTAs (`parts` 1, a grid of `ctas` of them); 16, 32, 64 or 128 tokens a CTA, the depth in `parts` parts.
 // features > 0: out are the codes and out_scales the scales of that many gated features, n the rows of the gated weight.
-ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, const void* x_scales, const void* tiles, const float* bias, const float* add, int t, int n, int k, int features,
+// weight_map: alofa_mx_weight_map's of the tiles.
+ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, const void* x_scales, const void* tiles, const void* weight_map, const float* bias, const float* add, int t, int n, int k, int features,
                             float gate_alpha, float gate_limit, int bn, int parts, int ctas, int out_bf16, int* status, void* stream) {
-  if (t < 0 || n <= 0 || k <= 0 || k > (1 << 30) || n > (1 << 30) || (uintptr_t)x_codes % 16 || (uintptr_t)x_scales % 4 || (uintptr_t)tiles % 16) return ALOFA_ERR_ARGUMENT;
+  if (t < 0 || n <= 0 || k <= 0 || k > (1 << 30) || n > (1 << 30) || (uintptr_t)x_codes % 16 || (uintptr_t)x_scales % 4 || (uintptr_t)tiles % 32) return ALOFA_ERR_ARGUMENT;
   if (features < 0 || (features && (n != 2 * ((features + 15) / 16 * 16) || !out_scales || (uintptr_t)out % 16))) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
   MxArgs args = {};
@@ -642,19 +656,20 @@ ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, co
   const bool few = bn == 16 || bn == 32 || bn == 64 || bn == 128;
   if (!few && bn != 256) return ALOFA_ERR_ARGUMENT;
   if (parts < 1 || parts > args.slices || parts > (few ? FEW_PARTS : 1)) return ALOFA_ERR_ARGUMENT;
-  CUtensorMap map;
-  if (!make_rows_map(&map, x_codes, (uint64_t)t, (uint64_t)args.slices * MX_GROUP, few ? bn : 128)) return ALOFA_ERR_ARGUMENT;
+  CUtensorMap map_w, map_x;
+  memcpy(&map_w, weight_map, sizeof(map_w));
+  if (!make_rows_map(&map_x, x_codes, (uint64_t)t, (uint64_t)args.slices * MX_GROUP, few ? bn : 128)) return ALOFA_ERR_ARGUMENT;
   cudaStream_t s = (cudaStream_t)stream;
   switch (bn) {
-    case 16: return launch_few<16>(map, args, parts, s);
-    case 32: return launch_few<32>(map, args, parts, s);
-    case 64: return launch_few<64>(map, args, parts, s);
-    case 128: return launch_few<128>(map, args, parts, s);
+    case 16: return launch_few<16>(map_w, map_x, args, parts, s);
+    case 32: return launch_few<32>(map_w, map_x, args, parts, s);
+    case 64: return launch_few<64>(map_w, map_x, args, parts, s);
+    case 128: return launch_few<128>(map_w, map_x, args, parts, s);
   }
   const long long pair_tiles = (((long long)n + 255) / 256) * (((long long)t + 255) / 256);
   if (ctas < 2 || pair_tiles > 0x3fffffffll) return ALOFA_ERR_ARGUMENT;
   if (!allow_shared((const void*)mx_pair_kernel, (int)PAIR_SMEM, pair_allowed)) return ALOFA_ERR_LAUNCH;
   const long long grid = 2 * pair_tiles < ctas ? 2 * pair_tiles : ctas / 2 * 2;
-  launch_dep_cluster(mx_pair_kernel, dim3((unsigned)grid), PAIR_THREADS, PAIR_SMEM, s, 2, map, args);
+  launch_dep_cluster(mx_pair_kernel, dim3((unsigned)grid), PAIR_THREADS, PAIR_SMEM, s, 2, map_w, map_x, args);
   return launch_status();
 }

@@ -22,6 +22,7 @@ beside as much of the GPU's time: operands are checked once each, in one pass
 over what a launch goes by, and rows are one allocation."""
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -145,7 +146,7 @@ class MxWeight:
     are a gate's, the second an up projection's.  Made by :func:`pack_weight`
     or :meth:`from_codes`."""
 
-    __slots__ = ("tiles", "n", "k", "gated", "rows", "device", "at")
+    __slots__ = ("tiles", "n", "k", "gated", "rows", "device", "at", "map")
 
     def __init__(self, n: int, k: int, gated: bool, here: int):
         if n <= 0 or k <= 0 or (gated and n % 2):
@@ -155,6 +156,9 @@ class MxWeight:
         self.rows = 2 * (-(-(n // 2) // GATE_ROWS) * GATE_ROWS) if gated else n
         self.tiles = torch.empty((-(-self.rows // TILE_ROWS), padded(k) // GROUP, TILE_BYTES), dtype=_U8, device=here)
         self.at = self.tiles.data_ptr()
+        #: how the copies of the product see the tiles (a tensor map)
+        self.map = ctypes.create_string_buffer(128)
+        ops.mx_launched(ops.mx_library().alofa_mx_weight_map(self.map, self.at, self.tiles.shape[0] * self.tiles.shape[1]), 0, "mx weight", lambda: f"rows={n} depth={k}")
 
     @classmethod
     def from_codes(cls, codes, scales, k: int, gated: bool = False) -> "MxWeight":
@@ -195,7 +199,7 @@ class MxWeight:
             raise AlofaError("invalid_argument", "the first rows of a weight that is not gated", f"rows={n} of {self.n} gated={self.gated}")
         part = MxWeight.__new__(MxWeight)
         part.n, part.rows, part.k, part.gated, part.device = n, n, self.k, False, self.device
-        part.tiles, part.at = self.tiles[: -(-n // TILE_ROWS)], self.at
+        part.tiles, part.at, part.map = self.tiles[: -(-n // TILE_ROWS)], self.at, self.map
         return part
 
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
@@ -295,7 +299,7 @@ def _product(x: MxRows, w: MxWeight, out_at, scales_at, bias_at, add_at, feature
     bn, parts = how or plan(x.rows, w.rows, w.k)
     status_at = None if status is None else _at(status, "status", _I32, status.shape, here)
     rc = ops.mx_library().alofa_mx_gemm(
-        out_at, scales_at, x.codes_at, x.scales_at, w.at, bias_at, add_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16, status_at, _stream(here)
+        out_at, scales_at, x.codes_at, x.scales_at, w.at, w.map, bias_at, add_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16, status_at, _stream(here)
     )
     ops.mx_launched(rc, 1, what, lambda: f"tokens={x.rows} rows={w.rows} depth={w.k} how={(bn, parts)}")
 
