@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   constexpr int STAGES = Tile::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  __shared__ uint64_t weights_in[STAGES], tokens_in[STAGES], stage_free[STAGES], sums_done;
+  __shared__ uint64_t landed[STAGES], stage_free[STAGES], sums_done;
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
 
@@ -200,8 +200,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&weights_in[s], 1);
-      mbar_init(&tokens_in[s], 32 + 1);
+      mbar_init(&landed[s], 1 + 1 + 32);  // the weight's bytes, the tokens', the copies of their scales
       mbar_init(&stage_free[s], 1);
     }
     mbar_init(&sums_done, 1);
@@ -215,60 +214,75 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
 
   if (warp == 0) {
     if (lane == 0) {
-      int i = 0;
+      int i = 0, s = 0;
+      uint32_t round = 1;  // parity of the phase in which this stage was last freed; the first round waits for nothing
+      bool free = true;
       for (; i < n; ++i) {
-        const int s = i % STAGES, tile = f_tile * args.slices + first + i;
-        if (i >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(i / STAGES - 1) & 1u, &abort_flag)) break;
+        if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) break;
         const uint32_t stage = tiles + s * Tile::STAGE_BYTES;
-        mbar_expect_tx(&weights_in[s], MX_TILE_BYTES);
-        load_tile(stage, &map_w, &weights_in[s], 0, tile * MX_TILE_MAP_ROWS);
-        load_bytes(stage + Tile::A_BYTES + Tile::B_BYTES, args.tiles + (size_t)tile * MX_TILE_BYTES + MX_TILE_CODES, MX_TILE_BYTES - MX_TILE_CODES, &weights_in[s]);
+        const int tile = f_tile * args.slices + first + i;
+        uint64_t* bar = &landed[s];
+        s = s + 1 == STAGES ? 0 : s + 1;
+        round ^= s == 0 ? 1u : 0u;
+        free = i + 1 < STAGES || mbar_complete(&stage_free[s], round);
+        mbar_expect_tx(bar, MX_TILE_BYTES);
+        load_tile(stage, &map_w, bar, 0, tile * MX_TILE_MAP_ROWS);
+        load_bytes(stage + Tile::A_BYTES + Tile::B_BYTES, args.tiles + (size_t)tile * MX_TILE_BYTES + MX_TILE_CODES, MX_TILE_BYTES - MX_TILE_CODES, bar);
       }
-      if (*(volatile int*)&abort_flag)
-        for (int j = max(0, i - STAGES); j < i; ++j) drain(&weights_in[j % STAGES], (uint32_t)(j / STAGES) & 1u);
     }
   } else if (warp == 4) {
     pdl_wait();
     pdl_launch();
     const int row_bytes = 4 * args.slices;
-    int i = 0;
+    int i = 0, s = 0;
+    uint32_t round = 1;
+    bool free = true;
     for (; i < n; ++i) {
-      const int s = i % STAGES;
-      if (i >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(i / STAGES - 1) & 1u, &abort_flag)) break;
+      if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) break;
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES + 512;
+      uint64_t* bar = &landed[s];
+      s = s + 1 == STAGES ? 0 : s + 1;
+      round ^= s == 0 ? 1u : 0u;
+      free = i + 1 < STAGES || mbar_complete(&stage_free[s], round);
       if (lane == 0) {
-        mbar_expect_tx(&tokens_in[s], Tile::B_BYTES);
-        load_tile(stage + Tile::A_BYTES, &map_x, &tokens_in[s], (first + i) * MX_GROUP, t0);
+        mbar_expect_tx(bar, Tile::B_BYTES);
+        load_tile(stage + Tile::A_BYTES, &map_x, bar, (first + i) * MX_GROUP, t0);
       }
 #pragma unroll
       for (int r = 0; r < BN; r += 32) {
         const int t = r + lane;
         if (t < BN && t0 + t < args.T) copy4(scales + (uint32_t)mx_scale_at(t, 0), args.x_scales + (size_t)(t0 + t) * row_bytes + 4 * (first + i));
       }
-      arrive_when_landed(&tokens_in[s]);
+      arrive_when_landed(bar);
     }
     if (*(volatile int*)&abort_flag)
-      for (int j = max(0, i - STAGES); j < i; ++j) drain(&tokens_in[j % STAGES], (uint32_t)(j / STAGES) & 1u);
-  } else if (warp == 5 && lane == 0) {
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const int s = i % STAGES;
-      const uint32_t parity = (uint32_t)(i / STAGES) & 1u;
-      ok = mbar_wait(&weights_in[s], parity, &abort_flag) && mbar_wait(&tokens_in[s], parity, &abort_flag);
-      if (!ok) break;
-      fence_to_tensor_core();
-      tc_fence_after();
-      const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES;
-      const uint32_t scale_a = tmem + BN + s * 8, scale_b = scale_a + 4;
-      scales_to_tmem(scale_a, scales);
-      scales_to_tmem(scale_b, scales + 512);
-      const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + Tile::A_BYTES);
+      for (int j = max(0, i - STAGES); j < i; ++j) drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+  } else if (warp == 5) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t round = 0;
+      bool ok = true, ready = false;
+      for (int i = 0; i < n; ++i) {
+        if (!ready) ok = mbar_wait(&landed[s], round, &abort_flag);
+        if (!ok) break;
+        const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES;
+        const uint32_t scale_a = tmem + BN + s * 8, scale_b = scale_a + 4;
+        uint64_t* freed = &stage_free[s];
+        s = s + 1 == STAGES ? 0 : s + 1;
+        round ^= s == 0 ? 1u : 0u;
+        fence_to_tensor_core();
+        tc_fence_after();
+        ready = i + 1 < n && mbar_complete(&landed[s], round);
+        scales_to_tmem(scale_a, scales);
+        scales_to_tmem(scale_b, scales + 512);
+        const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + Tile::A_BYTES);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) umma_mx(tmem, a + 2 * j, b + 2 * j, mx_idesc(E2M1, E4M3, 128, BN, j), scale_a, scale_b, (i | j) ? 1u : 0u);
-      umma_commit(&stage_free[s]);
+        for (int j = 0; j < 4; ++j) umma_mx(tmem, a + 2 * j, b + 2 * j, mx_idesc(E2M1, E4M3, 128, BN, j), scale_a, scale_b, (i | j) ? 1u : 0u);
+        umma_commit(freed);
+      }
+      umma_commit(&sums_done);
+      if (!ok) drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
     }
-    umma_commit(&sums_done);
-    if (!ok) drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
   }
   if (warp == 4) copies_wait();  // landed long ago, unless a wait ran out
   __syncwarp();
@@ -329,14 +343,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
 // scales of all 256 rows stand in both CTAs' tensor memory, those of its own tokens in each.
 //
 // Tensor memory holds 512 columns: two accumulators of 256 and the scales do not fit.  The accumulators therefore
-// share 32 columns (0-255 and 224-479), and the epilogue takes the block that holds them first: the next tile's
-// products begin when it has those in registers, and run beside the rest of the epilogue.
+// share 64 columns (0-255 and 192-447), and the epilogue takes those first: the next tile's products begin when it has
+// them in registers, and run beside the rest of the epilogue.  Scales have a place for each stage of the ring: those of
+// a slice are written when the products of the slice before it there are complete.
 // ---------------------------------------------------------------------------
 constexpr int PAIR_THREADS = 384;  // warp 0 weights, 1 tokens, 2 products (second CTA: tells the first what has landed), 4-11 epilogue
-constexpr int PAIR_STAGES = 6;
+constexpr int PAIR_STAGES = 5;
 constexpr uint32_t PAIR_STAGE_BYTES = 2 * 128 * MX_GROUP + 2048;  // tokens, weight rows, 512 bytes of the tokens' scales, 1,024 of the weight's
 constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 1024;
-constexpr uint32_t PAIR_SECOND = 224, PAIR_SCALES = 480;  // columns of the second accumulator, of two places of 12 for scales
+constexpr uint32_t PAIR_SECOND = 192, PAIR_SCALES = 448;  // columns of the second accumulator, and of 12 for a stage's scales
 
 __device__ __forceinline__ void pair_load64(uint32_t tmem, uint32_t (&r)[64]) {
 #pragma unroll
@@ -427,8 +442,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
   constexpr uint32_t A_BYTES = 128 * MX_GROUP, B_BYTES = 128 * MX_GROUP;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  // landed: this CTA's own copies of a slice; peer_landed (first CTA): the second one's; sums_ready, sums_taken: a tile's accumulator
-  __shared__ uint64_t landed[STAGES], peer_landed[STAGES], stage_free[STAGES], sums_ready, sums_taken, gave_up;
+  // landed: the copies of a slice, in the first CTA those of both; sums_ready, sums_taken: a tile's accumulator
+  __shared__ uint64_t landed[STAGES], stage_free[STAGES], sums_ready, sums_taken, gave_up;
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
 
@@ -440,8 +455,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&landed[s], 1 + 32 + 1);
-      mbar_init(&peer_landed[s], 1);
+      mbar_init(&landed[s], 1 + 1 + 32 + (rank == 0 ? 1 : 0));  // the weight's bytes, the tokens', the copies of their scales; the second CTA's word
       mbar_init(&stage_free[s], 1);
     }
     mbar_init(&sums_ready, 1);
@@ -457,22 +471,26 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;  // slices asked for so far, over all tiles
-      bool ok = true;
+      int it = 0, s = 0;  // slices asked for so far, over all tiles; the ring's stage
+      uint32_t round = 1;  // parity of the phase in which it was last freed; the first round waits for nothing
+      bool ok = true, free = true;
       for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
         // a number of rows that is no multiple of 256 leaves the second CTA without any: it reads the last ones, and what comes of them is not stored
         const int even = tile % f_tiles * 2 * slices, odd = min(tile % f_tiles * 2 + 1, last_weight_tile) * slices;
         for (int i = 0; i < slices; ++i, ++it) {
-          const int s = it % STAGES;
-          if (it >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(it / STAGES - 1) & 1u, &abort_flag)) {
+          if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) {
             ok = false;
             break;
           }
           const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES + 512;
-          mbar_expect_tx(&landed[s], MX_TILE_CODES + 1024);
-          load_tile(stage + A_BYTES, &map_w, &landed[s], 0, ((rank ? odd : even) + i) * MX_TILE_MAP_ROWS);
-          load_bytes(scales, args.tiles + (size_t)(even + i) * MX_TILE_BYTES + MX_TILE_CODES, 512, &landed[s]);
-          load_bytes(scales + 512, args.tiles + (size_t)(odd + i) * MX_TILE_BYTES + MX_TILE_CODES, 512, &landed[s]);
+          uint64_t* bar = &landed[s];
+          s = s + 1 == STAGES ? 0 : s + 1;
+          round ^= s == 0 ? 1u : 0u;
+          free = it + 1 < STAGES || mbar_complete(&stage_free[s], round);
+          mbar_expect_tx(bar, MX_TILE_CODES + 1024);
+          load_tile(stage + A_BYTES, &map_w, bar, 0, ((rank ? odd : even) + i) * MX_TILE_MAP_ROWS);
+          load_bytes(scales, args.tiles + (size_t)(even + i) * MX_TILE_BYTES + MX_TILE_CODES, 512, bar);
+          load_bytes(scales + 512, args.tiles + (size_t)(odd + i) * MX_TILE_BYTES + MX_TILE_CODES, 512, bar);
         }
       }
     }
@@ -480,66 +498,77 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
     pdl_wait();
     pdl_launch();
     const int row_bytes = 4 * slices;
-    int it = 0;
-    bool ok = true;
+    int it = 0, s = 0;
+    uint32_t round = 1;
+    bool ok = true, free = true;
     for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
       const int t0 = tile / f_tiles * 256 + (int)rank * 128;
       for (int i = 0; i < slices; ++i, ++it) {
-        const int s = it % STAGES;
-        if (it >= STAGES && !mbar_wait(&stage_free[s], (uint32_t)(it / STAGES - 1) & 1u, &abort_flag)) {
+        if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) {
           ok = false;
           break;
         }
         const uint32_t stage = tiles + s * PAIR_STAGE_BYTES;
+        uint64_t* bar = &landed[s];
+        s = s + 1 == STAGES ? 0 : s + 1;
+        round ^= s == 0 ? 1u : 0u;
+        free = it + 1 < STAGES || mbar_complete(&stage_free[s], round);
         if (lane == 0) {
-          mbar_expect_tx(&landed[s], A_BYTES);
-          load_tile(stage, &map_x, &landed[s], i * MX_GROUP, t0);
+          mbar_expect_tx(bar, A_BYTES);
+          load_tile(stage, &map_x, bar, i * MX_GROUP, t0);
         }
 #pragma unroll
         for (int r = 0; r < 128; r += 32)
           if (t0 + r + lane < args.T) copy4(stage + A_BYTES + B_BYTES + (uint32_t)mx_scale_at(r + lane, 0), args.x_scales + (size_t)(t0 + r + lane) * row_bytes + 4 * i);
-        arrive_when_landed(&landed[s]);
+        arrive_when_landed(bar);
       }
     }
     if (*(volatile int*)&abort_flag)
       for (int j = max(0, it - STAGES); j < it; ++j) drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
   } else if (warp == 2) {
     if (lane == 0 && rank == 1) {
-      int it = 0;
-      bool ok = true;
+      int s = 0;
+      uint32_t round = 0;
+      bool ok = true, ready = false;
+      const uint32_t first_landed = in_cluster_cta(&landed[0], 0);
       for (int tile = pair; tile < n_tiles && ok; tile += n_pairs)
-        for (int i = 0; i < slices; ++i, ++it) {
-          ok = mbar_wait(&landed[it % STAGES], (uint32_t)(it / STAGES) & 1u, &abort_flag);
+        for (int i = 0; i < slices; ++i) {
+          if (!ready) ok = mbar_wait(&landed[s], round, &abort_flag);
           if (!ok) break;
+          const uint32_t tell = first_landed + (uint32_t)s * 8;
+          s = s + 1 == STAGES ? 0 : s + 1;
+          round ^= s == 0 ? 1u : 0u;
+          ready = mbar_complete(&landed[s], round);
           fence_to_tensor_core();
-          mbar_arrive_in_cluster(in_cluster_cta(&peer_landed[it % STAGES], 0));
+          mbar_arrive_in_cluster(tell);
         }
     } else if (lane == 0) {
-      int it = 0, done = 0;  // slices consumed, tiles begun
-      bool ok = true;
+      int done = 0, s = 0;  // tiles begun, the ring's stage
+      uint32_t round = 0;
+      bool ok = true, ready = false;
       for (int tile = pair; tile < n_tiles && ok; tile += n_pairs, ++done) {
         if (done) ok = mbar_wait_in_cluster(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag);
         if (!ok) break;
         tc_fence_after();
         const uint32_t sums = tmem + (done & 1 ? PAIR_SECOND : 0);
-        for (int i = 0; i < slices; ++i, ++it) {
-          const int s = it % STAGES;
-          const uint32_t parity = (uint32_t)(it / STAGES) & 1u;
-          ok = mbar_wait(&landed[s], parity, &abort_flag) && mbar_wait_in_cluster(&peer_landed[s], parity, &abort_flag);
-          // the scales' two places take turns: the products of the slice before last are complete
-          if (ok && it >= 2) ok = mbar_wait(&stage_free[(it - 2) % STAGES], (uint32_t)((it - 2) / STAGES) & 1u, &abort_flag);
+        for (int i = 0; i < slices; ++i) {
+          if (!ready) ok = mbar_wait_in_cluster(&landed[s], round, &abort_flag);
           if (!ok) break;
+          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES;
+          const uint32_t scale_a = tmem + PAIR_SCALES + s * 12, scale_b = scale_a + 4;
+          uint64_t* freed = &stage_free[s];
+          s = s + 1 == STAGES ? 0 : s + 1;
+          round ^= s == 0 ? 1u : 0u;
           fence_to_tensor_core();
           tc_fence_after();
-          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES;
-          const uint32_t scale_a = tmem + PAIR_SCALES + (it & 1) * 12, scale_b = scale_a + 4;
+          ready = mbar_complete_in_cluster(&landed[s], round);
           scales_to_tmem_pair(scale_a, scales);
           scales_to_tmem_pair(scale_b, scales + 512);
           scales_to_tmem_pair(scale_b + 4, scales + 1024);
           const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + A_BYTES);
 #pragma unroll
           for (int j = 0; j < 4; ++j) umma_mx_pair(sums, a + 2 * j, b + 2 * j, mx_idesc(E4M3, E2M1, 256, 256, j), scale_a, scale_b, (i | j) ? 1u : 0u);
-          umma_commit_pair(&stage_free[s], 3);
+          umma_commit_pair(freed, 3);
         }
         if (ok) umma_commit_pair(&sums_ready, 3);
       }
