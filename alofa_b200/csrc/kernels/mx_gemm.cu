@@ -50,12 +50,17 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
 }
 // A weight's tile: 128 rows of codes (a tile is 136 rows of 64 bytes, the last eight its scales); 8,192 bytes are counted.
+// The same by either CTA of a pair; bar: the first CTA's barrier.
+__device__ __forceinline__ void load_tile_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ void load_bytes(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-// Ends early: what is still in flight lands in a bounded time.
+// After a wait that ran out: what is still in flight ends in a bounded time.
+constexpr uint32_t DRAIN_LIMIT = 1u << 14;
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
-  for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(bar, parity); ++w) {
+  for (uint32_t w = 0; w < DRAIN_LIMIT && !mbar_try_wait(bar, parity); ++w) {
   }
 }
 
@@ -344,14 +349,21 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
 //
 // Tensor memory holds 512 columns: two accumulators of 256 and the scales do not fit.  The accumulators therefore
 // share 64 columns (0-255 and 192-447), and the epilogue takes those first: the next tile's products begin when it has
-// them in registers, and run beside the rest of the epilogue.  Scales have a place for each stage of the ring: those of
-// a slice are written when the products of the slice before it there are complete.
+// them in registers, and run beside the rest of the epilogue.  Scales have five places in turn: those of a slice are
+// written when the products of the slice before it there are complete.
+//
+// A slice's way round the ring (its room freed, its copies asked for, landed, its products issued, complete) takes
+// several times as long as its products, so nothing may stand on it that need not: the copies of both CTAs count on
+// the first one's barrier, and the tokens' scales, which no copy of the tensor kind can fetch (rows of 4 bytes a slice),
+// come eight slices at a time, ahead of the ring, by loads of a warp of their own.
 // ---------------------------------------------------------------------------
-constexpr int PAIR_THREADS = 384;  // warp 0 weights, 1 tokens, 2 products (second CTA: tells the first what has landed), 4-11 epilogue
-constexpr int PAIR_STAGES = 5;
-constexpr uint32_t PAIR_STAGE_BYTES = 2 * 128 * MX_GROUP + 2048;  // tokens, weight rows, 512 bytes of the tokens' scales, 1,024 of the weight's
-constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 1024;
-constexpr uint32_t PAIR_SECOND = 192, PAIR_SCALES = 448;  // columns of the second accumulator, and of 12 for a stage's scales
+constexpr int PAIR_THREADS = 384;  // warp 0 weights, 1 tokens, 2 products (first CTA), 3 the tokens' scales, 4-11 epilogue
+constexpr int PAIR_STAGES = 6;
+constexpr uint32_t PAIR_STAGE_BYTES = 2 * 128 * MX_GROUP + 1024;  // tokens, weight rows, the scales of 256 weight rows
+constexpr int PAIR_CHUNK = 8;  // slices whose token scales are fetched together: 512 bytes each, two chunks' room
+constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 2 * PAIR_CHUNK * 512 + 1024;
+constexpr uint32_t PAIR_SECOND = 192, PAIR_SCALES = 448;  // columns of the second accumulator, and of the scales
+constexpr int PAIR_SCALE_PLACES = 5;  // of 12 columns
 
 __device__ __forceinline__ void pair_load64(uint32_t tmem, uint32_t (&r)[64]) {
 #pragma unroll
@@ -437,13 +449,13 @@ __device__ __forceinline__ void pair_finish64(const MxArgs& args, const uint32_t
   }
 }
 
-__global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MxArgs args) {
+__global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_x, const MxArgs args) {
   constexpr int STAGES = PAIR_STAGES;
   constexpr uint32_t A_BYTES = 128 * MX_GROUP, B_BYTES = 128 * MX_GROUP;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  // landed: the copies of a slice, in the first CTA those of both; sums_ready, sums_taken: a tile's accumulator
-  __shared__ uint64_t landed[STAGES], stage_free[STAGES], sums_ready, sums_taken, gave_up;
+  // landed (first CTA): the copies of a slice, those of both CTAs; scales_in (first CTA), chunk_free: a chunk of the tokens' scales; sums_ready, sums_taken: a tile's accumulator
+  __shared__ uint64_t landed[STAGES], stage_free[STAGES], scales_in[2], chunk_free[2], sums_ready, sums_taken, gave_up;
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
 
@@ -455,8 +467,12 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&landed[s], 1 + 1 + 32 + (rank == 0 ? 1 : 0));  // the weight's bytes, the tokens', the copies of their scales; the second CTA's word
+      mbar_init(&landed[s], 1);
       mbar_init(&stage_free[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&scales_in[b], 2);
+      mbar_init(&chunk_free[b], 1);
     }
     mbar_init(&sums_ready, 1);
     mbar_init(&sums_taken, 16);  // the epilogue warps of both CTAs
@@ -469,112 +485,121 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = tmem_base_smem;
 
-  if (warp == 0) {
+  const uint32_t chunk_room = tiles + STAGES * PAIR_STAGE_BYTES;
+  if (warp < 2) {
+    // warp 0 the weight's rows and the scales of all 256, warp 1 the tokens: both CTAs' copies count on the first one's barrier
+    if (warp == 1) {
+      pdl_wait();
+      pdl_launch();
+    }
     if (lane == 0) {
       int it = 0, s = 0;  // slices asked for so far, over all tiles; the ring's stage
       uint32_t round = 1;  // parity of the phase in which it was last freed; the first round waits for nothing
       bool ok = true, free = true;
+      const uint32_t first_landed = in_cluster_cta(&landed[0], 0);
       for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
         // a number of rows that is no multiple of 256 leaves the second CTA without any: it reads the last ones, and what comes of them is not stored
         const int even = tile % f_tiles * 2 * slices, odd = min(tile % f_tiles * 2 + 1, last_weight_tile) * slices;
+        const int t0 = tile / f_tiles * 256 + (int)rank * 128;
         for (int i = 0; i < slices; ++i, ++it) {
           if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) {
             ok = false;
             break;
           }
-          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES + 512;
-          uint64_t* bar = &landed[s];
+          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, bar = first_landed + (uint32_t)s * 8;
+          uint64_t* mine = &landed[s];
           s = s + 1 == STAGES ? 0 : s + 1;
           round ^= s == 0 ? 1u : 0u;
           free = it + 1 < STAGES || mbar_complete(&stage_free[s], round);
-          mbar_expect_tx(bar, MX_TILE_CODES + 1024);
-          load_tile(stage + A_BYTES, &map_w, bar, 0, ((rank ? odd : even) + i) * MX_TILE_MAP_ROWS);
-          load_bytes(scales, args.tiles + (size_t)(even + i) * MX_TILE_BYTES + MX_TILE_CODES, 512, bar);
-          load_bytes(scales + 512, args.tiles + (size_t)(odd + i) * MX_TILE_BYTES + MX_TILE_CODES, 512, bar);
+          if (warp == 0) {
+            if (rank == 0) mbar_expect_tx(mine, 2 * (A_BYTES + MX_TILE_CODES + 1024));
+            load_tile_pair(stage + A_BYTES, &map_w, bar, 0, ((rank ? odd : even) + i) * MX_TILE_MAP_ROWS);
+            load_tile_pair(stage + A_BYTES + B_BYTES, &map_s, bar, 0, (even + i) * MX_TILE_MAP_ROWS + MX_TILE_ROWS);
+            load_tile_pair(stage + A_BYTES + B_BYTES + 512, &map_s, bar, 0, (odd + i) * MX_TILE_MAP_ROWS + MX_TILE_ROWS);
+          } else {
+            load_tile_pair(stage, &map_x, bar, i * MX_GROUP, t0);
+          }
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 3) {
     pdl_wait();
-    pdl_launch();
     const int row_bytes = 4 * slices;
-    int it = 0, s = 0;
-    uint32_t round = 1;
-    bool ok = true, free = true;
+    const bool wide = slices % 4 == 0 && (uintptr_t)args.x_scales % 16 == 0;
+    const uint32_t tell = in_cluster_cta(&scales_in[0], 0);
+    int c = 0;  // chunks so far
+    bool ok = true;
     for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
       const int t0 = tile / f_tiles * 256 + (int)rank * 128;
-      for (int i = 0; i < slices; ++i, ++it) {
-        if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) {
-          ok = false;
-          break;
-        }
-        const uint32_t stage = tiles + s * PAIR_STAGE_BYTES;
-        uint64_t* bar = &landed[s];
-        s = s + 1 == STAGES ? 0 : s + 1;
-        round ^= s == 0 ? 1u : 0u;
-        free = it + 1 < STAGES || mbar_complete(&stage_free[s], round);
-        if (lane == 0) {
-          mbar_expect_tx(bar, A_BYTES);
-          load_tile(stage, &map_x, bar, i * MX_GROUP, t0);
-        }
+      for (int i = 0; i < slices; i += PAIR_CHUNK, ++c) {
+        const int have = min(PAIR_CHUNK, slices - i);
+        uint32_t v[4][PAIR_CHUNK];
 #pragma unroll
-        for (int r = 0; r < 128; r += 32)
-          if (t0 + r + lane < args.T) copy4(stage + A_BYTES + B_BYTES + (uint32_t)mx_scale_at(r + lane, 0), args.x_scales + (size_t)(t0 + r + lane) * row_bytes + 4 * i);
-        arrive_when_landed(bar);
+        for (int r = 0; r < 4; ++r) {  // a lane has rows lane, 32 + lane, ...
+          const int t = t0 + r * 32 + lane;
+          const uint8_t* src = args.x_scales + (size_t)min(t, args.T - 1) * row_bytes + 4 * i;
+          if (wide && have >= 4) {
+            const uint4 a = *reinterpret_cast<const uint4*>(src);
+            const uint4 b = have == 8 ? *reinterpret_cast<const uint4*>(src + 16) : make_uint4(0u, 0u, 0u, 0u);
+            v[r][0] = a.x, v[r][1] = a.y, v[r][2] = a.z, v[r][3] = a.w, v[r][4] = b.x, v[r][5] = b.y, v[r][6] = b.z, v[r][7] = b.w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < PAIR_CHUNK; ++j) v[r][j] = j < have ? *reinterpret_cast<const uint32_t*>(src + 4 * j) : 0u;
+          }
+        }
+        if (c >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&chunk_free[c & 1], (uint32_t)(c / 2 - 1) & 1u, &abort_flag));
+        if (!ok) break;
+        const uint32_t room = chunk_room + (uint32_t)((c & 1) * PAIR_CHUNK * 512 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < PAIR_CHUNK; ++j)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(room + j * 512), "r"(v[0][j]), "r"(v[1][j]), "r"(v[2][j]), "r"(v[3][j]) : "memory");
+        fence_to_tensor_core();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_in_cluster(tell + (uint32_t)(c & 1) * 8);
       }
     }
-    if (*(volatile int*)&abort_flag)
-      for (int j = max(0, it - STAGES); j < it; ++j) drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
   } else if (warp == 2) {
-    if (lane == 0 && rank == 1) {
-      int s = 0;
+    if (lane == 0 && rank == 0) {
+      int done = 0, it = 0, c = 0, s = 0, place = 0;  // tiles begun, slices and chunks so far, the ring's stage, the scales' place
       uint32_t round = 0;
-      bool ok = true, ready = false;
-      const uint32_t first_landed = in_cluster_cta(&landed[0], 0);
-      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs)
-        for (int i = 0; i < slices; ++i) {
-          if (!ready) ok = mbar_wait(&landed[s], round, &abort_flag);
-          if (!ok) break;
-          const uint32_t tell = first_landed + (uint32_t)s * 8;
-          s = s + 1 == STAGES ? 0 : s + 1;
-          round ^= s == 0 ? 1u : 0u;
-          ready = mbar_complete(&landed[s], round);
-          fence_to_tensor_core();
-          mbar_arrive_in_cluster(tell);
-        }
-    } else if (lane == 0) {
-      int done = 0, s = 0;  // tiles begun, the ring's stage
-      uint32_t round = 0;
-      bool ok = true, ready = false;
+      bool ok = true, ready = false, place_free = true;
       for (int tile = pair; tile < n_tiles && ok; tile += n_pairs, ++done) {
         if (done) ok = mbar_wait_in_cluster(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag);
         if (!ok) break;
         tc_fence_after();
         const uint32_t sums = tmem + (done & 1 ? PAIR_SECOND : 0);
-        for (int i = 0; i < slices; ++i) {
-          if (!ready) ok = mbar_wait_in_cluster(&landed[s], round, &abort_flag);
+        for (int i = 0; i < slices; ++i, ++it) {
+          if (i % PAIR_CHUNK == 0) ok = mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag);
+          if (ok && !ready) ok = mbar_wait_in_cluster(&landed[s], round, &abort_flag);
+          // the slice before it in this place of the scales: five slices ago, whose stage is the next one's now
+          if (ok && !place_free) ok = mbar_wait(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it - PAIR_SCALE_PLACES) / STAGES) & 1u, &abort_flag);
           if (!ok) break;
           const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES;
-          const uint32_t scale_a = tmem + PAIR_SCALES + s * 12, scale_b = scale_a + 4;
+          const uint32_t token_scales = chunk_room + (uint32_t)((c & 1) * PAIR_CHUNK + i % PAIR_CHUNK) * 512;
+          const uint32_t scale_a = tmem + PAIR_SCALES + place * 12, scale_b = scale_a + 4;
           uint64_t* freed = &stage_free[s];
           s = s + 1 == STAGES ? 0 : s + 1;
+          place = place + 1 == PAIR_SCALE_PLACES ? 0 : place + 1;
           round ^= s == 0 ? 1u : 0u;
-          fence_to_tensor_core();
           tc_fence_after();
           ready = mbar_complete_in_cluster(&landed[s], round);
-          scales_to_tmem_pair(scale_a, scales);
-          scales_to_tmem_pair(scale_b, scales + 512);
-          scales_to_tmem_pair(scale_b + 4, scales + 1024);
+          place_free = it + 1 < PAIR_SCALE_PLACES || mbar_complete(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it + 1 - PAIR_SCALE_PLACES) / STAGES) & 1u);
+          scales_to_tmem_pair(scale_a, token_scales);
+          scales_to_tmem_pair(scale_b, scales);
+          scales_to_tmem_pair(scale_b + 4, scales + 512);
           const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + A_BYTES);
 #pragma unroll
           for (int j = 0; j < 4; ++j) umma_mx_pair(sums, a + 2 * j, b + 2 * j, mx_idesc(E4M3, E2M1, 256, 256, j), scale_a, scale_b, (i | j) ? 1u : 0u);
           umma_commit_pair(freed, 3);
+          if (i % PAIR_CHUNK == PAIR_CHUNK - 1 || i == slices - 1) umma_commit_pair(&chunk_free[c++ & 1], 3);
         }
         if (ok) umma_commit_pair(&sums_ready, 3);
       }
       if (!ok) {  // the products issued so far end before tensor memory is given back
         umma_commit_pair(&gave_up, 3);
         drain(&gave_up, 0);
+        // and the copies asked for land
+        for (int j = 0; j < STAGES; ++j) drain(&landed[j], 0), drain(&landed[j], 1);
       }
     }
   } else if (warp >= 4) {
@@ -607,7 +632,6 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
       tc_fence_before();
     }
   }
-  if (warp == 1) copies_wait();  // landed long ago, unless a wait ran out
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves, or frees tensor memory, while the other may still signal or read it
@@ -631,17 +655,21 @@ static bool make_rows_map(CUtensorMap* map, const void* base, uint64_t rows, uin
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A weight's tiles as rows of 64 bytes, 128 numbers of 4 bits, seen as boxes of 128 rows; 128 bytes at `map`.
-ALOFA_API int alofa_mx_weight_map(void* map, const void* tiles, long long n_tiles) {
+// Two maps of a weight's tiles as rows of 64 bytes, 256 bytes at `maps`: 128 numbers of 4 bits, boxes of 128 rows (a tile's
+// codes, unpacked on the way); bytes, boxes of 8 rows (its scales).
+ALOFA_API int alofa_mx_weight_maps(void* maps, const void* tiles, long long n_tiles) {
   EncodeTiledFn fn = encode_fn();
   if (!fn || (uintptr_t)tiles % 32 || n_tiles <= 0 || n_tiles * MX_TILE_MAP_ROWS > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
-  cuuint64_t dims[2] = {MX_GROUP, (cuuint64_t)(n_tiles * MX_TILE_MAP_ROWS)}, strides[1] = {MX_GROUP / 2};
-  cuuint32_t box[2] = {MX_GROUP, MX_TILE_ROWS}, elem[2] = {1, 1};
-  CUtensorMap m;
-  if (fn(&m, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(tiles), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  cuuint64_t rows = (cuuint64_t)(n_tiles * MX_TILE_MAP_ROWS), codes[2] = {MX_GROUP, rows}, bytes[2] = {MX_GROUP / 2, rows}, strides[1] = {MX_GROUP / 2};
+  cuuint32_t codes_box[2] = {MX_GROUP, MX_TILE_ROWS}, bytes_box[2] = {MX_GROUP / 2, MX_TILE_MAP_ROWS - MX_TILE_ROWS}, elem[2] = {1, 1};
+  CUtensorMap m[2];
+  if (fn(&m[0], CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(tiles), codes, strides, codes_box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return ALOFA_ERR_ARGUMENT;
-  memcpy(map, &m, sizeof(m));
+  if (fn(&m[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(tiles), bytes, strides, bytes_box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return ALOFA_ERR_ARGUMENT;
+  memcpy(maps, m, sizeof(m));
   return ALOFA_OK;
 }
 
@@ -670,8 +698,8 @@ static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const 
 
 // bn: 256: pairs of CTAs (`parts` 1, a grid of `ctas` of them); 16, 32, 64 or 128 tokens a CTA, the depth in `parts` parts.
 // features > 0: out are the codes and out_scales the scales of that many gated features, n the rows of the gated weight.
-// weight_map: alofa_mx_weight_map's of the tiles.
-ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, const void* x_scales, const void* tiles, const void* weight_map, const float* bias, const float* add, int t, int n, int k, int features,
+// weight_maps: alofa_mx_weight_maps' of the tiles.
+ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, const void* x_scales, const void* tiles, const void* weight_maps, const float* bias, const float* add, int t, int n, int k, int features,
                             float gate_alpha, float gate_limit, int bn, int parts, int ctas, int out_bf16, int* status, void* stream) {
   if (t < 0 || n <= 0 || k <= 0 || k > (1 << 30) || n > (1 << 30) || (uintptr_t)x_codes % 16 || (uintptr_t)x_scales % 4 || (uintptr_t)tiles % 32) return ALOFA_ERR_ARGUMENT;
   if (features < 0 || (features && (n != 2 * ((features + 15) / 16 * 16) || !out_scales || (uintptr_t)out % 16))) return ALOFA_ERR_ARGUMENT;
@@ -685,8 +713,9 @@ ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, co
   const bool few = bn == 16 || bn == 32 || bn == 64 || bn == 128;
   if (!few && bn != 256) return ALOFA_ERR_ARGUMENT;
   if (parts < 1 || parts > args.slices || parts > (few ? FEW_PARTS : 1)) return ALOFA_ERR_ARGUMENT;
-  CUtensorMap map_w, map_x;
-  memcpy(&map_w, weight_map, sizeof(map_w));
+  CUtensorMap map_w, map_s, map_x;
+  memcpy(&map_w, weight_maps, sizeof(map_w));
+  memcpy(&map_s, (const uint8_t*)weight_maps + sizeof(map_w), sizeof(map_s));
   if (!make_rows_map(&map_x, x_codes, (uint64_t)t, (uint64_t)args.slices * MX_GROUP, few ? bn : 128)) return ALOFA_ERR_ARGUMENT;
   cudaStream_t s = (cudaStream_t)stream;
   switch (bn) {
@@ -699,6 +728,6 @@ ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, co
   if (ctas < 2 || pair_tiles > 0x3fffffffll) return ALOFA_ERR_ARGUMENT;
   if (!allow_shared((const void*)mx_pair_kernel, (int)PAIR_SMEM, pair_allowed)) return ALOFA_ERR_LAUNCH;
   const long long grid = 2 * pair_tiles < ctas ? 2 * pair_tiles : ctas / 2 * 2;
-  launch_dep_cluster(mx_pair_kernel, dim3((unsigned)grid), PAIR_THREADS, PAIR_SMEM, s, 2, map_w, map_x, args);
+  launch_dep_cluster(mx_pair_kernel, dim3((unsigned)grid), PAIR_THREADS, PAIR_SMEM, s, 2, map_w, map_s, map_x, args);
   return launch_status();
 }

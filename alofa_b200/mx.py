@@ -146,7 +146,7 @@ class MxWeight:
     are a gate's, the second an up projection's.  Made by :func:`pack_weight`
     or :meth:`from_codes`."""
 
-    __slots__ = ("tiles", "n", "k", "gated", "rows", "device", "at", "map")
+    __slots__ = ("tiles", "n", "k", "gated", "rows", "device", "at", "maps")
 
     def __init__(self, n: int, k: int, gated: bool, here: int):
         if n <= 0 or k <= 0 or (gated and n % 2):
@@ -156,9 +156,9 @@ class MxWeight:
         self.rows = 2 * (-(-(n // 2) // GATE_ROWS) * GATE_ROWS) if gated else n
         self.tiles = torch.empty((-(-self.rows // TILE_ROWS), padded(k) // GROUP, TILE_BYTES), dtype=_U8, device=here)
         self.at = self.tiles.data_ptr()
-        #: how the copies of the product see the tiles (a tensor map)
-        self.map = ctypes.create_string_buffer(128)
-        ops.mx_launched(ops.mx_library().alofa_mx_weight_map(self.map, self.at, self.tiles.shape[0] * self.tiles.shape[1]), 0, "mx weight", lambda: f"rows={n} depth={k}")
+        #: how the copies of the product see the tiles (two tensor maps)
+        self.maps = ctypes.create_string_buffer(256)
+        ops.mx_launched(ops.mx_library().alofa_mx_weight_maps(self.maps, self.at, self.tiles.shape[0] * self.tiles.shape[1]), 0, "mx weight", lambda: f"rows={n} depth={k}")
 
     @classmethod
     def from_codes(cls, codes, scales, k: int, gated: bool = False) -> "MxWeight":
@@ -199,7 +199,7 @@ class MxWeight:
             raise AlofaError("invalid_argument", "the first rows of a weight that is not gated", f"rows={n} of {self.n} gated={self.gated}")
         part = MxWeight.__new__(MxWeight)
         part.n, part.rows, part.k, part.gated, part.device = n, n, self.k, False, self.device
-        part.tiles, part.at, part.map = self.tiles[: -(-n // TILE_ROWS)], self.at, self.map
+        part.tiles, part.at, part.maps = self.tiles[: -(-n // TILE_ROWS)], self.at, self.maps
         return part
 
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
@@ -299,7 +299,7 @@ def _product(x: MxRows, w: MxWeight, out_at, scales_at, bias_at, add_at, feature
     bn, parts = how or plan(x.rows, w.rows, w.k)
     status_at = None if status is None else _at(status, "status", _I32, status.shape, here)
     rc = ops.mx_library().alofa_mx_gemm(
-        out_at, scales_at, x.codes_at, x.scales_at, w.at, w.map, bias_at, add_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16, status_at, _stream(here)
+        out_at, scales_at, x.codes_at, x.scales_at, w.at, w.maps, bias_at, add_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16, status_at, _stream(here)
     )
     ops.mx_launched(rc, 1, what, lambda: f"tokens={x.rows} rows={w.rows} depth={w.k} how={(bn, parts)}")
 
