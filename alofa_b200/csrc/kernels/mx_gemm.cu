@@ -57,6 +57,22 @@ __device__ __forceinline__ void load_tile_pair(uint32_t dst, const CUtensorMap* 
 __device__ __forceinline__ void load_bytes(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+// The warps that copy and issue run their loops whole, every lane through the same waits and counters, and only the
+// instructions themselves are one lane's: what those take (addresses, descriptors, barriers) then stands in uniform
+// registers.  With the whole loop inside `if (lane == 0)` each tcgen05 instruction took 65 to 100 clocks to issue, and a
+// slice of the pair kernel 1,060 where its products take 512.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t chosen;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(chosen));
+  return chosen != 0;
+}
+__device__ __forceinline__ bool all_lanes(bool v) { return __all_sync(0xffffffffu, v); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }  // a value that every lane has
+
 // After a wait that ran out: what is still in flight ends in a bounded time.
 constexpr uint32_t DRAIN_LIMIT = 1u << 14;
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
@@ -197,7 +213,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int part = blockIdx.x % parts, f_tile = blockIdx.x / parts;  // a cluster: the parts of one tile's depth
   const int f0 = f_tile * MX_TILE_ROWS, t0 = blockIdx.y * BN;
   // parts that differ by one slice at most
@@ -218,18 +234,19 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   const uint32_t tmem = tmem_base_smem;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int i = 0, s = 0;
-      uint32_t round = 1;  // parity of the phase in which this stage was last freed; the first round waits for nothing
-      bool free = true;
-      for (; i < n; ++i) {
-        if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) break;
-        const uint32_t stage = tiles + s * Tile::STAGE_BYTES;
-        const int tile = f_tile * args.slices + first + i;
-        uint64_t* bar = &landed[s];
-        s = s + 1 == STAGES ? 0 : s + 1;
-        round ^= s == 0 ? 1u : 0u;
-        free = i + 1 < STAGES || mbar_complete(&stage_free[s], round);
+    const bool chosen = elect_lane();
+    int i = 0, s = 0;
+    uint32_t round = 1;  // parity of the phase in which this stage was last freed; the first round waits for nothing
+    bool free = true;
+    for (; i < n; ++i) {
+      if (!all_lanes(free) && !all_lanes(mbar_wait(&stage_free[s], round, &abort_flag))) break;
+      const uint32_t stage = tiles + s * Tile::STAGE_BYTES;
+      const int tile = f_tile * args.slices + first + i;
+      uint64_t* bar = &landed[s];
+      s = s + 1 == STAGES ? 0 : s + 1;
+      round ^= s == 0 ? 1u : 0u;
+      free = i + 1 < STAGES || mbar_complete(&stage_free[s], round);
+      if (chosen) {
         mbar_expect_tx(bar, MX_TILE_BYTES);
         load_tile(stage, &map_w, bar, 0, tile * MX_TILE_MAP_ROWS);
         load_bytes(stage + Tile::A_BYTES + Tile::B_BYTES, args.tiles + (size_t)tile * MX_TILE_BYTES + MX_TILE_CODES, MX_TILE_BYTES - MX_TILE_CODES, bar);
@@ -238,18 +255,19 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   } else if (warp == 4) {
     pdl_wait();
     pdl_launch();
+    const bool chosen = elect_lane();
     const int row_bytes = 4 * args.slices;
     int i = 0, s = 0;
     uint32_t round = 1;
     bool free = true;
     for (; i < n; ++i) {
-      if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) break;
+      if (!all_lanes(free) && !all_lanes(mbar_wait(&stage_free[s], round, &abort_flag))) break;
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES + 512;
       uint64_t* bar = &landed[s];
       s = s + 1 == STAGES ? 0 : s + 1;
       round ^= s == 0 ? 1u : 0u;
       free = i + 1 < STAGES || mbar_complete(&stage_free[s], round);
-      if (lane == 0) {
+      if (chosen) {
         mbar_expect_tx(bar, Tile::B_BYTES);
         load_tile(stage + Tile::A_BYTES, &map_x, bar, (first + i) * MX_GROUP, t0);
       }
@@ -263,28 +281,32 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
     if (*(volatile int*)&abort_flag)
       for (int j = max(0, i - STAGES); j < i; ++j) drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
   } else if (warp == 5) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t round = 0;
-      bool ok = true, ready = false;
-      for (int i = 0; i < n; ++i) {
-        if (!ready) ok = mbar_wait(&landed[s], round, &abort_flag);
-        if (!ok) break;
-        const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES;
-        const uint32_t scale_a = tmem + BN + s * 8, scale_b = scale_a + 4;
-        uint64_t* freed = &stage_free[s];
-        s = s + 1 == STAGES ? 0 : s + 1;
-        round ^= s == 0 ? 1u : 0u;
-        fence_to_tensor_core();
-        tc_fence_after();
-        ready = i + 1 < n && mbar_complete(&landed[s], round);
+    const bool chosen = elect_lane();
+    const uint32_t sums = uniform(tmem);
+    int s = 0;
+    uint32_t round = 0;
+    bool ok = true, ready = false;
+    for (int i = 0; i < n; ++i) {
+      if (!all_lanes(ready)) ok = all_lanes(mbar_wait(&landed[s], round, &abort_flag));
+      if (!ok) break;
+      const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES;
+      const uint32_t scale_a = sums + BN + s * 8, scale_b = scale_a + 4;
+      uint64_t* freed = &stage_free[s];
+      s = s + 1 == STAGES ? 0 : s + 1;
+      round ^= s == 0 ? 1u : 0u;
+      fence_to_tensor_core();
+      tc_fence_after();
+      ready = i + 1 < n && mbar_complete(&landed[s], round);
+      const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + Tile::A_BYTES);
+      if (chosen) {
         scales_to_tmem(scale_a, scales);
         scales_to_tmem(scale_b, scales + 512);
-        const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + Tile::A_BYTES);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) umma_mx(tmem, a + 2 * j, b + 2 * j, mx_idesc(E2M1, E4M3, 128, BN, j), scale_a, scale_b, (i | j) ? 1u : 0u);
+        for (int j = 0; j < 4; ++j) umma_mx(sums, a + 2 * j, b + 2 * j, mx_idesc(E2M1, E4M3, 128, BN, j), scale_a, scale_b, (i | j) ? 1u : 0u);
         umma_commit(freed);
       }
+    }
+    if (chosen) {
       umma_commit(&sums_done);
       if (!ok) drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
     }
@@ -459,8 +481,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cta_in_cluster();
+  const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const uint32_t rank = uniform(cta_in_cluster());
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, slices = args.slices;
   const int f_tiles = (args.N + 255) / 256, n_tiles = f_tiles * ((args.T + 255) / 256);  // the weight's tiles innermost
   const int last_weight_tile = (args.N + MX_TILE_ROWS - 1) / MX_TILE_ROWS - 1;
@@ -492,25 +514,24 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
       pdl_wait();
       pdl_launch();
     }
-    if (lane == 0) {
-      int it = 0, s = 0;  // slices asked for so far, over all tiles; the ring's stage
-      uint32_t round = 1;  // parity of the phase in which it was last freed; the first round waits for nothing
-      bool ok = true, free = true;
-      const uint32_t first_landed = in_cluster_cta(&landed[0], 0);
-      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
-        // a number of rows that is no multiple of 256 leaves the second CTA without any: it reads the last ones, and what comes of them is not stored
-        const int even = tile % f_tiles * 2 * slices, odd = min(tile % f_tiles * 2 + 1, last_weight_tile) * slices;
-        const int t0 = tile / f_tiles * 256 + (int)rank * 128;
-        for (int i = 0; i < slices; ++i, ++it) {
-          if (!free && !mbar_wait(&stage_free[s], round, &abort_flag)) {
-            ok = false;
-            break;
-          }
-          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, bar = first_landed + (uint32_t)s * 8;
-          uint64_t* mine = &landed[s];
-          s = s + 1 == STAGES ? 0 : s + 1;
-          round ^= s == 0 ? 1u : 0u;
-          free = it + 1 < STAGES || mbar_complete(&stage_free[s], round);
+    const bool chosen = elect_lane();
+    int it = 0, s = 0;  // slices asked for so far, over all tiles; the ring's stage
+    uint32_t round = 1;  // parity of the phase in which it was last freed; the first round waits for nothing
+    bool ok = true, free = true;
+    const uint32_t first_landed = uniform(in_cluster_cta(&landed[0], 0));
+    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+      // a number of rows that is no multiple of 256 leaves the second CTA without any: it reads the last ones, and what comes of them is not stored
+      const int even = tile % f_tiles * 2 * slices, odd = min(tile % f_tiles * 2 + 1, last_weight_tile) * slices;
+      const int t0 = tile / f_tiles * 256 + (int)rank * 128;
+      for (int i = 0; i < slices; ++i, ++it) {
+        if (!all_lanes(free)) ok = all_lanes(mbar_wait(&stage_free[s], round, &abort_flag));
+        if (!ok) break;
+        const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, bar = first_landed + (uint32_t)s * 8;
+        uint64_t* mine = &landed[s];
+        s = s + 1 == STAGES ? 0 : s + 1;
+        round ^= s == 0 ? 1u : 0u;
+        free = it + 1 < STAGES || mbar_complete(&stage_free[s], round);
+        if (chosen) {
           if (warp == 0) {
             if (rank == 0) mbar_expect_tx(mine, 2 * (A_BYTES + MX_TILE_CODES + 1024));
             load_tile_pair(stage + A_BYTES, &map_w, bar, 0, ((rank ? odd : even) + i) * MX_TILE_MAP_ROWS);
@@ -559,24 +580,26 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
       }
     }
   } else if (warp == 2) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool chosen = elect_lane();
+      const uint32_t base = uniform(tmem);
       int done = 0, it = 0, c = 0, s = 0, place = 0;  // tiles begun, slices and chunks so far, the ring's stage, the scales' place
       uint32_t round = 0;
       bool ok = true, ready = false, place_free = true;
       for (int tile = pair; tile < n_tiles && ok; tile += n_pairs, ++done) {
-        if (done) ok = mbar_wait_in_cluster(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag);
+        if (done) ok = all_lanes(mbar_wait_in_cluster(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t sums = tmem + (done & 1 ? PAIR_SECOND : 0);
+        const uint32_t sums = base + (done & 1 ? PAIR_SECOND : 0);
         for (int i = 0; i < slices; ++i, ++it) {
-          if (i % PAIR_CHUNK == 0) ok = mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag);
-          if (ok && !ready) ok = mbar_wait_in_cluster(&landed[s], round, &abort_flag);
+          if (i % PAIR_CHUNK == 0) ok = all_lanes(mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag));
+          if (ok && !all_lanes(ready)) ok = all_lanes(mbar_wait_in_cluster(&landed[s], round, &abort_flag));
           // the slice before it in this place of the scales: five slices ago, whose stage is the next one's now
-          if (ok && !place_free) ok = mbar_wait(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it - PAIR_SCALE_PLACES) / STAGES) & 1u, &abort_flag);
+          if (ok && !all_lanes(place_free)) ok = all_lanes(mbar_wait(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it - PAIR_SCALE_PLACES) / STAGES) & 1u, &abort_flag));
           if (!ok) break;
           const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES;
           const uint32_t token_scales = chunk_room + (uint32_t)((c & 1) * PAIR_CHUNK + i % PAIR_CHUNK) * 512;
-          const uint32_t scale_a = tmem + PAIR_SCALES + place * 12, scale_b = scale_a + 4;
+          const uint32_t scale_a = base + PAIR_SCALES + place * 12, scale_b = scale_a + 4;
           uint64_t* freed = &stage_free[s];
           s = s + 1 == STAGES ? 0 : s + 1;
           place = place + 1 == PAIR_SCALE_PLACES ? 0 : place + 1;
@@ -584,18 +607,22 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
           tc_fence_after();
           ready = mbar_complete_in_cluster(&landed[s], round);
           place_free = it + 1 < PAIR_SCALE_PLACES || mbar_complete(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it + 1 - PAIR_SCALE_PLACES) / STAGES) & 1u);
-          scales_to_tmem_pair(scale_a, token_scales);
-          scales_to_tmem_pair(scale_b, scales);
-          scales_to_tmem_pair(scale_b + 4, scales + 512);
           const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + A_BYTES);
+          const bool chunk_ends = i % PAIR_CHUNK == PAIR_CHUNK - 1 || i == slices - 1;
+          if (chosen) {
+            scales_to_tmem_pair(scale_a, token_scales);
+            scales_to_tmem_pair(scale_b, scales);
+            scales_to_tmem_pair(scale_b + 4, scales + 512);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) umma_mx_pair(sums, a + 2 * j, b + 2 * j, mx_idesc(E4M3, E2M1, 256, 256, j), scale_a, scale_b, (i | j) ? 1u : 0u);
-          umma_commit_pair(freed, 3);
-          if (i % PAIR_CHUNK == PAIR_CHUNK - 1 || i == slices - 1) umma_commit_pair(&chunk_free[c++ & 1], 3);
+            for (int j = 0; j < 4; ++j) umma_mx_pair(sums, a + 2 * j, b + 2 * j, mx_idesc(E4M3, E2M1, 256, 256, j), scale_a, scale_b, (i | j) ? 1u : 0u);
+            umma_commit_pair(freed, 3);
+            if (chunk_ends) umma_commit_pair(&chunk_free[c & 1], 3);
+          }
+          c += chunk_ends ? 1 : 0;
         }
-        if (ok) umma_commit_pair(&sums_ready, 3);
+        if (ok && chosen) umma_commit_pair(&sums_ready, 3);
       }
-      if (!ok) {  // the products issued so far end before tensor memory is given back
+      if (!ok && chosen) {  // the products issued so far end before tensor memory is given back
         umma_commit_pair(&gave_up, 3);
         drain(&gave_up, 0);
         // and the copies asked for land
