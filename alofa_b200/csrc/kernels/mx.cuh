@@ -98,21 +98,22 @@ __device__ __forceinline__ void mx_put8(const float (&v)[8], uint8_t* codes, uin
   if ((threadIdx.x & 3) == 0) *scale = (uint8_t)s;
 }
 
-// silu(g) * u, or the clamped form (gate_times in common.cuh), where what comes out is rounded to 8 bits: a number near the
-// border of two codes takes the other one if it is off by little, so e^-g is taken with the product g log2(e) in two parts
-// (the rounding of that product alone would cost up to |g| / 2 units in the last place).  ex2.approx is within 2 units, rcp.approx within 1.
+// silu(g) * u, or (CLAMPED) the clamped form (gate_times in common.cuh), where what comes out is rounded to 8 bits: a number
+// near the border of two codes takes the other one if it is off by little, so e^-z is taken with the product z log2(e) in two
+// parts (the rounding of that product alone would cost up to |z| / 2 units in the last place).  ex2.approx is within 2 units,
+// rcp.approx within 1.  From z = -88 down it is zero.
 __device__ __forceinline__ float mx_logistic(float z) {
-  const float hi = -1.4426950408889634f * z;
+  const float hi = fminf(-1.4426950408889634f * z, 126.f);
   const float lo = fmaf(-1.4426950408889634f, z, -hi) - 1.92596299e-8f * z;  // log2(e) is 1.92596299e-8 more than the float
-  float e, r, far;
+  float e, r;
   asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(hi));
   e = fmaf(e, 0.6931471805599453f * lo, e);
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  asm("ex2.approx.f32 %0, %1;" : "=f"(far) : "f"(-hi));
-  return fabsf(hi) < 100.f ? r : hi >= 100.f ? far : hi <= -100.f ? 1.0f : hi;  // far out it is e^z or one; NaN stays
+  return r;
 }
+template <bool CLAMPED>
 __device__ __forceinline__ float mx_gate_times(float g, float u, float alpha, float limit) {
-  if (alpha == 0.f) return g * mx_logistic(g) * u;
+  if (!CLAMPED) return g * mx_logistic(g) * u;
   g = fminf(g, limit);
   u = fminf(fmaxf(u, -limit), limit);
   return g * mx_logistic(alpha * g) * (u + 1.0f);

@@ -152,7 +152,8 @@ __device__ __forceinline__ void few_gated_token(const MxArgs& args, float4 v, in
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float u = __shfl_xor_sync(0xffffffffu, g[j], 4);
-    g[j] = f + j < args.F ? mx_gate_times(g[j], u, args.gate_alpha, args.gate_limit) : 0.f;
+    const float y = args.gate_alpha == 0.f ? mx_gate_times<false>(g[j], u, 0.f, 0.f) : mx_gate_times<true>(g[j], u, args.gate_alpha, args.gate_limit);
+    g[j] = f + j < args.F ? y : 0.f;
   }
   if ((lane & 4) == 0)
 #pragma unroll
@@ -398,33 +399,43 @@ __device__ __forceinline__ void pair_load64(uint32_t tmem, uint32_t (&r)[64]) {
   tmem_ld_wait();
 }
 
-// 64 rows' sums of one token: stored, or (two features' rows for each) one block of codes and its scale.
-__device__ __forceinline__ void pair_finish64(const MxArgs& args, const uint32_t (&r)[64], int t, int row, bool good) {
-  const float nan = __uint_as_float(0x7fc00000u);
-  if (args.F) {
-    const int f = row / 2, fp = (args.F + MX_GROUP - 1) / MX_GROUP * MX_GROUP;
-    if (f >= fp) return;
-    float v[32];
-    uint32_t largest = 0;
+// 64 rows' sums of one token of a gated weight: one block of codes and its scale.  The clamped form and the last
+// features' zeros are told apart once, not for every number: this is what the tensor cores wait for when the depth is short.
+template <bool CLAMPED>
+__device__ __forceinline__ void pair_gated64(const MxArgs& args, const uint32_t (&r)[64], int t, int row, bool good) {
+  const int f = row / 2, fp = (args.F + MX_GROUP - 1) / MX_GROUP * MX_GROUP;
+  if (f >= fp) return;
+  float v[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const int at = (j / 16) * 32 + j % 16;
-      float y = mx_gate_times(__uint_as_float(r[at]), __uint_as_float(r[at + 16]), args.gate_alpha, args.gate_limit);
-      y = good ? y : nan;
-      v[j] = f + j < args.F ? y : 0.f;
-      largest = max(largest, mx_size(v[j]));
-    }
-    const uint32_t s = mx_row_scale(largest);
-    const float over = mx_over(s);
-    uint32_t c[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c[j] = s == 255u ? 0u : mx_e4m3(v[4 * j] * over, v[4 * j + 1] * over, v[4 * j + 2] * over, v[4 * j + 3] * over);
-    uint4* codes = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(args.out) + (size_t)t * fp + f);
-    codes[0] = make_uint4(c[0], c[1], c[2], c[3]);
-    codes[1] = make_uint4(c[4], c[5], c[6], c[7]);
-    args.out_scales[(size_t)t * (fp / MX_BLOCK) + f / MX_BLOCK] = (uint8_t)s;
-    return;
+  for (int j = 0; j < 32; ++j) {
+    const int at = (j / 16) * 32 + j % 16;
+    v[j] = mx_gate_times<CLAMPED>(__uint_as_float(r[at]), __uint_as_float(r[at + 16]), args.gate_alpha, args.gate_limit);
   }
+  if (f + 32 > args.F) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = f + j < args.F ? v[j] : 0.f;
+  }
+  uint32_t largest = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) largest = max(largest, mx_size(v[j]));
+  const uint32_t s = good ? mx_row_scale(largest) : 255u;
+  const float over = mx_over(s);
+  uint32_t c[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = mx_e4m3(v[4 * j] * over, v[4 * j + 1] * over, v[4 * j + 2] * over, v[4 * j + 3] * over);
+  if (s == 255u) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = 0u;
+  }
+  uint4* codes = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(args.out) + (size_t)t * fp + f);
+  codes[0] = make_uint4(c[0], c[1], c[2], c[3]);
+  codes[1] = make_uint4(c[4], c[5], c[6], c[7]);
+  args.out_scales[(size_t)t * (fp / MX_BLOCK) + f / MX_BLOCK] = (uint8_t)s;
+}
+
+// The same sums of a product that is stored.
+__device__ __forceinline__ void pair_stored64(const MxArgs& args, const uint32_t (&r)[64], int t, int row, bool good) {
+  const float nan = __uint_as_float(0x7fc00000u);
   const size_t at = (size_t)t * args.N + row;
 #pragma unroll
   for (int j = 0; j < 64; j += 8) {
@@ -654,7 +665,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
           __syncwarp();
           if (lane == 0) mbar_arrive_in_cluster(taken);
         }
-        if (t < args.T) pair_finish64(args, r, t, row0 + block * 64, good);
+        if (t >= args.T) continue;
+        if (!args.F) pair_stored64(args, r, t, row0 + block * 64, good);
+        else if (args.gate_alpha == 0.f) pair_gated64<false>(args, r, t, row0 + block * 64, good);
+        else pair_gated64<true>(args, r, t, row0 + block * 64, good);
       }
       tc_fence_before();
     }
