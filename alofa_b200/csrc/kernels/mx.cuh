@@ -11,6 +11,8 @@
 // enters.  Dividing by the scale multiplies by a power of two that is a normal number, exact up to
 // what falls below the smallest subnormal code anyway; the conversions round to nearest even.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 
 constexpr int MX_BLOCK = 32;       // numbers that share a scale
@@ -61,16 +63,20 @@ __device__ __forceinline__ uint32_t mx_e2m1(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
-__device__ __forceinline__ float mx_from_e4m3(uint32_t code) {
-  const uint32_t sign = (code & 0x80u) << 24, e = (code >> 3) & 15u, m = code & 7u;
-  if ((code & 0x7fu) == 0x7fu) return __uint_as_float(0x7fc00000u);
-  const float v = e ? __uint_as_float(((e + 120u) << 23) | (m << 20)) : (float)m * (1.0f / 512.0f);
-  return __uint_as_float(__float_as_uint(v) | sign);
+// Two codes' numbers, the first in the low byte (half byte).  Every one of them is a half-precision number.
+__device__ __forceinline__ float2 mx_from_e4m3(uint16_t codes) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(codes));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
-__device__ __forceinline__ float mx_from_e2m1(uint32_t code) {
-  const uint32_t sign = (code & 8u) << 28, e = (code >> 1) & 3u, m = code & 1u;
-  const float v = e ? __uint_as_float(((e + 126u) << 23) | (m << 22)) : 0.5f * (float)m;
-  return __uint_as_float(__float_as_uint(v) | sign);
+__device__ __forceinline__ float2 mx_from_e2m1(uint32_t codes) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
+      : "=r"(h)
+      : "r"(codes));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 
 // The row of a gated weight that holds feature f of the gate (half 0) or of the up projection (half 1).

@@ -5,8 +5,8 @@
 //   alofa_mx_rows_values, alofa_mx_weight_values   the numbers that rows, or a weight, stand for
 // Kp is K rounded up to whole groups of 128; the codes behind K are zeros.
 //
-// All of them are bound by memory: a lane takes eight neighbouring numbers (16 or 32 bytes of input, 8 of
-// rows or 4 of a weight), four lanes have a block and find its largest magnitude by two shuffles.
+// All of them are bound by memory: a lane takes eight or sixteen neighbouring numbers, the lanes that share a
+// block find its largest magnitude by one or two shuffles, and codes are converted by the hardware's instructions.
 #include "mx.cuh"
 
 template <typename T>
@@ -55,66 +55,87 @@ static inline int padded(int k) { return (k + MX_GROUP - 1) / MX_GROUP * MX_GROU
 static inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 // ---------------------------------------------------------------------------
-// Rows
+// Rows: a lane has sixteen neighbouring numbers, two lanes a block.  Lanes are numbered over all rows in 32 bits
+// (a 64-bit division by the row's length was a third of the instructions); what they address is 64.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) mx_rows_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, long long chunks, int k, int kp, bool whole) {
+__global__ void __launch_bounds__(256) mx_rows_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, unsigned chunks, int k, int kp, bool whole) {
   pdl_wait();
   pdl_launch();
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;  // kp / 8 is a multiple of 16: four lanes with a block are in one row
+  const unsigned i = blockIdx.x * blockDim.x + threadIdx.x, per_row = (unsigned)kp >> 4;  // a multiple of 8: a block's two lanes are in one row
   const bool live = i < chunks;
-  const int per_row = kp >> 3;
-  const long long row = live ? i / per_row : 0;
-  const int c = live ? (int)(i - row * per_row) * 8 : 0;
-  float v[8];
-  load8(v, x + row * k + c, live ? k - c : 0, whole);
-  mx_put8(v, codes + row * kp + c, scales + row * (kp / MX_BLOCK) + c / MX_BLOCK, live);
+  const unsigned row = live ? i / per_row : 0u;
+  const int c = live ? (int)(i - row * per_row) * 16 : 0;
+  float v[2][8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) load8(v[h], x + (size_t)row * k + c + 8 * h, live ? k - c - 8 * h : 0, whole);
+  uint32_t largest = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) largest = max(largest, mx_size(v[j >> 3][j & 7]));
+  largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+  if (!live) return;
+  const uint32_t s = mx_row_scale(largest);
+  const float over = mx_over(s);
+  uint4 q = make_uint4(0u, 0u, 0u, 0u);
+  if (s != 255u) {
+    q.x = mx_e4m3(v[0][0] * over, v[0][1] * over, v[0][2] * over, v[0][3] * over);
+    q.y = mx_e4m3(v[0][4] * over, v[0][5] * over, v[0][6] * over, v[0][7] * over);
+    q.z = mx_e4m3(v[1][0] * over, v[1][1] * over, v[1][2] * over, v[1][3] * over);
+    q.w = mx_e4m3(v[1][4] * over, v[1][5] * over, v[1][6] * over, v[1][7] * over);
+  }
+  *reinterpret_cast<uint4*>(codes + (size_t)row * kp + c) = q;
+  if ((threadIdx.x & 1) == 0) scales[(size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK] = (uint8_t)s;
 }
 
 ALOFA_API int alofa_mx_rows(void* codes, void* scales, const void* x, int t, int k, int bf16_x, void* stream) {
-  if (t < 0 || k <= 0 || k > (1 << 30) || !aligned(codes, 8)) return ALOFA_ERR_ARGUMENT;
+  if (t < 0 || k <= 0 || k > (1 << 30) || !aligned(codes, 16)) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
   const int kp = padded(k);
-  const long long chunks = (long long)t * (kp / 8), blocks = (chunks + 255) / 256;
-  if (blocks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  const long long chunks = (long long)t * (kp / 16);
+  if (chunks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  const unsigned blocks = (unsigned)((chunks + 255) / 256);
   const bool whole = k % 8 == 0 && aligned(x, 16);
   if (bf16_x)
-    launch_dep(mx_rows_kernel<bf16>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const bf16*)x, chunks, k, kp, whole);
+    launch_dep(mx_rows_kernel<bf16>, blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const bf16*)x, (unsigned)chunks, k, kp, whole);
   else
-    launch_dep(mx_rows_kernel<float>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const float*)x, chunks, k, kp, whole);
+    launch_dep(mx_rows_kernel<float>, blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const float*)x, (unsigned)chunks, k, kp, whole);
   return launch_status();
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) mx_rows_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long chunks, int k, int kp, bool whole) {
+__global__ void __launch_bounds__(256) mx_rows_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, unsigned chunks, int k, int kp, bool whole) {
   pdl_wait();
   pdl_launch();
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const unsigned i = blockIdx.x * blockDim.x + threadIdx.x, per_row = (unsigned)(k + 15) >> 4;
   if (i >= chunks) return;
-  const int per_row = (k + 7) >> 3;
-  const long long row = i / per_row;
-  const int c = (int)(i - row * per_row) * 8;
-  const uint2 p = *reinterpret_cast<const uint2*>(codes + row * kp + c);
-  const float by = mx_power(scales[row * (kp / MX_BLOCK) + c / MX_BLOCK]);
-  float v[8];
+  const unsigned row = i / per_row;
+  const int c = (int)(i - row * per_row) * 16;
+  const uint4 p = *reinterpret_cast<const uint4*>(codes + (size_t)row * kp + c);
+  const float by = mx_power(scales[(size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK]);
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[j] = mx_from_e4m3((p.x >> (8 * j)) & 255u) * by;
-    v[4 + j] = mx_from_e4m3((p.y >> (8 * j)) & 255u) * by;
+  for (int h = 0; h < 2; ++h) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 two = mx_from_e4m3((uint16_t)(w[2 * h + (j >> 1)] >> (16 * (j & 1))));
+      v[2 * j] = two.x * by, v[2 * j + 1] = two.y * by;
+    }
+    store8(out + (size_t)row * k + c + 8 * h, v, k - c - 8 * h, whole);
   }
-  store8(out + row * k + c, v, k - c, whole);
 }
 
 ALOFA_API int alofa_mx_rows_values(void* out, const void* codes, const void* scales, int t, int k, int bf16_out, void* stream) {
-  if (t < 0 || k <= 0 || k > (1 << 30) || !aligned(codes, 8)) return ALOFA_ERR_ARGUMENT;
+  if (t < 0 || k <= 0 || k > (1 << 30) || !aligned(codes, 16)) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
-  const long long chunks = (long long)t * ((k + 7) / 8), blocks = (chunks + 255) / 256;
-  if (blocks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  const long long chunks = (long long)t * ((k + 15) / 16);
+  if (chunks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  const unsigned blocks = (unsigned)((chunks + 255) / 256);
   const bool whole = k % 8 == 0 && aligned(out, 16);
   if (bf16_out)
-    launch_dep(mx_rows_values_kernel<bf16>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, chunks, k, padded(k), whole);
+    launch_dep(mx_rows_values_kernel<bf16>, blocks, 256, 0, (cudaStream_t)stream, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, (unsigned)chunks, k, padded(k), whole);
   else
-    launch_dep(mx_rows_values_kernel<float>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, (float*)out, (const uint8_t*)codes, (const uint8_t*)scales, chunks, k, padded(k), whole);
+    launch_dep(mx_rows_values_kernel<float>, blocks, 256, 0, (cudaStream_t)stream, (float*)out, (const uint8_t*)codes, (const uint8_t*)scales, (unsigned)chunks, k, padded(k), whole);
   return launch_status();
 }
 
@@ -212,8 +233,8 @@ ALOFA_API int alofa_mx_norm(void* codes, void* scales, float* h, const float* ba
 }
 
 // ---------------------------------------------------------------------------
-// Weights: a block makes one tile of 128 rows and 128 numbers of each; a warp has two rows at a time, 256
-// bytes of bf16 from each.  `features` > 0: a gated weight whose row f is the gate's and features + f the up
+// Weights: a block makes one tile of 128 rows and 128 numbers of each; a lane has eight neighbouring numbers of
+// four rows, all their loads in flight together.  `features` > 0: a gated weight whose row f is the gate's and features + f the up
 // projection's.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int weight_source_row(int r, int n, int features) {
@@ -222,19 +243,21 @@ __device__ __forceinline__ int weight_source_row(int r, int n, int features) {
   return f < features ? half * features + f : -1;
 }
 
+constexpr int PACK_THREADS = 512;
+
 template <typename T>
-__global__ void __launch_bounds__(256) mx_pack_kernel(uint8_t* __restrict__ tiles, const T* __restrict__ w, int n, int k, int features, bool whole) {
+__global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 2 ? 3 : 2) mx_pack_kernel(uint8_t* __restrict__ tiles, const T* __restrict__ w, int n, int k, int features, bool whole) {
   uint8_t* tile = tiles + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * MX_TILE_BYTES;
-  const int c = (threadIdx.x & 15) * 8, kc = blockIdx.x * MX_GROUP + c;
-  float v[8][8];
+  const int c = (threadIdx.x & 15) * 8, kc = blockIdx.x * MX_GROUP + c, r0 = threadIdx.x >> 4;
+  float v[4][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int src = weight_source_row(blockIdx.y * MX_TILE_ROWS + i * 16 + (threadIdx.x >> 4), n, features);
+  for (int i = 0; i < 4; ++i) {
+    const int src = weight_source_row(blockIdx.y * MX_TILE_ROWS + i * 32 + r0, n, features);
     load8(v[i], w + (size_t)max(src, 0) * k + kc, src < 0 ? 0 : k - kc, whole);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 16 + (threadIdx.x >> 4);
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 32 + r0;
     const uint32_t s = mx_weight_scale(mx_largest4(v[i]));
     const float over = mx_over(s);
 #pragma unroll
@@ -262,29 +285,36 @@ ALOFA_API int alofa_mx_pack(void* tiles, const void* w, int n, int k, int gated,
   const dim3 grid((unsigned)(padded(k) / MX_GROUP), (unsigned)tall);
   const bool whole = k % 8 == 0 && aligned(w, 16);
   if (bf16_w)
-    launch_whole(mx_pack_kernel<bf16>, grid, 256, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const bf16*)w, n, k, gated ? n / 2 : 0, whole);
+    launch_whole(mx_pack_kernel<bf16>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const bf16*)w, n, k, gated ? n / 2 : 0, whole);
   else
-    launch_whole(mx_pack_kernel<float>, grid, 256, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const float*)w, n, k, gated ? n / 2 : 0, whole);
+    launch_whole(mx_pack_kernel<float>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const float*)w, n, k, gated ? n / 2 : 0, whole);
   const int rc = launch_status();
   return rc ? rc : alofa_mx_settle(stream);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) mx_weight_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ tiles, int n, int k, int features, bool whole) {
+__global__ void __launch_bounds__(PACK_THREADS) mx_weight_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ tiles, int n, int k, int features, bool whole) {
   const uint8_t* tile = tiles + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * MX_TILE_BYTES;
-  const int c = (threadIdx.x & 15) * 8, kc = blockIdx.x * MX_GROUP + c;
+  const int c = (threadIdx.x & 15) * 8, kc = blockIdx.x * MX_GROUP + c, r0 = threadIdx.x >> 4;
   pdl_wait();
   pdl_launch();
+  uint32_t p[4], s[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 16 + (threadIdx.x >> 4), src = weight_source_row(blockIdx.y * MX_TILE_ROWS + r, n, features);
-    if (src < 0 || kc >= k) continue;
-    const uint32_t p = *reinterpret_cast<const uint32_t*>(tile + r * (MX_GROUP / 2) + c / 2);
-    const float by = mx_power(tile[MX_TILE_CODES + mx_scale_at(r, c / MX_BLOCK)]);
+  for (int i = 0; i < 4; ++i) {
+    p[i] = *reinterpret_cast<const uint32_t*>(tile + (i * 32 + r0) * (MX_GROUP / 2) + c / 2);
+    s[i] = tile[MX_TILE_CODES + mx_scale_at(i * 32 + r0, c / MX_BLOCK)];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int src = weight_source_row(blockIdx.y * MX_TILE_ROWS + i * 32 + r0, n, features);
+    const float by = mx_power(s[i]);
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = mx_from_e2m1((p >> (4 * j)) & 15u) * by;
-    store8(out + (size_t)src * k + kc, v, k - kc, whole);
+    for (int j = 0; j < 4; ++j) {
+      const float2 two = mx_from_e2m1(p[i] >> (8 * j));
+      v[2 * j] = two.x * by, v[2 * j + 1] = two.y * by;
+    }
+    if (src >= 0 && kc < k) store8(out + (size_t)src * k + kc, v, k - kc, whole);
   }
 }
 
@@ -295,8 +325,8 @@ ALOFA_API int alofa_mx_weight_values(void* out, const void* tiles, int n, int k,
   const dim3 grid((unsigned)(padded(k) / MX_GROUP), (unsigned)tall);
   const bool whole = k % 8 == 0 && aligned(out, 16);
   if (bf16_out)
-    launch_dep(mx_weight_values_kernel<bf16>, grid, 256, 0, (cudaStream_t)stream, (bf16*)out, (const uint8_t*)tiles, n, k, gated ? n / 2 : 0, whole);
+    launch_dep(mx_weight_values_kernel<bf16>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (bf16*)out, (const uint8_t*)tiles, n, k, gated ? n / 2 : 0, whole);
   else
-    launch_dep(mx_weight_values_kernel<float>, grid, 256, 0, (cudaStream_t)stream, (float*)out, (const uint8_t*)tiles, n, k, gated ? n / 2 : 0, whole);
+    launch_dep(mx_weight_values_kernel<float>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (float*)out, (const uint8_t*)tiles, n, k, gated ? n / 2 : 0, whole);
   return launch_status();
 }

@@ -67,12 +67,28 @@ def _matrix(t, name: str, here: int) -> tuple:
 
 def _here() -> int:
     try:
+        return torch._C._cuda_getDevice()
+    except (RuntimeError, AttributeError):  # CUDA is not initialised yet, or there is none
+        pass
+    try:
         return torch.cuda.current_device()
     except (RuntimeError, AssertionError) as err:
         raise AlofaError("unsupported", "kernels run on CUDA tensors only", str(err)) from err
 
 
 _stream = ops.current_stream_handle
+
+
+class _Library:
+    """The library's functions, looked up once each."""
+
+    def __getattr__(self, name: str):
+        fn = getattr(ops.mx_library(), name)
+        setattr(self, name, fn)
+        return fn
+
+
+_lib = _Library()
 
 
 def padded(k: int) -> int:
@@ -129,7 +145,7 @@ class MxRows:
         if dtype is not _BF16 and dtype is not _F32:
             raise AlofaError("unsupported", "numbers come in bfloat16 or float32", f"dtype={dtype}")
         out = torch.empty((self.rows, self.width), dtype=dtype, device=here)
-        rc = ops.mx_library().alofa_mx_rows_values(out.data_ptr(), self.codes_at, self.scales_at, self.rows, self.width, dtype is _BF16, _stream(here))
+        rc = _lib.alofa_mx_rows_values(out.data_ptr(), self.codes_at, self.scales_at, self.rows, self.width, dtype is _BF16, _stream(here))
         ops.mx_launched(rc, 1, "mx rows' values", lambda: f"rows={self.rows} width={self.width}")
         return out
 
@@ -158,7 +174,7 @@ class MxWeight:
         self.at = self.tiles.data_ptr()
         #: how the copies of the product see the tiles (two tensor maps)
         self.maps = ctypes.create_string_buffer(256)
-        ops.mx_launched(ops.mx_library().alofa_mx_weight_maps(self.maps, self.at, self.tiles.shape[0] * self.tiles.shape[1]), 0, "mx weight", lambda: f"rows={n} depth={k}")
+        ops.mx_launched(_lib.alofa_mx_weight_maps(self.maps, self.at, self.tiles.shape[0] * self.tiles.shape[1]), 0, "mx weight", lambda: f"rows={n} depth={k}")
 
     @classmethod
     def from_codes(cls, codes, scales, k: int, gated: bool = False) -> "MxWeight":
@@ -190,7 +206,7 @@ class MxWeight:
         w.tiles[:, :, :size] = c.view(tall, TILE_ROWS, slices, GROUP // 2).permute(0, 2, 1, 3).reshape(tall, slices, size)
         w.tiles[:, :, size:] = s.view(tall, 4, 32, slices, 4).permute(0, 3, 2, 1, 4).reshape(tall, slices, TILE_BYTES - size)
         # the product reads tiles ahead of the kernel before it
-        ops.mx_launched(ops.mx_library().alofa_mx_settle(_stream(here)), 1, "mx weight", str)
+        ops.mx_launched(_lib.alofa_mx_settle(_stream(here)), 1, "mx weight", str)
         return w
 
     def first_rows(self, n: int) -> "MxWeight":
@@ -208,7 +224,7 @@ class MxWeight:
         if dtype is not _BF16 and dtype is not _F32:
             raise AlofaError("unsupported", "numbers come in bfloat16 or float32", f"dtype={dtype}")
         out = torch.empty((self.n, self.k), dtype=dtype, device=here)
-        rc = ops.mx_library().alofa_mx_weight_values(out.data_ptr(), self.at, self.n, self.k, self.gated, dtype is _BF16, _stream(here))
+        rc = _lib.alofa_mx_weight_values(out.data_ptr(), self.at, self.n, self.k, self.gated, dtype is _BF16, _stream(here))
         ops.mx_launched(rc, 1, "mx weight's values", lambda: f"rows={self.n} depth={self.k}")
         return out
 
@@ -219,7 +235,7 @@ def pack_weight(w: torch.Tensor, gated: bool = False) -> MxWeight:
     here = _here()
     at, n, k, bf16 = _matrix(w, "w", here)
     out = MxWeight(n, k, gated, here)
-    rc = ops.mx_library().alofa_mx_pack(out.at, at, n, k, out.gated, bf16, _stream(here))
+    rc = _lib.alofa_mx_pack(out.at, at, n, k, out.gated, bf16, _stream(here))
     ops.mx_launched(rc, 2, "pack_weight", lambda: f"rows={n} depth={k}")
     return out
 
@@ -231,7 +247,7 @@ def quantize_rows(x: torch.Tensor, buf=None) -> MxRows:
     if not k:
         raise AlofaError("invalid_argument", "rows have a width", "width=0")
     rows = MxRows._empty(t, k, here, buf)
-    rc = ops.mx_library().alofa_mx_rows(rows.codes_at, rows.scales_at, at, t, k, bf16, _stream(here))
+    rc = _lib.alofa_mx_rows(rows.codes_at, rows.scales_at, at, t, k, bf16, _stream(here))
     ops.mx_launched(rc, 1, "quantize_rows", lambda: f"rows={t} width={k}")
     return rows
 
@@ -248,7 +264,7 @@ def norm_rows(h: torch.Tensor, weight: torch.Tensor, eps: float, base=None, owed
         _refuse(h, "h", "float32 of two dimensions", here)
     splits = owed.shape[0] if isinstance(owed, torch.Tensor) and owed.dim() else 0
     rows = MxRows._empty(t, k, here, buf)
-    rc = ops.mx_library().alofa_mx_norm(
+    rc = _lib.alofa_mx_norm(
         rows.codes_at, rows.scales_at, at, at if base is None else _at(base, "base", _F32, (t, k), here), None if owed is None else _at(owed, "owed", _F32, (splits, t, k), here), splits,
         None if bias is None else _at(bias, "bias", _F32, (k,), here), _at(weight, "weight", _F32, (k,), here), None if shift is None else _at(shift, "shift", _F32, (k,), here), t, k, eps, _stream(here),
     )
@@ -277,28 +293,55 @@ def _sms(here: int) -> int:
     return _SMS[here]
 
 
-def plan(tokens: int, rows: int, depth: int) -> tuple:
-    """(tokens a tile, parts of the depth) of a product; 256 tokens: pairs of CTAs."""
-    key = (tokens, rows, depth)
+# What a product takes, fitted to the times of every way at the shapes of 0.5 to 7 billion parameters and 1 to 1,536 tokens: the way
+# it chooses is 2.4 % off the fastest on the average.  Microseconds for a slice of 128 numbers of a CTA of the kernel for a few
+# tokens, by its tokens: alone on its SM, and where two share one.
+_FEW_SLICE = {16: (0.27, 0.40), 32: (0.31, 0.42), 64: (0.30, 0.49), 128: (0.72, 1.29)}
+
+
+def _few_us(tokens: int, rows: int, slices: int, gated: bool, bn: int, parts: int, sms: int) -> float:
+    ctas = -(-rows // TILE_ROWS) * -(-tokens // bn) * parts
+    alone, shared = _FEW_SLICE[bn]
+    room = 2 * sms if parts == 1 else int(0.946 * 2 * sms)  # clusters do not fill every SM
+    whole, rest = divmod(ctas, room)
+    rounds = whole * shared + (shared if rest > sms else alone if rest else 0.0)
+    return 2.9 + 0.15 * parts + (0.3 * parts + 0.044 * bn if gated else 0.0) + rounds * -(-slices // parts) + 3.1 * (whole - (rest == 0))
+
+
+def _pair_us(tokens: int, rows: int, slices: int, sms: int) -> float:
+    tiles = -(-rows // 256) * -(-tokens // 256)
+    return 5.4 + -(-tiles // (sms // 2)) * (0.8 + 0.454 * slices)
+
+
+def plan(tokens: int, rows: int, depth: int, gated: bool = False) -> tuple:
+    """(tokens a tile, parts of the depth) of a product; 256 tokens: pairs of CTAs.
+
+    The kernel for a few tokens has one tile of up to 64 of them, and its depth
+    goes in as many parts as make it shortest (us, depth x rows): 1 token, 18,944
+    x 3,584 in 8 parts 10.4, in 4 12.8; 896 x 9,728 gated undivided 3.9, in 2
+    parts 4.5.  Beyond 64 tokens tiles of 64 or 128 of it are weighed against
+    pairs, which take long to begin and then do a slice of 256 x 256 in the time
+    the others take for a quarter of it: 256 tokens, 3,584 x 4,608 10.7 in tiles
+    of 64 and 16.6 on pairs; 192 tokens, 3,584 x 37,888 gated 51.8 and 33.2;
+    1,024 tokens, 18,944 x 3,584 91.5 and 59.3, 8,960 x 1,536 27.0 and 30.2."""
+    key = (tokens, rows, depth, gated)
     found = _plans.get(key)
     if found is None:
         slices, sms = padded(depth) // GROUP, _sms(_here())
-        if tokens > 128:
-            found = (256, 1)
-        else:
-            bn = next(b for b in TOKEN_TILES if tokens <= b)
-            ctas = -(-rows // TILE_ROWS) * -(-tokens // bn)
-            found = (bn, max(1, min(MOST_PARTS, slices, 2 * sms // max(1, ctas))))
+        tiles = [next(b for b in TOKEN_TILES if tokens <= b)] if tokens <= 64 else [64, 128]
+        ways = [(_few_us(tokens, rows, slices, gated, bn, parts, sms), bn, parts) for bn in tiles for parts in (1, 2, 3, 4, 6, 8) if parts <= slices]
+        if tokens > 64:
+            ways.append((_pair_us(tokens, rows, slices, sms), 256, 1))
         if len(_plans) >= 4096:
             _plans.clear()
-        _plans[key] = found
+        found = _plans[key] = min(ways)[1:]
     return found
 
 
 def _product(x: MxRows, w: MxWeight, out_at, scales_at, bias_at, add_at, features: int, gate, out_bf16, status, how, here: int, what: str) -> None:
-    bn, parts = how or plan(x.rows, w.rows, w.k)
+    bn, parts = how or plan(x.rows, w.rows, w.k, w.gated)
     status_at = None if status is None else _at(status, "status", _I32, status.shape, here)
-    rc = ops.mx_library().alofa_mx_gemm(
+    rc = _lib.alofa_mx_gemm(
         out_at, scales_at, x.codes_at, x.scales_at, w.at, w.maps, bias_at, add_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16, status_at, _stream(here)
     )
     ops.mx_launched(rc, 1, what, lambda: f"tokens={x.rows} rows={w.rows} depth={w.k} how={(bn, parts)}")
