@@ -7,6 +7,8 @@
 //
 // All of them are bound by memory: a lane takes eight or sixteen neighbouring numbers, the lanes that share a
 // block find its largest magnitude by one or two shuffles, and codes are converted by the hardware's instructions.
+#include <string.h>
+
 #include "mx.cuh"
 
 template <typename T>
@@ -140,24 +142,41 @@ ALOFA_API int alofa_mx_rows_values(void* out, const void* codes, const void* sca
 }
 
 // ---------------------------------------------------------------------------
-// The norm.  A block has a row; a thread keeps its CH chunks of eight numbers in registers, so the row is
-// read once; sums are taken in a fixed order.  Formula: src/alofa/kernels/cpu/scalar.mojo:93-129.
+// The norm.  A block has a row and a thread CH chunks of eight numbers of it, which stay in registers: the row is
+// read once, with all its loads in flight together, four planes of owed sums at a time.  Sums are taken in a
+// fixed order.  Formula: src/alofa/kernels/cpu/scalar.mojo:93-129.
 // ---------------------------------------------------------------------------
 template <int CH>
-__global__ void mx_norm_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, float* __restrict__ h, const float* __restrict__ base, const float* __restrict__ owed, int splits,
-                               const float* __restrict__ bias, const float* __restrict__ w, const float* __restrict__ shift, int t, int k, int kp, float eps, bool whole) {
+__global__ void __launch_bounds__(512) mx_norm_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, float* h, const float* base, const float* __restrict__ owed, int splits,
+                                                      const float* __restrict__ bias, const float* __restrict__ w, const float* __restrict__ shift, int t, int k, int kp, float eps, bool whole) {
   __shared__ float scratch[32];
   pdl_wait();
   const int row = blockIdx.x;
   const size_t at = (size_t)row * k, plane = (size_t)t * k;
-  float v[CH][8];
+  constexpr int PLANES = CH == 1 ? 4 : 1;
+  float v[CH][8], g[CH == 1 ? 1 : CH][8];
   float ss = 0.f, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int c = (threadIdx.x + i * blockDim.x) * 8, have = k - c;
-    load8(v[i], base + at + c, have, whole);
+    const int c = (threadIdx.x + i * blockDim.x) * 8;
+    load8(v[i], base + at + c, k - c, whole);
+    if (CH == 1) load8(g[i], w + c, k - c, whole);
   }
-  for (int z = 0; z < splits; ++z) {
+  int z = 0;
+  for (; z + PLANES <= splits; z += PLANES) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = (threadIdx.x + i * blockDim.x) * 8;
+      float p[PLANES][8];
+#pragma unroll
+      for (int q = 0; q < PLANES; ++q) load8(p[q], owed + (z + q) * plane + at + c, k - c, whole);
+#pragma unroll
+      for (int q = 0; q < PLANES; ++q)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] += p[q][j];
+    }
+  }
+  for (; z < splits; ++z) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = (threadIdx.x + i * blockDim.x) * 8;
@@ -203,13 +222,13 @@ __global__ void mx_norm_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict_
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int c = (threadIdx.x + i * blockDim.x) * 8, have = k - c;
-    float g[8], s[8];
-    load8(g, w + c, have, whole);
+    float s[8];
+    if (CH > 1) load8(g[i], w + c, have, whole);
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] = 0.f;
     if (shift) load8(s, shift + c, have, whole);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = c + j < k ? fmaf((v[i][j] - mean) * scale, g[j], s[j]) : 0.f;
+    for (int j = 0; j < 8; ++j) v[i][j] = c + j < k ? fmaf((v[i][j] - mean) * scale, g[i][j], s[j]) : 0.f;
     mx_put8(v[i], codes + (size_t)row * kp + c, scales + (size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK, c < kp);
   }
 }
@@ -219,23 +238,27 @@ ALOFA_API int alofa_mx_norm(void* codes, void* scales, float* h, const float* ba
   if (t < 0 || k <= 0 || splits < 0 || !aligned(codes, 8)) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
   const int kp = padded(k), chunks = kp / 8;
-  const int threads = chunks <= 128 ? 128 : chunks <= 2048 ? 256 : 512, per = (chunks + threads - 1) / threads;
-  if (per > 8) return ALOFA_ERR_ARGUMENT;
+  // a chunk a thread where the rows are few and a row's time is what counts, two where they are many: 2,048 rows of 3,584
+  // with one plane 21.4 and 18.9 us, one row of 896 with four planes 3.8 and 5.8
+  const int per = chunks <= (t >= 2 * 148 ? 256 : 512) ? 1 : chunks <= 1024 ? 2 : chunks <= 2048 ? 4 : 8, threads = ((chunks + per - 1) / per + 31) / 32 * 32;
+  if (threads > 512) return ALOFA_ERR_ARGUMENT;
   bool whole = k % 8 == 0 && aligned(h, 16) && aligned(base, 16) && aligned(owed, 16) && aligned(bias, 16) && aligned(w, 16) && aligned(shift, 16);
   if (!splits) owed = nullptr;
 #define GO(CH) launch_dep(mx_norm_kernel<CH>, t, threads, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, h, base, owed, splits, bias, w, shift, t, k, kp, eps, whole)
-  if (per <= 1) GO(1);
-  else if (per <= 2) GO(2);
-  else if (per <= 4) GO(4);
-  else GO(8);
+  switch (per) {
+    case 1: GO(1); break;
+    case 2: GO(2); break;
+    case 4: GO(4); break;
+    default: GO(8); break;
+  }
 #undef GO
   return launch_status();
 }
 
 // ---------------------------------------------------------------------------
-// Weights: a block makes one tile of 128 rows and 128 numbers of each; a lane has eight neighbouring numbers of
-// four rows, all their loads in flight together.  `features` > 0: a gated weight whose row f is the gate's and features + f the up
-// projection's.
+// Weights: a block makes tiles of 128 rows and 128 numbers of each, up to four along the depth; a lane has eight
+// neighbouring numbers of four rows of a tile, and asks for the next tile's before it works on this one's.
+// `features` > 0: a gated weight whose row f is the gate's and features + f the up projection's.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int weight_source_row(int r, int n, int features) {
   if (!features) return r < n ? r : -1;
@@ -243,27 +266,68 @@ __device__ __forceinline__ int weight_source_row(int r, int n, int features) {
   return f < features ? half * features + f : -1;
 }
 
-constexpr int PACK_THREADS = 512;
+constexpr int PACK_THREADS = 512, PACK_TILES = 4;  // tiles of a block, where there are enough for two blocks an SM (one each otherwise)
 
 template <typename T>
-__global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 2 ? 3 : 2) mx_pack_kernel(uint8_t* __restrict__ tiles, const T* __restrict__ w, int n, int k, int features, bool whole) {
-  uint8_t* tile = tiles + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * MX_TILE_BYTES;
-  const int c = (threadIdx.x & 15) * 8, kc = blockIdx.x * MX_GROUP + c, r0 = threadIdx.x >> 4;
-  float v[4][8];
+struct Raw8 {  // eight numbers as they are loaded
+  uint4 q[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* src, int have, bool whole) {
+    if (whole && have >= 8) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int src = weight_source_row(blockIdx.y * MX_TILE_ROWS + i * 32 + r0, n, features);
-    load8(v[i], w + (size_t)max(src, 0) * k + kc, src < 0 ? 0 : k - kc, whole);
+      for (int j = 0; j < (int)(sizeof(T) / 2); ++j) q[j] = reinterpret_cast<const uint4*>(src)[j];
+      return;
+    }
+    T v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < have ? src[j] : from_f<T>(0.f);
+    memcpy(q, v, sizeof(v));
   }
+  __device__ __forceinline__ void numbers(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    } else {
+      memcpy(v, q, sizeof(v));
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 2 ? 2 : 1) mx_pack_kernel(uint8_t* __restrict__ tiles, const T* __restrict__ w, int n, int k, int slices, int each, int features, bool whole) {
+  const int c = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4, first = blockIdx.x * each, last = min(slices, first + each);
+  const T* src[4];
+  bool there[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = i * 32 + r0;
-    const uint32_t s = mx_weight_scale(mx_largest4(v[i]));
-    const float over = mx_over(s);
+    const int row = weight_source_row(blockIdx.y * MX_TILE_ROWS + i * 32 + r0, n, features);
+    there[i] = row >= 0;
+    src[i] = w + (size_t)max(row, 0) * k + c;
+  }
+  Raw8<T> next[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] *= over;
-    *reinterpret_cast<uint32_t*>(tile + r * (MX_GROUP / 2) + c / 2) = s == 255u ? 0u : mx_e2m1(v[i]);
-    if ((threadIdx.x & 3) == 0) tile[MX_TILE_CODES + mx_scale_at(r, c / MX_BLOCK)] = (uint8_t)s;
+  for (int i = 0; i < 4; ++i) next[i].load(src[i] + first * MX_GROUP, there[i] ? k - c - first * MX_GROUP : 0, whole);
+  for (int s = first; s < last; ++s) {
+    uint8_t* tile = tiles + ((size_t)blockIdx.y * slices + s) * MX_TILE_BYTES;
+    Raw8<T> now[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) now[i] = next[i];
+    if (s + 1 < last) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) next[i].load(src[i] + (s + 1) * MX_GROUP, there[i] ? k - c - (s + 1) * MX_GROUP : 0, whole);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 32 + r0;
+      float v[8];
+      now[i].numbers(v);
+      const uint32_t e = mx_weight_scale(mx_largest4(v));
+      const float over = mx_over(e);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= over;
+      *reinterpret_cast<uint32_t*>(tile + r * (MX_GROUP / 2) + c / 2) = e == 255u ? 0u : mx_e2m1(v);
+      if ((threadIdx.x & 3) == 0) tile[MX_TILE_CODES + mx_scale_at(r, c / MX_BLOCK)] = (uint8_t)e;
+    }
   }
 }
 
@@ -282,12 +346,14 @@ ALOFA_API int alofa_mx_pack(void* tiles, const void* w, int n, int k, int gated,
   if (n <= 0 || k <= 0 || k > (1 << 30) || (gated && n % 2) || !aligned(tiles, 16)) return ALOFA_ERR_ARGUMENT;
   const long long rows = gated ? 2ll * ((n / 2 + 15) / 16 * 16) : n, tall = (rows + MX_TILE_ROWS - 1) / MX_TILE_ROWS;
   if (tall > 65535) return ALOFA_ERR_ARGUMENT;
-  const dim3 grid((unsigned)(padded(k) / MX_GROUP), (unsigned)tall);
+  const int slices = padded(k) / MX_GROUP;
+  const int each = slices * tall >= 2 * 148 * PACK_TILES ? PACK_TILES : 1;
+  const dim3 grid((unsigned)((slices + each - 1) / each), (unsigned)tall);
   const bool whole = k % 8 == 0 && aligned(w, 16);
   if (bf16_w)
-    launch_whole(mx_pack_kernel<bf16>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const bf16*)w, n, k, gated ? n / 2 : 0, whole);
+    launch_whole(mx_pack_kernel<bf16>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const bf16*)w, n, k, slices, each, gated ? n / 2 : 0, whole);
   else
-    launch_whole(mx_pack_kernel<float>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const float*)w, n, k, gated ? n / 2 : 0, whole);
+    launch_whole(mx_pack_kernel<float>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const float*)w, n, k, slices, each, gated ? n / 2 : 0, whole);
   const int rc = launch_status();
   return rc ? rc : alofa_mx_settle(stream);
 }
