@@ -145,6 +145,7 @@ struct FewTile {
 
 // Four neighbouring rows' sums of one token, as a gated weight has them (16 rows of the gate, the same 16 of the up
 // projection): the warp's 64 features as codes and two scales.  f0: the first of the tile's features.
+template <bool CLAMPED>
 __device__ __forceinline__ void few_gated_token(const MxArgs& args, float4 v, int t, int f0, int lane) {
   const int f = f0 + (lane >> 3) * 16 + (lane & 3) * 4;  // lanes with bit 2 clear have the gate's rows, those with it set the up projection's
   float g[4] = {v.x, v.y, v.z, v.w};
@@ -152,7 +153,7 @@ __device__ __forceinline__ void few_gated_token(const MxArgs& args, float4 v, in
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float u = __shfl_xor_sync(0xffffffffu, g[j], 4);
-    const float y = args.gate_alpha == 0.f ? mx_gate_times<false>(g[j], u, 0.f, 0.f) : mx_gate_times<true>(g[j], u, args.gate_alpha, args.gate_limit);
+    const float y = CLAMPED ? mx_gate_times<true>(g[j], u, args.gate_alpha, args.gate_limit) : mx_gate_times<false>(g[j], u, 0.f, 0.f);
     g[j] = f + j < args.F ? y : 0.f;
   }
   if ((lane & 4) == 0)
@@ -353,8 +354,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
 #pragma unroll
     for (int z = 1; z < FEW_PARTS; ++z)
       if (z < parts) v[0].x += v[z].x, v[0].y += v[z].y, v[0].z += v[z].z, v[0].w += v[z].w;
-    if (args.F) few_gated_token(args, v[0], t0 + t, f_tile * (MX_TILE_ROWS / 2), lane);
-    else few_stored_token(args, v[0], t0 + t, f0 + lane * 4);
+    if (!args.F) few_stored_token(args, v[0], t0 + t, f0 + lane * 4);
+    else if (args.gate_alpha == 0.f) few_gated_token<false>(args, v[0], t0 + t, f_tile * (MX_TILE_ROWS / 2), lane);
+    else few_gated_token<true>(args, v[0], t0 + t, f_tile * (MX_TILE_ROWS / 2), lane);
   }
   if (parts > 1) cluster_sync_all();  // nobody leaves while its sums are read
   else __syncthreads();
@@ -737,11 +739,33 @@ static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const 
   return launch_status();
 }
 
+// A product as its caller packs it: one argument, where twenty-two would take longer to hand over than the launch.
 // bn: 256: pairs of CTAs (`parts` 1, a grid of `ctas` of them); 16, 32, 64 or 128 tokens a CTA, the depth in `parts` parts.
 // features > 0: out are the codes and out_scales the scales of that many gated features, n the rows of the gated weight.
 // weight_maps: alofa_mx_weight_maps' of the tiles.
-ALOFA_API int alofa_mx_gemm(void* out, void* out_scales, const void* x_codes, const void* x_scales, const void* tiles, const void* weight_maps, const float* bias, const float* add, int t, int n, int k, int features,
-                            float gate_alpha, float gate_limit, int bn, int parts, int ctas, int out_bf16, int* status, void* stream) {
+struct MxCall {
+  void* out;
+  void* out_scales;
+  const void* x_codes;
+  const void* x_scales;
+  const void* tiles;
+  const void* weight_maps;
+  const float* bias;
+  const float* add;
+  int* status;
+  int t, n, k, features;
+  float gate_alpha, gate_limit;
+  int bn, parts, ctas, out_bf16;
+};
+static_assert(sizeof(MxCall) == 9 * 8 + 10 * 4, "as the caller packs it");
+
+ALOFA_API int alofa_mx_gemm(const MxCall* call, void* stream) {
+  void *out = call->out, *out_scales = call->out_scales;
+  const void *x_codes = call->x_codes, *x_scales = call->x_scales, *tiles = call->tiles, *weight_maps = call->weight_maps;
+  const float *bias = call->bias, *add = call->add;
+  const int t = call->t, n = call->n, k = call->k, features = call->features, bn = call->bn, parts = call->parts, ctas = call->ctas, out_bf16 = call->out_bf16;
+  const float gate_alpha = call->gate_alpha, gate_limit = call->gate_limit;
+  int* status = call->status;
   if (t < 0 || n <= 0 || k <= 0 || k > (1 << 30) || n > (1 << 30) || (uintptr_t)x_codes % 16 || (uintptr_t)x_scales % 4 || (uintptr_t)tiles % 32) return ALOFA_ERR_ARGUMENT;
   if (features < 0 || (features && (n != 2 * ((features + 15) / 16 * 16) || !out_scales || (uintptr_t)out % 16))) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;

@@ -1612,7 +1612,7 @@ def mx_library():
             "alofa_mx_settle": [_P],
             "alofa_mx_weight_values": [_P, _P, _I, _I, _I, _I, _P],
             "alofa_mx_weight_maps": [_P, _P, ctypes.c_longlong],
-            "alofa_mx_gemm": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _I, _I, _I, _I, _P, _P],
+            "alofa_mx_gemm": [_P, _P],
         }
         for name, args in sigs.items():
             fn = getattr(lib, name)

@@ -23,6 +23,7 @@ over what a launch goes by, and rows are one allocation."""
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -144,7 +145,7 @@ class MxRows:
         here = _on(self, "rows", _here())
         if dtype is not _BF16 and dtype is not _F32:
             raise AlofaError("unsupported", "numbers come in bfloat16 or float32", f"dtype={dtype}")
-        out = torch.empty((self.rows, self.width), dtype=dtype, device=here)
+        out = (self._codes if self._data is None else self._data).new_empty((self.rows, self.width), dtype=dtype)
         rc = _lib.alofa_mx_rows_values(out.data_ptr(), self.codes_at, self.scales_at, self.rows, self.width, dtype is _BF16, _stream(here))
         ops.mx_launched(rc, 1, "mx rows' values", lambda: f"rows={self.rows} width={self.width}")
         return out
@@ -162,7 +163,7 @@ class MxWeight:
     are a gate's, the second an up projection's.  Made by :func:`pack_weight`
     or :meth:`from_codes`."""
 
-    __slots__ = ("tiles", "n", "k", "gated", "rows", "device", "at", "maps")
+    __slots__ = ("tiles", "n", "k", "gated", "rows", "device", "at", "maps", "maps_at")
 
     def __init__(self, n: int, k: int, gated: bool, here: int):
         if n <= 0 or k <= 0 or (gated and n % 2):
@@ -174,6 +175,7 @@ class MxWeight:
         self.at = self.tiles.data_ptr()
         #: how the copies of the product see the tiles (two tensor maps)
         self.maps = ctypes.create_string_buffer(256)
+        self.maps_at = ctypes.addressof(self.maps)
         ops.mx_launched(_lib.alofa_mx_weight_maps(self.maps, self.at, self.tiles.shape[0] * self.tiles.shape[1]), 0, "mx weight", lambda: f"rows={n} depth={k}")
 
     @classmethod
@@ -215,7 +217,7 @@ class MxWeight:
             raise AlofaError("invalid_argument", "the first rows of a weight that is not gated", f"rows={n} of {self.n} gated={self.gated}")
         part = MxWeight.__new__(MxWeight)
         part.n, part.rows, part.k, part.gated, part.device = n, n, self.k, False, self.device
-        part.tiles, part.at, part.maps = self.tiles[: -(-n // TILE_ROWS)], self.at, self.maps
+        part.tiles, part.at, part.maps, part.maps_at = self.tiles[: -(-n // TILE_ROWS)], self.at, self.maps, self.maps_at
         return part
 
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
@@ -223,7 +225,7 @@ class MxWeight:
         here = _on(self, "weight", _here())
         if dtype is not _BF16 and dtype is not _F32:
             raise AlofaError("unsupported", "numbers come in bfloat16 or float32", f"dtype={dtype}")
-        out = torch.empty((self.n, self.k), dtype=dtype, device=here)
+        out = self.tiles.new_empty((self.n, self.k), dtype=dtype)
         rc = _lib.alofa_mx_weight_values(out.data_ptr(), self.at, self.n, self.k, self.gated, dtype is _BF16, _stream(here))
         ops.mx_launched(rc, 1, "mx weight's values", lambda: f"rows={self.n} depth={self.k}")
         return out
@@ -283,6 +285,7 @@ def _operands(x, w, what: str, gated: bool, here: int, buf) -> MxRows:
     return x
 
 
+_CALL = struct.Struct("9Q4i2f4i").pack  # a product's arguments (MxCall in kernels/mx_gemm.cu)
 _plans: dict = {}
 _SMS: dict = {}  # of a device
 
@@ -340,10 +343,9 @@ def plan(tokens: int, rows: int, depth: int, gated: bool = False) -> tuple:
 
 def _product(x: MxRows, w: MxWeight, out_at, scales_at, bias_at, add_at, features: int, gate, out_bf16, status, how, here: int, what: str) -> None:
     bn, parts = how or plan(x.rows, w.rows, w.k, w.gated)
-    status_at = None if status is None else _at(status, "status", _I32, status.shape, here)
-    rc = _lib.alofa_mx_gemm(
-        out_at, scales_at, x.codes_at, x.scales_at, w.at, w.maps, bias_at, add_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16, status_at, _stream(here)
-    )
+    status_at = 0 if status is None else _at(status, "status", _I32, status.shape, here)
+    call = _CALL(out_at, scales_at, x.codes_at, x.scales_at, w.at, w.maps_at, bias_at, add_at, status_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16)
+    rc = _lib.alofa_mx_gemm(call, _stream(here))
     ops.mx_launched(rc, 1, what, lambda: f"tokens={x.rows} rows={w.rows} depth={w.k} how={(bn, parts)}")
 
 
@@ -360,15 +362,15 @@ def linear(x, w: MxWeight, bias=None, add=None, out=None, dtype=None, buf=None, 
         dtype = dtype or (_BF16 if add is None else _F32)
         if dtype is not _BF16 and dtype is not _F32:
             raise AlofaError("unsupported", "a product is stored in bfloat16 or float32", f"dtype={dtype}")
-        out = torch.empty((t, n), dtype=dtype, device=here) if buf is None else buf((t, n), dtype)
+        out = w.tiles.new_empty((t, n), dtype=dtype) if buf is None else buf((t, n), dtype)
         out_at, out_bf16 = out.data_ptr(), dtype is _BF16
     else:
         out_at, rows, columns, out_bf16 = _matrix(out, "out", here)
         if rows != t or columns != n:
             _refuse(out, "out", f"({t}, {n})", here)
-    bias_at = None if bias is None else _at(bias, "bias", _F32, (n,), here)
-    add_at = None if add is None else _at(add, "add", _F32, (t, n), here)
-    _product(x, w, out_at, None, bias_at, add_at, 0, ops.SILU_GATE, out_bf16, status, how, here, "linear")
+    bias_at = 0 if bias is None else _at(bias, "bias", _F32, (n,), here)
+    add_at = 0 if add is None else _at(add, "add", _F32, (t, n), here)
+    _product(x, w, out_at, 0, bias_at, add_at, 0, ops.SILU_GATE, out_bf16, status, how, here, "linear")
     return out
 
 
@@ -380,5 +382,5 @@ def gated_linear(x, w: MxWeight, gate=ops.SILU_GATE, buf=None, status=None, how:
     x = _operands(x, w, "gated_linear", True, here, buf)
     features = w.n // 2
     rows = MxRows._empty(x.rows, features, here, buf)
-    _product(x, w, rows.codes_at, rows.scales_at, None, None, features, gate, False, status, how, here, "gated_linear")
+    _product(x, w, rows.codes_at, rows.scales_at, 0, 0, features, gate, False, status, how, here, "gated_linear")
     return rows
