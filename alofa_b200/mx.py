@@ -147,7 +147,7 @@ class MxRows:
             raise AlofaError("unsupported", "numbers come in bfloat16 or float32", f"dtype={dtype}")
         out = (self._codes if self._data is None else self._data).new_empty((self.rows, self.width), dtype=dtype)
         rc = _lib.alofa_mx_rows_values(out.data_ptr(), self.codes_at, self.scales_at, self.rows, self.width, dtype is _BF16, _stream(here))
-        ops.mx_launched(rc, 1, "mx rows' values", lambda: f"rows={self.rows} width={self.width}")
+        ops.mx_launched(rc, 1 if self.rows else 0, "mx rows' values", lambda: f"rows={self.rows} width={self.width}")
         return out
 
 
@@ -250,7 +250,7 @@ def quantize_rows(x: torch.Tensor, buf=None) -> MxRows:
         raise AlofaError("invalid_argument", "rows have a width", "width=0")
     rows = MxRows._empty(t, k, here, buf)
     rc = _lib.alofa_mx_rows(rows.codes_at, rows.scales_at, at, t, k, bf16, _stream(here))
-    ops.mx_launched(rc, 1, "quantize_rows", lambda: f"rows={t} width={k}")
+    ops.mx_launched(rc, 1 if t else 0, "quantize_rows", lambda: f"rows={t} width={k}")
     return rows
 
 
@@ -270,7 +270,7 @@ def norm_rows(h: torch.Tensor, weight: torch.Tensor, eps: float, base=None, owed
         rows.codes_at, rows.scales_at, at, at if base is None else _at(base, "base", _F32, (t, k), here), None if owed is None else _at(owed, "owed", _F32, (splits, t, k), here), splits,
         None if bias is None else _at(bias, "bias", _F32, (k,), here), _at(weight, "weight", _F32, (k,), here), None if shift is None else _at(shift, "shift", _F32, (k,), here), t, k, eps, _stream(here),
     )
-    ops.mx_launched(rc, 1, "norm_rows", lambda: f"rows={t} width={k} most={MOST_WIDTH}")
+    ops.mx_launched(rc, 1 if t else 0, "norm_rows", lambda: f"rows={t} width={k} most={MOST_WIDTH}")
     return rows
 
 
@@ -342,6 +342,8 @@ def plan(tokens: int, rows: int, depth: int, gated: bool = False) -> tuple:
 
 
 def _product(x: MxRows, w: MxWeight, out_at, scales_at, bias_at, add_at, features: int, gate, out_bf16, status, how, here: int, what: str) -> None:
+    if not x.rows:
+        return
     bn, parts = how or plan(x.rows, w.rows, w.k, w.gated)
     status_at = 0 if status is None else _at(status, "status", _I32, status.shape, here)
     call = _CALL(out_at, scales_at, x.codes_at, x.scales_at, w.at, w.maps_at, bias_at, add_at, status_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16)

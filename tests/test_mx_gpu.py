@@ -291,3 +291,199 @@ def test_gated_linear(t, f, k, how, gate):
     sizes, room = np.abs(full).reshape(t, -1, 32), pad.reshape(t, -1, 32)
     scales = host(rows.scales)
     assert (scales >= plain.scale_bytes(np.maximum(sizes - room, 0).max(-1), False)).all() and (scales <= plain.scale_bytes((sizes + room).max(-1), False)).all()
+
+
+# ---- as a program uses them ------------------------------------------------------------------------------------------
+
+
+def chain(h, weight, w1, w2, owed):
+    """A norm, a gated feed-forward and its sum into the stream: the operators one after another."""
+    x = mx.norm_rows(h, weight, 1e-6, owed=owed)
+    return mx.linear(mx.gated_linear(x, w1), w2, add=h)
+
+
+def chain_operands(t, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    h, weight, owed = rnd(t, 384), 1 + 0.1 * rnd(384), rnd(1, t, 384)
+    wg, wd = 0.05 * rnd(2 * 640, 384), 0.05 * rnd(384, 640)
+    return h, weight, wg, wd, owed
+
+
+@pytest.mark.parametrize("t", [1, 20, 150, 600])
+def test_a_run_of_them_together(t):
+    h, weight, wg, wd, owed = chain_operands(t, 1)
+    h0 = h.clone()
+    got = chain(h, weight, mx.pack_weight(wg, True), mx.pack_weight(wd), owed)
+    f64 = lambda v: v.cpu().double().numpy()  # noqa: E731
+    hh = f64(h0) + f64(owed[0])
+    x = plain.values(plain.norm(hh, f64(weight), 1e-6))
+    w = plain.values(wg.cpu(), True)
+    g, u = x @ w[:640].T, x @ w[640:].T
+    want = hh + plain.values(plain.silu(g) * u) @ plain.values(wd.cpu(), True).T
+    # a number next to a border of two codes may take the other one, a step of 2^-3 of it at most: a few of them move a sum of
+    # 640 products by a few times 2^-3 / sqrt(640) of its size, 0.5 % each
+    size = np.sqrt((want - hh).std() ** 2)
+    assert np.abs(f64(got) - want).max() <= 0.05 * size and np.sqrt(((f64(got) - want) ** 2).mean()) <= 0.003 * size
+    assert (np.abs(f64(h) - hh) <= 2.0**-23 * (np.abs(f64(h0)) + np.abs(f64(owed[0])))).all()
+
+
+def test_captured_and_replayed_on_new_inputs():
+    t = 40
+    h, weight, wg, wd, owed = chain_operands(t, 2)
+    w1, w2 = mx.pack_weight(wg, True), mx.pack_weight(wd)
+    want = [chain(h.clone().mul_(s), weight, w1, w2, owed).clone() for s in (1.0, 3.0, 0.01)]
+    src, work = h.clone(), h.clone()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(stream):
+        work.copy_(src)
+        chain(work, weight, w1, w2, owed)
+        for _ in range(2):  # two graphs of the same calls: neither shares a workspace with the other
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                work.copy_(src)
+                out = chain(work, weight, w1, w2, owed)
+            graphs.append((graph, out))
+    for scale, ref in zip((1.0, 3.0, 0.01), want):
+        for graph, out in graphs:
+            src.copy_(h * scale)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, ref)
+
+
+def test_a_weight_packed_and_used_in_one_graph():
+    """The product reads its weight ahead of the kernel before it; what packs one leaves it settled."""
+    w = torch.randn(2, 1152, 896, device="cuda") * 0.05
+    x = mx.quantize_rows(torch.randn(8, 896, device="cuda"))
+    want = [mx.linear(x, mx.pack_weight(w[i])).clone() for i in range(2)]
+    src = w[0].clone()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        mx.linear(x, mx.pack_weight(src))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            packed = mx.pack_weight(src)
+            out = mx.linear(x, packed)
+    for i in (1, 0, 1, 1, 0) * 10:
+        src.copy_(w[i])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
+
+
+def test_two_streams_at_once():
+    """The same weight and rows, other outputs, beside each other."""
+    operands = [chain_operands(t, 5 + t) for t in (3, 300)]
+    packed = [(mx.pack_weight(o[2], True), mx.pack_weight(o[3])) for o in operands]
+    want = [chain(o[0].clone(), o[1], *p, o[4]) for o, p in zip(operands, packed)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in operands]
+    got = [[] for _ in operands]
+    hs = [[o[0].clone() for _ in range(20)] for o in operands]
+    torch.cuda.synchronize()
+    for k in range(20):
+        for i, (o, p, s) in enumerate(zip(operands, packed, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(chain(hs[i][k], o[1], *p, o[4]))
+    torch.cuda.synchronize()
+    for g, ref in zip(got, want):
+        assert all(torch.equal(x, ref) for x in g)
+
+
+def test_no_tokens():
+    w, wg = mx.pack_weight(torch.randn(64, 96, device="cuda")), mx.pack_weight(torch.randn(64, 96, device="cuda"), True)
+    x = mx.quantize_rows(torch.empty(0, 96, device="cuda"))
+    assert x.dequantize().shape == (0, 96) and mx.linear(x, w).shape == (0, 64) and mx.gated_linear(x, wg).shape == (0, 32)
+    assert mx.norm_rows(torch.empty(0, 96, device="cuda"), torch.ones(96, device="cuda"), 1e-6).shape == (0, 96)
+
+
+def test_refusals():
+    def refused(code, call, *args, **kw):
+        with pytest.raises(AlofaError) as err:
+            call(*args, **kw)
+        assert err.value.code == code, err.value
+
+    x, w = torch.randn(4, 96, device="cuda"), mx.pack_weight(torch.randn(64, 96, device="cuda"))
+    wg, rows, ones = mx.pack_weight(torch.randn(64, 96, device="cuda"), True), mx.quantize_rows(x), torch.ones(96, device="cuda")
+    refused("invalid_argument", mx.quantize_rows, x.half())
+    refused("invalid_argument", mx.quantize_rows, x.t())
+    refused("invalid_argument", mx.quantize_rows, [1.0])
+    refused("invalid_argument", mx.quantize_rows, x[0])
+    refused("invalid_argument", mx.quantize_rows, torch.empty(3, 0, device="cuda"))
+    refused("unsupported", mx.quantize_rows, x.cpu())
+    refused("invalid_argument", mx.pack_weight, torch.empty(0, 96, device="cuda"))
+    refused("invalid_argument", mx.pack_weight, torch.randn(3, 96, device="cuda"), True)  # an odd number of rows
+    refused("invalid_argument", mx.linear, rows, wg)
+    refused("invalid_argument", mx.gated_linear, rows, w)
+    refused("invalid_argument", mx.linear, rows, torch.randn(64, 96, device="cuda"))
+    refused("invalid_argument", mx.linear, mx.quantize_rows(torch.randn(4, 128, device="cuda")), w)  # another depth
+    refused("invalid_argument", mx.linear, rows, w, bias=torch.zeros(63, device="cuda"))
+    refused("invalid_argument", mx.linear, rows, w, bias=torch.zeros(64, device="cuda").bfloat16())
+    refused("invalid_argument", mx.linear, rows, w, add=torch.zeros(4, 65, device="cuda"))
+    refused("invalid_argument", mx.linear, rows, w, out=torch.zeros(5, 64, device="cuda"))
+    refused("unsupported", mx.linear, rows, w, dtype=torch.float16)
+    refused("unsupported", mx.linear, rows, w, how=(48, 1))
+    refused("unsupported", mx.linear, rows, w, how=(16, 2))  # a part without a slice
+    refused("unsupported", mx.linear, rows, w, how=(256, 2))
+    refused("unsupported", rows.dequantize, torch.float16)
+    refused("unsupported", w.dequantize, torch.float16)
+    refused("invalid_argument", mx.norm_rows, x.bfloat16(), ones, 1e-6)
+    refused("invalid_argument", mx.norm_rows, x, ones[:95], 1e-6)
+    refused("invalid_argument", mx.norm_rows, x, ones, 1e-6, owed=torch.zeros(4, 96, device="cuda"))
+    refused("invalid_argument", mx.norm_rows, x, ones, 1e-6, base=x[:3])
+    refused("invalid_argument", mx.norm_rows, x, ones, 1e-6, shift=ones.double())
+    refused("unsupported", mx.norm_rows, torch.zeros(1, mx.MOST_WIDTH + 128, device="cuda"), torch.ones(mx.MOST_WIDTH + 128, device="cuda"), 1e-6)
+    refused("invalid_argument", mx.MxRows, rows.codes[:, :64].contiguous(), rows.scales, 96)
+    refused("invalid_argument", mx.MxRows, rows.codes, rows.scales[:3], 96)
+    refused("unsupported", mx.MxRows, torch.zeros(4 * 128 + 1, dtype=torch.uint8, device="cuda")[1:].view(4, 128), rows.scales, 96)  # off its alignment
+    refused("invalid_argument", mx.MxWeight.from_codes, rows.codes, rows.scales, 300)
+    refused("invalid_argument", w.first_rows, 65)
+    refused("invalid_argument", wg.first_rows, 3)
+
+
+def test_rows_given_by_their_codes():
+    x = numbers(9, 300, 60)
+    made = mx.quantize_rows(x.cuda())
+    again = mx.MxRows(made.codes.clone(), made.scales.clone(), 300)
+    w = mx.pack_weight(numbers(130, 300, 61).cuda())
+    assert torch.equal(mx.linear(made, w), mx.linear(again, w)) and torch.equal(made.dequantize(), again.dequantize())
+    assert torch.equal(mx.linear(x.cuda(), w), mx.linear(made, w))  # a tensor of numbers is made rows first
+
+
+def test_first_rows_of_a_weight():
+    xr, wp, xv, wv = product_operands(5, 300, 256, 62)
+    part = wp.first_rows(140)
+    assert torch.equal(part.dequantize(), wp.dequantize()[:140].contiguous()) and torch.equal(mx.linear(xr, part), mx.linear(xr, wp)[:, :140].contiguous())
+
+
+def test_the_widest_norm_and_a_deep_product():
+    k = mx.MOST_WIDTH
+    h, weight = numbers(2, k, 63), 1 + 0.1 * torch.randn(k)
+    rows = mx.norm_rows(h.cuda(), weight.cuda(), 1e-6)
+    assert plain.near(host(rows.codes), host(rows.scales), plain.norm(h.double().numpy(), weight.double().numpy(), 1e-6), ROWS_SLACK)
+    xr, wp, xv, wv = product_operands(3, 128, 40000, 64)
+    assert (np.abs(host(mx.linear(xr, wp, dtype=F32)) - xv @ wv.T) <= sum_bound(xv, wv)).all()
+
+
+def test_status_is_left_alone():
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for t in (4, 300):
+        xr, wp, _, _ = product_operands(t, 300, 256, 65)
+        mx.linear(xr, wp, status=status)
+    assert int(status) == 0
+
+
+def test_launches_are_counted():
+    from alofa_b200.csrc import ops
+
+    x, w = torch.randn(4, 96, device="cuda"), torch.randn(64, 96, device="cuda")
+    for call, launches in ((lambda: mx.pack_weight(w), 2), (lambda: mx.quantize_rows(x), 1), (lambda: mx.quantize_rows(x).dequantize(), 2), (lambda: mx.norm_rows(x, torch.ones(96, device="cuda"), 1e-6), 1)):
+        before = ops.launch_count()
+        call()
+        assert ops.launch_count() - before == launches
