@@ -7,6 +7,7 @@ Public entry points:
 * :class:`alofa_b200.engine.Engine` - load a model folder and generate tokens.
 * ``python -m alofa_b200.cli.generate`` - the command line of the same.
 * ``bin/trace_run`` - feed given token ids step by step and dump logits.
+* :mod:`alofa_b200.mx` - weights in 4 bits, rows in 8 bits, and their products.
 """
 
 __version__ = "0.1.0"

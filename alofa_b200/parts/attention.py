@@ -265,7 +265,8 @@ class GQAttention(PagedAttend, Part):
 
     def _project(self, ctx, lin, x, q, cache, group, table, rot, custom, vectorised, nkv_in, writes):
         qkv = ctx.buf((q.shape[0], (self.nh + 2 * nkv_in) * self.hd), self.rt.dtype)
-        owed = lin(qkv, x, defer=vectorised, buf=ctx.buf)
+        told = {"status": ctx.status} if getattr(lin, "takes_status", False) else {}
+        owed = lin(qkv, x, defer=vectorised, buf=ctx.buf, **told)
         self._rotate_and_store(ctx, q, qkv, owed, cache, group, table, rot, custom, vectorised, nkv_in, writes)
 
     def _rotate_and_store(self, ctx, q, qkv, owed, cache, group, table, rot, custom, vectorised, nkv_in, writes):

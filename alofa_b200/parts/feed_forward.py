@@ -49,7 +49,7 @@ class GatedMLP(Part):
 
     def forward(self, ctx, x, h):
         if self.rt.weight_format is not None:
-            add_into_stream(ctx, self.down, h, self.gate_up.gated_rows(x, ctx.buf))
+            add_into_stream(ctx, self.down, h, self.gate_up.gated_rows(x, ctx.buf, ctx.status))
             return
         act = ctx.buf((x.shape[0], self.inter), self.rt.dtype)
         self.gate_up(act, x, buf=ctx.buf)

@@ -172,6 +172,7 @@ def add_into_stream(ctx, linear: Linear, h, x) -> None:
         return
     if ctx.pending is not None and ctx.pending.h is h and (ctx.pending.acc is not None or ctx.pending.base is not h):
         ctx.flush_pending()  # the product adds in place or leaves planes on top of h itself
-    owed = linear(h, x, defer=True, buf=ctx.buf)
+    told = {"status": ctx.status} if getattr(linear, "takes_status", False) else {}
+    owed = linear(h, x, defer=True, buf=ctx.buf, **told)
     if owed is not None:
         ctx.set_pending(h, owed)

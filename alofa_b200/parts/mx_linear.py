@@ -30,6 +30,8 @@ class MxLinear:
         if bias is not None and epi == GATED:
             raise AlofaError("unsupported", "a gated product with weights in 4 bits takes no bias")
 
+    takes_status = True  # a call may name the step's status word, which a kernel raises that gave up on a wait
+
     def can_accumulate(self, tokens: int) -> bool:
         return False  # its sums are added by the norm that reads the stream next
 
@@ -38,16 +40,16 @@ class MxLinear:
             return x
         return mx.quantize_rows(x if isinstance(x, torch.Tensor) else x.rows(), buf)
 
-    def __call__(self, out, x, defer: bool = False, buf=None):
+    def __call__(self, out, x, defer: bool = False, buf=None, status=None):
         x = self._rows(x, buf)
         if defer and self.epi == RESIDUAL:
-            y = mx.linear(x, self.weight, dtype=torch.float32, buf=buf)
+            y = mx.linear(x, self.weight, dtype=torch.float32, buf=buf, status=status)
             return Partial(y.view(1, *y.shape), 1, self.bias)  # the norm that reads the stream next adds it
-        mx.linear(x, self.weight, bias=self.bias, add=out if self.epi == RESIDUAL else None, out=out, buf=buf)
+        mx.linear(x, self.weight, bias=self.bias, add=out if self.epi == RESIDUAL else None, out=out, buf=buf, status=status)
         return None
 
-    def gated_rows(self, x, buf=None) -> mx.MxRows:
-        return mx.gated_linear(self._rows(x, buf), self.weight, self.gate, buf)
+    def gated_rows(self, x, buf=None, status=None) -> mx.MxRows:
+        return mx.gated_linear(self._rows(x, buf), self.weight, self.gate, buf, status)
 
 
 def make_linear(rt, weight, bias, epi: int = STORE, gate=ops.SILU_GATE):
