@@ -1,6 +1,7 @@
 // What makes microscaled numbers (mx.cuh), and what turns them back:
 //   alofa_mx_rows        rows [T, K] in bf16 or fp32 -> E4M3 codes [T, Kp], scales [T, Kp / 32]
 //   alofa_mx_norm        h = base + sum_z owed[z] (+ bias); the RMSNorm (or layer norm) of h's rows as such rows
+//   alofa_mx_merge       the key splits of decode attention, joined, as such rows
 //   alofa_mx_pack        a weight [N, K] in bf16 or fp32 -> tiles of E2M1 codes and scales
 //   alofa_mx_rows_values, alofa_mx_weight_values   the numbers that rows, or a weight, stand for
 // Kp is K rounded up to whole groups of 128; the codes behind K are zeros.
@@ -252,6 +253,72 @@ ALOFA_API int alofa_mx_norm(void* codes, void* scales, float* h, const float* ba
     default: GO(8); break;
   }
 #undef GO
+  return launch_status();
+}
+
+// ---------------------------------------------------------------------------
+// Attention's output as rows: decode tokens whose keys were split over CTAs have an output, a maximum and a sum for
+// each split (scores in log2 units), and here they become one, o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, as
+// attention_combine_kernel has it (src/alofa/kernels/cpu/scalar.mojo:392-470), and go to 8 bits without a stop in
+// bfloat16.  A lane has eight channels; the loads of eight splits are in flight together.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(128) mx_merge_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const float* __restrict__ po, const float* __restrict__ pml, const int* __restrict__ positions,
+                                                       unsigned chunks, int t, int heads, int hd, int kp, int window, int split_keys) {
+  pdl_wait();
+  pdl_launch();
+  const unsigned i = blockIdx.x * blockDim.x + threadIdx.x, per_row = (unsigned)kp >> 3;
+  const bool live = i < chunks;
+  const int row = live ? (int)(i / per_row) : 0, c = live ? (int)(i % per_row) * 8 : 0;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if (live && c < heads * hd) {
+    const int head = c / hd, d = c - head * hd, p = positions[row];
+    const size_t rows = (size_t)t * heads, at = (size_t)row * heads + head;
+    const int first = (window > 0 ? max(0, p - window + 1) : 0) / split_keys, last = p / split_keys;  // splits that hold keys of this token
+    float m = -INFINITY, l = 0.f;
+    for (int s0 = first; s0 <= last; s0 += 8) {
+      float2 ml[8];
+      float4 lo[8], hi[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const size_t s = (size_t)min(s0 + k, last) * rows + at;
+        ml[k] = *reinterpret_cast<const float2*>(pml + s * 2);
+        const float4* o = reinterpret_cast<const float4*>(po + s * hd + d);
+        lo[k] = o[0], hi[k] = o[1];
+        if (s0 + k > last) ml[k].x = -INFINITY;
+      }
+      float next = m;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) next = fmaxf(next, ml[k].x);
+      if (next == -INFINITY) continue;  // splits that see nothing so far
+      const float keep = exp2f(m - next);
+      m = next, l *= keep;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= keep;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (ml[k].x == -INFINITY) continue;
+        const float w = exp2f(ml[k].x - m);
+        l = fmaf(ml[k].y, w, l);
+        v[0] = fmaf(lo[k].x, w, v[0]), v[1] = fmaf(lo[k].y, w, v[1]), v[2] = fmaf(lo[k].z, w, v[2]), v[3] = fmaf(lo[k].w, w, v[3]);
+        v[4] = fmaf(hi[k].x, w, v[4]), v[5] = fmaf(hi[k].y, w, v[5]), v[6] = fmaf(hi[k].z, w, v[6]), v[7] = fmaf(hi[k].w, w, v[7]);
+      }
+    }
+    const float over = 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= over;
+  }
+  mx_put8(v, codes + (size_t)row * kp + c, scales + (size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK, live);
+}
+
+ALOFA_API int alofa_mx_merge(void* codes, void* scales, const float* po, const float* pml, const int* positions, int t, int heads, int hd, int window, int split_keys, void* stream) {
+  if (t < 0 || heads <= 0 || hd <= 0 || hd % 8 || heads > (1 << 30) / hd || window < 0 || split_keys <= 0 || !aligned(codes, 16) || !aligned(po, 16) || !aligned(pml, 8)) return ALOFA_ERR_ARGUMENT;
+  if (t == 0) return ALOFA_OK;
+  const int kp = padded(heads * hd);
+  const long long chunks = (long long)t * (kp / 8);
+  if (chunks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  launch_dep(mx_merge_kernel, (unsigned)((chunks + 127) / 128), 128, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, po, pml, positions, (unsigned)chunks, t, heads, hd, kp, window, split_keys);
   return launch_status();
 }
 

@@ -274,6 +274,25 @@ def norm_rows(h: torch.Tensor, weight: torch.Tensor, eps: float, base=None, owed
     return rows
 
 
+def merge_rows(partial_o, partial_ml, positions, heads: int, window: int, split_keys: int, buf=None) -> MxRows:
+    """The attention output of decode tokens whose keys were split
+    (``partial_o [splits, T * heads, head_dim]``, ``partial_ml [splits, T *
+    heads, 2]``: each split's maximum, in log2 units, and sum; float32), joined,
+    as rows ``[T, heads * head_dim]`` in 8 bits.  ``positions [T]`` (int32): a
+    token's splits of ``split_keys`` keys are those that hold keys up to its
+    position, and (``window`` > 0) of its last ``window`` keys."""
+    here = _here()
+    if not isinstance(partial_o, torch.Tensor) or partial_o.dim() != 3 or heads <= 0 or partial_o.shape[1] % heads or not partial_o.shape[2] or partial_o.shape[2] % 8 or window < 0 or split_keys <= 0:
+        raise AlofaError("invalid_argument", "splits of heads of a multiple of 8 channels", f"partial_o={tuple(getattr(partial_o, 'shape', ()))} heads={heads} window={window} split_keys={split_keys}")
+    splits, n, hd = partial_o.shape
+    t = n // heads
+    o_at, ml_at, p_at = _at(partial_o, "partial_o", _F32, (splits, n, hd), here), _at(partial_ml, "partial_ml", _F32, (splits, n, 2), here), _at(positions, "positions", _I32, (t,), here)
+    rows = MxRows._empty(t, heads * hd, here, buf)
+    rc = _lib.alofa_mx_merge(rows.codes_at, rows.scales_at, o_at, ml_at, p_at, t, heads, hd, window, split_keys, _stream(here))
+    ops.mx_launched(rc, 1 if t else 0, "merge_rows", lambda: f"tokens={t} heads={heads} head_dim={hd} splits={splits}")
+    return rows
+
+
 def _operands(x, w, what: str, gated: bool, here: int, buf) -> MxRows:
     if not isinstance(w, MxWeight) or w.gated != gated:
         raise AlofaError("invalid_argument", f"{what} takes a weight that was packed for it", f"weight={type(w).__name__} gated={getattr(w, 'gated', None)}")

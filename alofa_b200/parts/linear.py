@@ -18,6 +18,7 @@ from typing import Optional
 
 import torch
 
+from .. import mx
 from ..csrc import ops
 from ..errors import AlofaError
 
@@ -60,6 +61,10 @@ class MergedSplits:
         out = self.buf(self.shape, torch.bfloat16)
         ops.attention_combine(out, self.partial_o, self.partial_ml, self.positions, self.heads, self.head_dim, self.window, self.split_keys, **self.library)
         return out
+
+    def mx_rows(self) -> mx.MxRows:
+        """The same in 8 bits, not rounded to bfloat16 on the way."""
+        return mx.merge_rows(self.partial_o, self.partial_ml, self.positions, self.heads, int(self.window or 0), self.split_keys, self.buf)
 
 
 class NormedRows:

@@ -38,7 +38,9 @@ class MxLinear:
     def _rows(self, x, buf):
         if isinstance(x, mx.MxRows):
             return x
-        return mx.quantize_rows(x if isinstance(x, torch.Tensor) else x.rows(), buf)
+        if not isinstance(x, torch.Tensor):  # decode attention whose splits are not joined yet
+            return x.mx_rows()
+        return mx.quantize_rows(x, buf)
 
     def __call__(self, out, x, defer: bool = False, buf=None, status=None):
         x = self._rows(x, buf)

@@ -153,6 +153,42 @@ def test_norm_rows(t, k, planes, bias, layer):
     assert torch.equal(h2, h) and torch.equal(again.codes, rows.codes) and torch.equal(again.scales, rows.scales) and torch.equal(base_dev.cpu(), base)
 
 
+# ---- attention's splits ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t,heads,hd,splits,split_keys,window", [(1, 14, 64, 3, 256, 0), (5, 3, 48, 1, 64, 0), (8, 28, 128, 16, 128, 0), (3, 5, 16, 9, 64, 0), (4, 2, 40, 12, 64, 200)])
+def test_merged_splits(t, heads, hd, splits, split_keys, window):
+    g = torch.Generator().manual_seed(9)
+    o, m = torch.randn(splits, t * heads, hd, generator=g), 20 * torch.randn(splits, t * heads, generator=g)
+    l = 1 + 5 * torch.rand(splits, t * heads, generator=g)
+    m[0, 0] = m[-1, -1] = -float("inf")  # a split that saw nothing (its sums are not read)
+    o[0, 0], o[-1, -1] = float("nan"), float("nan")
+    positions = torch.randint(0, splits * split_keys, (t,), generator=g)
+    positions[0] = splits * split_keys - 1
+    rows = mx.merge_rows(o.cuda(), torch.stack([m, l], -1).cuda(), positions.int().cuda(), heads, window, split_keys)
+    want = np.zeros((t, heads * hd))
+    for i in range(t):
+        p = int(positions[i])
+        first, last = (max(0, p - window + 1) if window else 0) // split_keys, p // split_keys
+        for h in range(heads):
+            r = i * heads + h
+            seen = [s for s in range(first, last + 1) if m[s, r] > -float("inf")]
+            top = max((float(m[s, r]) for s in seen), default=0.0)
+            w = [2.0 ** (float(m[s, r]) - top) for s in seen]
+            low = sum(a * float(l[s, r]) for a, s in zip(w, seen))
+            want[i, h * hd : (h + 1) * hd] = sum(a * o[s, r].double().numpy() for a, s in zip(w, seen)) / low if seen else np.nan
+    got = host(rows.dequantize(F32)).astype(np.float64)
+    bad = np.isnan(want)
+    if bad.any():  # a head that saw nothing: not a number, and its blocks
+        assert np.isnan(got[bad]).all()
+    keep = ~np.isnan(got)
+    assert not bad.any() or keep.any()
+    # sums over splits may cancel: what is off is off by a part of the sizes that went in, up to about 4 here
+    unit = np.exp2(host(rows.scales).astype(np.float64) - 127).repeat(32, -1)[:, : heads * hd]
+    step = unit * np.exp2(np.maximum(np.frexp(np.maximum(np.abs(got), np.abs(want)) / unit)[1] - 1, -6) - 3.0)
+    assert (np.abs(got - want) <= step / 2 + ROWS_SLACK * 4)[keep].all()
+
+
 # ---- the product -----------------------------------------------------------------------------------------------------
 
 
@@ -444,6 +480,13 @@ def test_refusals():
     refused("unsupported", mx.MxRows, torch.zeros(4 * 128 + 1, dtype=torch.uint8, device="cuda")[1:].view(4, 128), rows.scales, 96)  # off its alignment
     refused("invalid_argument", mx.MxWeight.from_codes, rows.codes, rows.scales, 300)
     refused("invalid_argument", w.first_rows, 65)
+    po, ml, at = torch.zeros(2, 6, 16, device="cuda"), torch.zeros(2, 6, 2, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    mx.merge_rows(po, ml, at, 3, 0, 64)
+    refused("invalid_argument", mx.merge_rows, po, ml, at, 4, 0, 64)
+    refused("invalid_argument", mx.merge_rows, po[..., :12].contiguous(), ml, at, 3, 0, 64)
+    refused("invalid_argument", mx.merge_rows, po, ml[:1], at, 3, 0, 64)
+    refused("invalid_argument", mx.merge_rows, po, ml, at.long(), 3, 0, 64)
+    refused("invalid_argument", mx.merge_rows, po, ml, at, 3, 0, 0)
     refused("invalid_argument", wg.first_rows, 3)
 
 
