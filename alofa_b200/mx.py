@@ -32,8 +32,6 @@ from .csrc import ops
 from .errors import AlofaError
 
 BLOCK, GROUP, TILE_ROWS, TILE_BYTES, GATE_ROWS = 32, 128, 128, 8704, 16  # as in kernels/mx.cuh
-TOKEN_TILES = (16, 32, 64, 128, 256)  # tokens that a CTA of the product may take, the last a pair of CTAs
-MOST_PARTS = 8  # of a depth
 MOST_WIDTH = 32768  # numbers of a row that the norm takes
 
 _BF16, _F32, _U8, _I32 = torch.bfloat16, torch.float32, torch.uint8, torch.int32
@@ -315,10 +313,10 @@ def _sms(here: int) -> int:
     return _SMS[here]
 
 
-# What a product takes, fitted to the times of every way at the shapes of 0.5 to 7 billion parameters and 1 to 1,536 tokens: the way
-# it chooses is 2.4 % off the fastest on the average.  Microseconds for a slice of 128 numbers of a CTA of the kernel for a few
+# What a product takes, fitted to the times of every way at the shapes of 0.5 to 7 billion parameters and 1 to 1,024 tokens: the way
+# it chooses is 1.3 % off the fastest on the average.  Microseconds for a slice of 128 numbers of a CTA of the kernel for a few
 # tokens, by its tokens: alone on its SM, and where two share one.
-_FEW_SLICE = {16: (0.27, 0.40), 32: (0.31, 0.42), 64: (0.30, 0.49), 128: (0.72, 1.29)}
+_FEW_SLICE = {16: (0.354, 0.400), 32: (0.225, 0.241), 64: (0.326, 0.420), 128: (0.743, 0.866)}
 
 
 def _few_us(tokens: int, rows: int, slices: int, gated: bool, bn: int, parts: int, sms: int) -> float:
@@ -327,30 +325,32 @@ def _few_us(tokens: int, rows: int, slices: int, gated: bool, bn: int, parts: in
     room = 2 * sms if parts == 1 else int(0.946 * 2 * sms)  # clusters do not fill every SM
     whole, rest = divmod(ctas, room)
     rounds = whole * shared + (shared if rest > sms else alone if rest else 0.0)
-    return 2.9 + 0.15 * parts + (0.3 * parts + 0.044 * bn if gated else 0.0) + rounds * -(-slices // parts) + 3.1 * (whole - (rest == 0))
+    last = (0.055 * (whole + (rest > 0)) if gated else 0.01) * min(tokens, bn) / parts  # a tile's last step: its tokens, over its parts
+    return 4.94 + 0.226 * parts + last + rounds * -(-slices // parts) + 3.69 * (whole - (rest == 0))
 
 
 def _pair_us(tokens: int, rows: int, slices: int, sms: int) -> float:
     tiles = -(-rows // 256) * -(-tokens // 256)
-    return 5.4 + -(-tiles // (sms // 2)) * (0.8 + 0.454 * slices)
+    return 5.4 + -(-tiles // (sms // 2)) * (0.8 + 0.499 * slices)
 
 
 def plan(tokens: int, rows: int, depth: int, gated: bool = False) -> tuple:
     """(tokens a tile, parts of the depth) of a product; 256 tokens: pairs of CTAs.
 
-    The kernel for a few tokens has one tile of up to 64 of them, and its depth
-    goes in as many parts as make it shortest (us, depth x rows): 1 token, 18,944
-    x 3,584 in 8 parts 10.4, in 4 12.8; 896 x 9,728 gated undivided 3.9, in 2
-    parts 4.5.  Beyond 64 tokens tiles of 64 or 128 of it are weighed against
-    pairs, which take long to begin and then do a slice of 256 x 256 in the time
-    the others take for a quarter of it: 256 tokens, 3,584 x 4,608 10.7 in tiles
-    of 64 and 16.6 on pairs; 192 tokens, 3,584 x 37,888 gated 51.8 and 33.2;
-    1,024 tokens, 18,944 x 3,584 91.5 and 59.3, 8,960 x 1,536 27.0 and 30.2."""
+    The kernel for a few tokens has tiles of up to 32 of them in steps of as many,
+    of 32 or 64 in larger ones; its depth goes in as many parts as make it
+    shortest (us, depth x rows): 1 token, 18,944 x 3,584 in 8 parts 10.4, in 4
+    12.8; 64 tokens, 896 x 9,728 gated in tiles of 32 8.1 and of 64 8.4.  Beyond 64
+    tokens it is weighed against pairs, which take long to begin and then do a
+    slice of 256 x 256 in the time the others take for a quarter of it: 256
+    tokens, 3,584 x 4,608 11.4 in tiles of 64 and 16.7 on pairs; 192 tokens, 3,584
+    x 37,888 gated 51.8 and 33.2; 1,024 tokens, 18,944 x 3,584 91.5 and 59.3,
+    8,960 x 1,536 27.0 and 30.2."""
     key = (tokens, rows, depth, gated)
     found = _plans.get(key)
     if found is None:
         slices, sms = padded(depth) // GROUP, _sms(_here())
-        tiles = [next(b for b in TOKEN_TILES if tokens <= b)] if tokens <= 64 else [64, 128]
+        tiles = (16,) if tokens <= 16 else (32,) if tokens <= 32 else (32, 64) if tokens <= 64 else (32, 64, 128) if tokens <= 96 else (64, 128)
         ways = [(_few_us(tokens, rows, slices, gated, bn, parts, sms), bn, parts) for bn in tiles for parts in (1, 2, 3, 4, 6, 8) if parts <= slices]
         if tokens > 64:
             ways.append((_pair_us(tokens, rows, slices, sms), 256, 1))

@@ -70,7 +70,7 @@ def norm(h, weight, eps, shift=None):
 
 
 def silu(g):
-    return g / (1 + np.exp(-g))
+    return g / (1 + np.exp(-np.maximum(g, -700)))  # below it is zero in 64 bits too
 
 
 def near(codes, scales, y, slack):

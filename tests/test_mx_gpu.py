@@ -286,6 +286,23 @@ def test_scales_over_their_whole_range():
     assert np.array_equal(got[normal], want[normal])
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_any_size(seed):
+    """Sizes drawn over the whole range, each the way the rule chooses."""
+    rng = np.random.default_rng(seed)
+    t, n, k = (int(np.exp(rng.uniform(0, np.log(most)))) for most in (1500, 3000, 4000))
+    xr, wp, xv, wv = product_operands(t, n, k, 70 + seed)
+    got = mx.linear(xr, wp, dtype=F32)
+    assert (np.abs(host(got) - xv @ wv.T) <= sum_bound(xv, wv)).all(), (t, n, k)
+    rows = mx.gated_linear(xr, mx.pack_weight(numbers(2 * n, k, 71 + seed, F32, 0.05).cuda(), True))
+    wg = plain.values(numbers(2 * n, k, 71 + seed, F32, 0.05), True)
+    g, u = xv @ wg[:n].T, xv @ wg[n:].T
+    want, slope = plain.silu(g) * u, 1.1 * np.abs(u) * sum_bound(xv, wg[:n]) + (np.abs(g) + 1) * sum_bound(xv, wg[n:])
+    largest = np.abs(np.pad(want, ((0, 0), (0, -n % 32)))).reshape(t, -1, 32).max(-1).repeat(32, -1)[:, :n]
+    off = np.abs(host(rows.dequantize(F32)).astype(np.float64) - want)
+    assert (off <= np.maximum(2.0**-4 * np.abs(want), 2.0**-17 * largest) * (1 + 2.0**-10) + slope).all(), (t, n, k)
+
+
 def test_a_block_of_nan_reaches_its_row_only():
     xr, wp, xv, wv = product_operands(5, 140, 300, 30)
     xr.scales[2, 1] = 255  # a view of the rows' own memory
@@ -313,7 +330,7 @@ def test_gated_linear(t, f, k, how, gate):
     else:
         a, top = gate
         g, u = np.minimum(g, top), np.clip(u, -top, top)
-        want, slope = g / (1 + np.exp(-a * g)) * (u + 1), 1.1 * (np.abs(u) + 1) * eg + (np.abs(g) + eg) * eu
+        want, slope = g / (1 + np.exp(np.minimum(-a * g, 700))) * (u + 1), 1.1 * (np.abs(u) + 1) * eg + (np.abs(g) + eg) * eu
     got = host(rows.dequantize(F32)).astype(np.float64)
     assert rows.shape == (t, f) and not host(rows.codes)[:, f:].any()
     unit = np.exp2(host(rows.scales).astype(np.float64) - 127).repeat(32, -1)[:, :f]
