@@ -6,8 +6,13 @@
 //   alofa_mx_rows_values, alofa_mx_weight_values   the numbers that rows, or a weight, stand for
 // Kp is K rounded up to whole groups of 128; the codes behind K are zeros.
 //
-// All of them are bound by memory: a lane takes eight or sixteen neighbouring numbers, the lanes that share a
-// block find its largest magnitude by one or two shuffles, and codes are converted by the hardware's instructions.
+// All of them are bound by memory, and all but the packing are there twice.  WHOLE: rows that begin on 16 bytes and are whole groups
+// of eight numbers: a lane takes eight or sixteen neighbouring ones with 16-byte loads, and the lanes that share a
+// block find its largest magnitude by one or two shuffles.  Every other width: a block is 32 lanes, a number each
+// (one instruction finds the largest), and a lane takes the same place of eight blocks: loads and stores of 2 or 4
+// bytes, but of whole lines a warp (1,999 rows of 1,537 numbers turned back: 22.2 us when each lane took eight
+// neighbouring ones, 9.2 so; the norm of as many with a plane 16.3 and 11.8).  Packing has four reductions a lane
+// that way where it has one with neighbours: 8,960 x 1,537 41.6 us, and 17.4 with eight loads of a number each.
 #include <string.h>
 
 #include "mx.cuh"
@@ -54,6 +59,49 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8], int have, bo
     if (j < have) dst[j] = from_f<T>(v[j]);
 }
 
+// Where a thread's eight numbers are: WHOLE eight neighbouring ones, else the lane's place in eight blocks that the warp
+// has in turn.  `unit` counts threads along the row, 32 to a warp.
+template <bool WHOLE>
+struct Eight {
+  int at;
+  __device__ __forceinline__ explicit Eight(int unit) : at(WHOLE ? unit * 8 : (unit >> 5) * 256 + (unit & 31)) {}
+  __device__ __forceinline__ int operator[](int j) const { return at + (WHOLE ? j : 32 * j); }
+};
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void load_eight(float (&v)[8], const T* row, Eight<WHOLE> e, int k) {
+  if constexpr (WHOLE) {
+    load8(v, row + e.at, k - e.at, true);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = e[j] < k ? to_f(row[e[j]]) : 0.f;
+  }
+}
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void store_eight(T* row, const float (&v)[8], Eight<WHOLE> e, int k) {
+  if constexpr (WHOLE) {
+    store8(row + e.at, v, k - e.at, true);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (e[j] < k) row[e[j]] = from_f<T>(v[j]);
+  }
+}
+// The same eight numbers as codes and scales of a row (every lane of the warp takes part).
+template <bool WHOLE>
+__device__ __forceinline__ void put_eight(const float (&v)[8], uint8_t* codes, uint8_t* scales, Eight<WHOLE> e, int kp, bool live) {
+  if constexpr (WHOLE) {
+    mx_put8(v, codes + e.at, scales + e.at / MX_BLOCK, live && e.at < kp);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t s = mx_row_scale(__reduce_max_sync(0xffffffffu, mx_size(v[j])));
+      if (!live || e[j] >= kp) continue;
+      codes[e[j]] = s == 255u ? (uint8_t)0 : (uint8_t)mx_e4m3(v[j] * mx_over(s), 0.f, 0.f, 0.f);
+      if ((threadIdx.x & 31) == 0) scales[e[j] / MX_BLOCK] = (uint8_t)s;
+    }
+  }
+}
+
 static inline int padded(int k) { return (k + MX_GROUP - 1) / MX_GROUP * MX_GROUP; }
 static inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -62,7 +110,7 @@ static inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n 
 // (a 64-bit division by the row's length was a third of the instructions); what they address is 64.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) mx_rows_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, unsigned chunks, int k, int kp, bool whole) {
+__global__ void __launch_bounds__(256) mx_rows_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, unsigned chunks, int k, int kp) {
   pdl_wait();
   pdl_launch();
   const unsigned i = blockIdx.x * blockDim.x + threadIdx.x, per_row = (unsigned)kp >> 4;  // a multiple of 8: a block's two lanes are in one row
@@ -71,7 +119,7 @@ __global__ void __launch_bounds__(256) mx_rows_kernel(uint8_t* __restrict__ code
   const int c = live ? (int)(i - row * per_row) * 16 : 0;
   float v[2][8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) load8(v[h], x + (size_t)row * k + c + 8 * h, live ? k - c - 8 * h : 0, whole);
+  for (int h = 0; h < 2; ++h) load8(v[h], x + (size_t)row * k + c + 8 * h, live ? k - c - 8 * h : 0, true);
   uint32_t largest = 0;
 #pragma unroll
   for (int j = 0; j < 16; ++j) largest = max(largest, mx_size(v[j >> 3][j & 7]));
@@ -90,55 +138,85 @@ __global__ void __launch_bounds__(256) mx_rows_kernel(uint8_t* __restrict__ code
   if ((threadIdx.x & 1) == 0) scales[(size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK] = (uint8_t)s;
 }
 
+// Every other width: a warp has 256 numbers of a row.
+template <typename T>
+__global__ void __launch_bounds__(256) mx_rows_any_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ x, unsigned warps, int k, int kp) {
+  pdl_wait();
+  pdl_launch();
+  const unsigned warp = blockIdx.x * 8 + (threadIdx.x >> 5), per_row = (unsigned)(kp + 255) >> 8;
+  const bool live = warp < warps;
+  const size_t row = live ? warp / per_row : 0u;
+  const Eight<false> e((int)(live ? warp % per_row : 0u) * 32 + (int)(threadIdx.x & 31));
+  float v[8];
+  load_eight(v, x + row * k, e, live ? k : 0);
+  put_eight(v, codes + row * kp, scales + row * (kp / MX_BLOCK), e, kp, live);
+}
+
 ALOFA_API int alofa_mx_rows(void* codes, void* scales, const void* x, int t, int k, int bf16_x, void* stream) {
   if (t < 0 || k <= 0 || k > (1 << 30) || !aligned(codes, 16)) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
   const int kp = padded(k);
-  const long long chunks = (long long)t * (kp / 16);
-  if (chunks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
-  const unsigned blocks = (unsigned)((chunks + 255) / 256);
   const bool whole = k % 8 == 0 && aligned(x, 16);
-  if (bf16_x)
-    launch_dep(mx_rows_kernel<bf16>, blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const bf16*)x, (unsigned)chunks, k, kp, whole);
-  else
-    launch_dep(mx_rows_kernel<float>, blocks, 256, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, (const float*)x, (unsigned)chunks, k, kp, whole);
+  const long long units = whole ? (long long)t * (kp / 16) : (long long)t * ((kp + 255) / 256);  // lanes, or warps
+  if (units > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  const unsigned blocks = (unsigned)(whole ? (units + 255) / 256 : (units + 7) / 8);
+  cudaStream_t s = (cudaStream_t)stream;
+  uint8_t *c = (uint8_t*)codes, *e = (uint8_t*)scales;
+  if (whole && bf16_x) launch_dep(mx_rows_kernel<bf16>, blocks, 256, 0, s, c, e, (const bf16*)x, (unsigned)units, k, kp);
+  else if (whole) launch_dep(mx_rows_kernel<float>, blocks, 256, 0, s, c, e, (const float*)x, (unsigned)units, k, kp);
+  else if (bf16_x) launch_dep(mx_rows_any_kernel<bf16>, blocks, 256, 0, s, c, e, (const bf16*)x, (unsigned)units, k, kp);
+  else launch_dep(mx_rows_any_kernel<float>, blocks, 256, 0, s, c, e, (const float*)x, (unsigned)units, k, kp);
   return launch_status();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) mx_rows_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, unsigned chunks, int k, int kp, bool whole) {
+// Turned back: a lane has eight numbers (a warp's stores are whole lines; with sixteen they were every other 16 bytes: 1,999
+// rows of 18,944 24.3 us, and 21.0 so), a thread two such places.
+constexpr int VALUES_THREADS = 256, VALUES_PLACES = 2 * VALUES_THREADS;
+
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(VALUES_THREADS) mx_rows_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, unsigned units, int k, int kp) {
   pdl_wait();
   pdl_launch();
-  const unsigned i = blockIdx.x * blockDim.x + threadIdx.x, per_row = (unsigned)(k + 15) >> 4;
-  if (i >= chunks) return;
-  const unsigned row = i / per_row;
-  const int c = (int)(i - row * per_row) * 16;
-  const uint4 p = *reinterpret_cast<const uint4*>(codes + (size_t)row * kp + c);
-  const float by = mx_power(scales[(size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK]);
-  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+  const unsigned per_row = WHOLE ? (unsigned)k >> 3 : (unsigned)(kp + 255) / 256 * 32;  // not WHOLE: whole warps
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
+    const unsigned i = blockIdx.x * VALUES_PLACES + h * VALUES_THREADS + threadIdx.x;
+    if (i >= units) return;
+    const size_t row = i / per_row;
+    const Eight<WHOLE> e((int)(i - (unsigned)row * per_row));
+    const uint8_t *c = codes + row * kp, *s = scales + row * (kp / MX_BLOCK);
     float v[8];
+    if constexpr (WHOLE) {
+      const uint2 p = *reinterpret_cast<const uint2*>(c + e.at);
+      const float by = mx_power(s[e.at / MX_BLOCK]);
+      const uint32_t w[2] = {p.x, p.y};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 two = mx_from_e4m3((uint16_t)(w[2 * h + (j >> 1)] >> (16 * (j & 1))));
-      v[2 * j] = two.x * by, v[2 * j + 1] = two.y * by;
+      for (int j = 0; j < 4; ++j) {
+        const float2 two = mx_from_e4m3((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+        v[2 * j] = two.x * by, v[2 * j + 1] = two.y * by;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = e[j] < k ? mx_from_e4m3(c[e[j]]).x * mx_power(s[e[j] / MX_BLOCK]) : 0.f;
     }
-    store8(out + (size_t)row * k + c + 8 * h, v, k - c - 8 * h, whole);
+    store_eight(out + row * k, v, e, k);
   }
 }
 
 ALOFA_API int alofa_mx_rows_values(void* out, const void* codes, const void* scales, int t, int k, int bf16_out, void* stream) {
   if (t < 0 || k <= 0 || k > (1 << 30) || !aligned(codes, 16)) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
-  const long long chunks = (long long)t * ((k + 15) / 16);
-  if (chunks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
-  const unsigned blocks = (unsigned)((chunks + 255) / 256);
+  const int kp = padded(k);
   const bool whole = k % 8 == 0 && aligned(out, 16);
-  if (bf16_out)
-    launch_dep(mx_rows_values_kernel<bf16>, blocks, 256, 0, (cudaStream_t)stream, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, (unsigned)chunks, k, padded(k), whole);
-  else
-    launch_dep(mx_rows_values_kernel<float>, blocks, 256, 0, (cudaStream_t)stream, (float*)out, (const uint8_t*)codes, (const uint8_t*)scales, (unsigned)chunks, k, padded(k), whole);
+  const long long units = (long long)t * (whole ? k / 8 : (kp + 255) / 256 * 32);
+  if (units > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
+  const unsigned blocks = (unsigned)((units + VALUES_PLACES - 1) / VALUES_PLACES);
+  cudaStream_t s = (cudaStream_t)stream;
+  const uint8_t *c = (const uint8_t*)codes, *e = (const uint8_t*)scales;
+  if (whole && bf16_out) launch_dep(mx_rows_values_kernel<bf16, true>, blocks, VALUES_THREADS, 0, s, (bf16*)out, c, e, (unsigned)units, k, kp);
+  else if (whole) launch_dep(mx_rows_values_kernel<float, true>, blocks, VALUES_THREADS, 0, s, (float*)out, c, e, (unsigned)units, k, kp);
+  else if (bf16_out) launch_dep(mx_rows_values_kernel<bf16, false>, blocks, VALUES_THREADS, 0, s, (bf16*)out, c, e, (unsigned)units, k, kp);
+  else launch_dep(mx_rows_values_kernel<float, false>, blocks, VALUES_THREADS, 0, s, (float*)out, c, e, (unsigned)units, k, kp);
   return launch_status();
 }
 
@@ -147,30 +225,29 @@ ALOFA_API int alofa_mx_rows_values(void* out, const void* codes, const void* sca
 // read once, with all its loads in flight together, four planes of owed sums at a time.  Sums are taken in a
 // fixed order.  Formula: src/alofa/kernels/cpu/scalar.mojo:93-129.
 // ---------------------------------------------------------------------------
-template <int CH>
+template <int CH, bool WHOLE>
 __global__ void __launch_bounds__(512) mx_norm_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, float* h, const float* base, const float* __restrict__ owed, int splits,
-                                                      const float* __restrict__ bias, const float* __restrict__ w, const float* __restrict__ shift, int t, int k, int kp, float eps, bool whole) {
+                                                      const float* __restrict__ bias, const float* __restrict__ w, const float* __restrict__ shift, int t, int k, int kp, float eps) {
   __shared__ float scratch[32];
   pdl_wait();
   const int row = blockIdx.x;
   const size_t at = (size_t)row * k, plane = (size_t)t * k;
   constexpr int PLANES = CH == 1 ? 4 : 1;
+  auto place = [&](int i) { return Eight<WHOLE>((int)(threadIdx.x + i * blockDim.x)); };
   float v[CH][8], g[CH == 1 ? 1 : CH][8];
   float ss = 0.f, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int c = (threadIdx.x + i * blockDim.x) * 8;
-    load8(v[i], base + at + c, k - c, whole);
-    if (CH == 1) load8(g[i], w + c, k - c, whole);
+    load_eight(v[i], base + at, place(i), k);
+    if (CH == 1) load_eight(g[i], w, place(i), k);
   }
   int z = 0;
   for (; z + PLANES <= splits; z += PLANES) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int c = (threadIdx.x + i * blockDim.x) * 8;
       float p[PLANES][8];
 #pragma unroll
-      for (int q = 0; q < PLANES; ++q) load8(p[q], owed + (z + q) * plane + at + c, k - c, whole);
+      for (int q = 0; q < PLANES; ++q) load_eight(p[q], owed + (z + q) * plane + at, place(i), k);
 #pragma unroll
       for (int q = 0; q < PLANES; ++q)
 #pragma unroll
@@ -180,9 +257,8 @@ __global__ void __launch_bounds__(512) mx_norm_kernel(uint8_t* __restrict__ code
   for (; z < splits; ++z) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int c = (threadIdx.x + i * blockDim.x) * 8;
       float p[8];
-      load8(p, owed + z * plane + at + c, k - c, whole);
+      load_eight(p, owed + z * plane + at, place(i), k);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] += p[j];
     }
@@ -190,14 +266,13 @@ __global__ void __launch_bounds__(512) mx_norm_kernel(uint8_t* __restrict__ code
   pdl_launch();
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int c = (threadIdx.x + i * blockDim.x) * 8, have = k - c;
     if (bias) {
       float p[8];
-      load8(p, bias + c, have, whole);
+      load_eight(p, bias, place(i), k);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] += p[j];
     }
-    if (owed || bias || h != base) store8(h + at + c, v[i], have, whole);
+    if (owed || bias || h != base) store_eight(h + at, v[i], place(i), k);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       ss = fmaf(v[i][j], v[i][j], ss);
@@ -210,10 +285,9 @@ __global__ void __launch_bounds__(512) mx_norm_kernel(uint8_t* __restrict__ code
     ss = 0.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int c = (threadIdx.x + i * blockDim.x) * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float d = c + j < k ? v[i][j] - mean : 0.f;
+        const float d = place(i)[j] < k ? v[i][j] - mean : 0.f;
         ss = fmaf(d, d, ss);
       }
     }
@@ -222,15 +296,14 @@ __global__ void __launch_bounds__(512) mx_norm_kernel(uint8_t* __restrict__ code
   const float scale = 1.0f / sqrtf(ss / (float)k + eps);
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int c = (threadIdx.x + i * blockDim.x) * 8, have = k - c;
     float s[8];
-    if (CH > 1) load8(g[i], w + c, have, whole);
+    if (CH > 1) load_eight(g[i], w, place(i), k);
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] = 0.f;
-    if (shift) load8(s, shift + c, have, whole);
+    if (shift) load_eight(s, shift, place(i), k);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = c + j < k ? fmaf((v[i][j] - mean) * scale, g[i][j], s[j]) : 0.f;
-    mx_put8(v[i], codes + (size_t)row * kp + c, scales + (size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK, c < kp);
+    for (int j = 0; j < 8; ++j) v[i][j] = place(i)[j] < k ? fmaf((v[i][j] - mean) * scale, g[i][j], s[j]) : 0.f;
+    put_eight(v[i], codes + (size_t)row * kp, scales + (size_t)row * (kp / MX_BLOCK), place(i), kp, true);
   }
 }
 
@@ -238,14 +311,19 @@ ALOFA_API int alofa_mx_norm(void* codes, void* scales, float* h, const float* ba
                             void* stream) {
   if (t < 0 || k <= 0 || splits < 0 || !aligned(codes, 8)) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
+  if (!splits) owed = nullptr;
   const int kp = padded(k), chunks = kp / 8;
   // a chunk a thread where the rows are few and a row's time is what counts, two where they are many: 2,048 rows of 3,584
-  // with one plane 21.4 and 18.9 us, one row of 896 with four planes 3.8 and 5.8
+  // with one plane 21.4 and 18.9 us, one row of 896 with four planes 3.8 and 5.8 (blocks that stay and ask for their next
+  // row ahead: 18.9 us, and without a plane 16.9 instead of 13.8)
   const int per = chunks <= (t >= 2 * 148 ? 256 : 512) ? 1 : chunks <= 1024 ? 2 : chunks <= 2048 ? 4 : 8, threads = ((chunks + per - 1) / per + 31) / 32 * 32;
   if (threads > 512) return ALOFA_ERR_ARGUMENT;
-  bool whole = k % 8 == 0 && aligned(h, 16) && aligned(base, 16) && aligned(owed, 16) && aligned(bias, 16) && aligned(w, 16) && aligned(shift, 16);
-  if (!splits) owed = nullptr;
-#define GO(CH) launch_dep(mx_norm_kernel<CH>, t, threads, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, h, base, owed, splits, bias, w, shift, t, k, kp, eps, whole)
+  const bool whole = k % 8 == 0 && aligned(h, 16) && aligned(base, 16) && aligned(owed, 16) && aligned(bias, 16) && aligned(w, 16) && aligned(shift, 16);
+#define GO(CH)                                                                                                                                                                        \
+  do {                                                                                                                                                                                \
+    if (whole) launch_dep(mx_norm_kernel<CH, true>, t, threads, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, h, base, owed, splits, bias, w, shift, t, k, kp, eps);        \
+    else launch_dep(mx_norm_kernel<CH, false>, t, threads, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, h, base, owed, splits, bias, w, shift, t, k, kp, eps);             \
+  } while (0)
   switch (per) {
     case 1: GO(1); break;
     case 2: GO(2); break;
@@ -335,19 +413,19 @@ __device__ __forceinline__ int weight_source_row(int r, int n, int features) {
 
 constexpr int PACK_THREADS = 512, PACK_TILES = 4;  // tiles of a block, where there are enough for two blocks an SM (one each otherwise)
 
-template <typename T>
-struct Raw8 {  // eight numbers as they are loaded
+template <typename T, bool WHOLE>
+struct Raw8 {  // eight neighbouring numbers as they are loaded, the first `have` of them
   uint4 q[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* src, int have, bool whole) {
-    if (whole && have >= 8) {
+  __device__ __forceinline__ void load(const T* src, int have) {
+    if constexpr (WHOLE) {
 #pragma unroll
-      for (int j = 0; j < (int)(sizeof(T) / 2); ++j) q[j] = reinterpret_cast<const uint4*>(src)[j];
-      return;
+      for (int j = 0; j < (int)(sizeof(T) / 2); ++j) q[j] = have > 0 ? reinterpret_cast<const uint4*>(src)[j] : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      T v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < have ? src[j] : from_f<T>(0.f);
+      memcpy(q, v, sizeof(v));
     }
-    T v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < have ? src[j] : from_f<T>(0.f);
-    memcpy(q, v, sizeof(v));
   }
   __device__ __forceinline__ void numbers(float (&v)[8]) const {
     if constexpr (sizeof(T) == 2) {
@@ -360,8 +438,8 @@ struct Raw8 {  // eight numbers as they are loaded
   }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 2 ? 2 : 1) mx_pack_kernel(uint8_t* __restrict__ tiles, const T* __restrict__ w, int n, int k, int slices, int each, int features, bool whole) {
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 2 ? 2 : 1) mx_pack_kernel(uint8_t* __restrict__ tiles, const T* __restrict__ w, int n, int k, int slices, int each, int features) {
   const int c = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4, first = blockIdx.x * each, last = min(slices, first + each);
   const T* src[4];
   bool there[4];
@@ -371,17 +449,17 @@ __global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 2 ? 2 : 1) mx_pack_
     there[i] = row >= 0;
     src[i] = w + (size_t)max(row, 0) * k + c;
   }
-  Raw8<T> next[4];
+  Raw8<T, WHOLE> next[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) next[i].load(src[i] + first * MX_GROUP, there[i] ? k - c - first * MX_GROUP : 0, whole);
+  for (int i = 0; i < 4; ++i) next[i].load(src[i] + first * MX_GROUP, there[i] ? k - c - first * MX_GROUP : 0);
   for (int s = first; s < last; ++s) {
     uint8_t* tile = tiles + ((size_t)blockIdx.y * slices + s) * MX_TILE_BYTES;
-    Raw8<T> now[4];
+    Raw8<T, WHOLE> now[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) now[i] = next[i];
     if (s + 1 < last) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) next[i].load(src[i] + (s + 1) * MX_GROUP, there[i] ? k - c - (s + 1) * MX_GROUP : 0, whole);
+      for (int i = 0; i < 4; ++i) next[i].load(src[i] + (s + 1) * MX_GROUP, there[i] ? k - c - (s + 1) * MX_GROUP : 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -414,19 +492,21 @@ ALOFA_API int alofa_mx_pack(void* tiles, const void* w, int n, int k, int gated,
   const long long rows = gated ? 2ll * ((n / 2 + 15) / 16 * 16) : n, tall = (rows + MX_TILE_ROWS - 1) / MX_TILE_ROWS;
   if (tall > 65535) return ALOFA_ERR_ARGUMENT;
   const int slices = padded(k) / MX_GROUP;
-  const int each = slices * tall >= 2 * 148 * PACK_TILES ? PACK_TILES : 1;
-  const dim3 grid((unsigned)((slices + each - 1) / each), (unsigned)tall);
   const bool whole = k % 8 == 0 && aligned(w, 16);
-  if (bf16_w)
-    launch_whole(mx_pack_kernel<bf16>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const bf16*)w, n, k, slices, each, gated ? n / 2 : 0, whole);
-  else
-    launch_whole(mx_pack_kernel<float>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (uint8_t*)tiles, (const float*)w, n, k, slices, each, gated ? n / 2 : 0, whole);
+  const int each = whole && slices * tall >= 2 * 148 * PACK_TILES ? PACK_TILES : 1;
+  const dim3 grid((unsigned)((slices + each - 1) / each), (unsigned)tall);
+  const int features = gated ? n / 2 : 0;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (whole && bf16_w) launch_whole(mx_pack_kernel<bf16, true>, grid, PACK_THREADS, 0, s, (uint8_t*)tiles, (const bf16*)w, n, k, slices, each, features);
+  else if (whole) launch_whole(mx_pack_kernel<float, true>, grid, PACK_THREADS, 0, s, (uint8_t*)tiles, (const float*)w, n, k, slices, each, features);
+  else if (bf16_w) launch_whole(mx_pack_kernel<bf16, false>, grid, PACK_THREADS, 0, s, (uint8_t*)tiles, (const bf16*)w, n, k, slices, each, features);
+  else launch_whole(mx_pack_kernel<float, false>, grid, PACK_THREADS, 0, s, (uint8_t*)tiles, (const float*)w, n, k, slices, each, features);
   const int rc = launch_status();
   return rc ? rc : alofa_mx_settle(stream);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(PACK_THREADS) mx_weight_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ tiles, int n, int k, int features, bool whole) {
+__global__ void __launch_bounds__(PACK_THREADS) mx_weight_values_kernel(T* __restrict__ out, const uint8_t* __restrict__ tiles, int n, int k, int features) {
   const uint8_t* tile = tiles + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * MX_TILE_BYTES;
   const int c = (threadIdx.x & 15) * 8, kc = blockIdx.x * MX_GROUP + c, r0 = threadIdx.x >> 4;
   pdl_wait();
@@ -447,7 +527,25 @@ __global__ void __launch_bounds__(PACK_THREADS) mx_weight_values_kernel(T* __res
       const float2 two = mx_from_e2m1(p[i] >> (8 * j));
       v[2 * j] = two.x * by, v[2 * j + 1] = two.y * by;
     }
-    if (src >= 0 && kc < k) store8(out + (size_t)src * k + kc, v, k - kc, whole);
+    if (src >= 0 && kc < k) store8(out + (size_t)src * k + kc, v, k - kc, true);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PACK_THREADS) mx_weight_values_any_kernel(T* __restrict__ out, const uint8_t* __restrict__ tiles, int n, int k, int features) {
+  const uint8_t* tile = tiles + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * MX_TILE_BYTES;
+  const int lane = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * 8, kc = blockIdx.x * MX_GROUP + lane;
+  pdl_wait();
+  pdl_launch();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + i, src = weight_source_row(blockIdx.y * MX_TILE_ROWS + r, n, features);
+    if (src < 0) continue;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const uint32_t code = tile[r * (MX_GROUP / 2) + b * 16 + lane / 2] >> (4 * (lane & 1));
+      if (kc + 32 * b < k) out[(size_t)src * k + kc + 32 * b] = from_f<T>(mx_from_e2m1(code & 15u).x * mx_power(tile[MX_TILE_CODES + mx_scale_at(r, b)]));
+    }
   }
 }
 
@@ -457,9 +555,11 @@ ALOFA_API int alofa_mx_weight_values(void* out, const void* tiles, int n, int k,
   if (tall > 65535) return ALOFA_ERR_ARGUMENT;
   const dim3 grid((unsigned)(padded(k) / MX_GROUP), (unsigned)tall);
   const bool whole = k % 8 == 0 && aligned(out, 16);
-  if (bf16_out)
-    launch_dep(mx_weight_values_kernel<bf16>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (bf16*)out, (const uint8_t*)tiles, n, k, gated ? n / 2 : 0, whole);
-  else
-    launch_dep(mx_weight_values_kernel<float>, grid, PACK_THREADS, 0, (cudaStream_t)stream, (float*)out, (const uint8_t*)tiles, n, k, gated ? n / 2 : 0, whole);
+  const int features = gated ? n / 2 : 0;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (whole && bf16_out) launch_dep(mx_weight_values_kernel<bf16>, grid, PACK_THREADS, 0, s, (bf16*)out, (const uint8_t*)tiles, n, k, features);
+  else if (whole) launch_dep(mx_weight_values_kernel<float>, grid, PACK_THREADS, 0, s, (float*)out, (const uint8_t*)tiles, n, k, features);
+  else if (bf16_out) launch_dep(mx_weight_values_any_kernel<bf16>, grid, PACK_THREADS, 0, s, (bf16*)out, (const uint8_t*)tiles, n, k, features);
+  else launch_dep(mx_weight_values_any_kernel<float>, grid, PACK_THREADS, 0, s, (float*)out, (const uint8_t*)tiles, n, k, features);
   return launch_status();
 }
