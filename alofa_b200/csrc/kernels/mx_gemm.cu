@@ -112,6 +112,12 @@ constexpr uint32_t mx_idesc(uint32_t a, uint32_t b, int m, int n, int block) {
   return (a << 7) | (b << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27) | ((uint32_t)block << 29) | ((uint32_t)block << 4);
 }
 
+// An arrival on another CTA's barrier that says only that this warp's reads of tensor memory are over (they are complete, and
+// tcgen05.fence::before_thread_sync stands between): nothing of ordinary memory goes with it.  As a release for the cluster it
+// took 1,200 to 1,500 clocks, and the next tile's products wait for it.
+__device__ __forceinline__ void tell_in_cluster(uint32_t bar_in_cluster) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_in_cluster) : "memory");
+}
 __device__ __forceinline__ uint32_t cta_in_cluster() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -618,13 +624,17 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
       uint32_t round = 0;
       bool ok = true, ready = false, place_free = true;
       for (int tile = pair; tile < n_tiles && ok; tile += n_pairs, ++done) {
-        if (done) ok = all_lanes(mbar_wait_in_cluster(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag));
+        // the tile's first slice and scales are there before the epilogue has the columns that this accumulator shares with the last one
+        ok = all_lanes(mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag));
+        if (ok && !all_lanes(ready)) ok = all_lanes(mbar_wait(&landed[s], round, &abort_flag));
+        ready = true;
+        if (ok && done) ok = all_lanes(mbar_wait(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag));
         if (!ok) break;
         tc_fence_after();
         const uint32_t sums = base + (done & 1 ? PAIR_SECOND : 0);
         for (int i = 0; i < slices; ++i, ++it) {
-          if (i % PAIR_CHUNK == 0) ok = all_lanes(mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag));
-          if (ok && !all_lanes(ready)) ok = all_lanes(mbar_wait_in_cluster(&landed[s], round, &abort_flag));
+          if (i % PAIR_CHUNK == 0 && i) ok = all_lanes(mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag));
+          if (ok && !all_lanes(ready)) ok = all_lanes(mbar_wait(&landed[s], round, &abort_flag));
           // the slice before it in this place of the scales: five slices ago, whose stage is the next one's now
           if (ok && !all_lanes(place_free)) ok = all_lanes(mbar_wait(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it - PAIR_SCALE_PLACES) / STAGES) & 1u, &abort_flag));
           if (!ok) break;
@@ -636,7 +646,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
           place = place + 1 == PAIR_SCALE_PLACES ? 0 : place + 1;
           round ^= s == 0 ? 1u : 0u;
           tc_fence_after();
-          ready = mbar_complete_in_cluster(&landed[s], round);
+          ready = mbar_complete(&landed[s], round);
           place_free = it + 1 < PAIR_SCALE_PLACES || mbar_complete(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it + 1 - PAIR_SCALE_PLACES) / STAGES) & 1u);
           const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + A_BYTES);
           const bool chunk_ends = i % PAIR_CHUNK == PAIR_CHUNK - 1 || i == slices - 1;
@@ -674,7 +684,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
       const bool second = done & 1, shared_half = half == (second ? 0 : 1);  // the shared columns: the first tile's last, the second's first
       const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (second ? PAIR_SECOND : 0) + half * 128;
       if (!shared_half) {  // this half's columns are no part of the next tile's accumulator
-        if (lane == 0) mbar_arrive_in_cluster(taken);
+        if (lane == 0) tell_in_cluster(taken);
       }
 #pragma unroll 1
       for (int k = 0; k < 2; ++k) {
@@ -684,7 +694,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
         if (k == 0 && shared_half) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_in_cluster(taken);
+          if (lane == 0) tell_in_cluster(taken);
         }
         if (!args.F) pair_stored64(args, r, t - lane, row0 + block * 64, good, turn, lane);
         else if (t >= args.T) continue;

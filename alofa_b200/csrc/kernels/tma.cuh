@@ -50,18 +50,7 @@ __device__ __forceinline__ bool mbar_complete(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// The same two where CTAs of a cluster arrive on the barrier: what they wrote before is visible after.
-__device__ __forceinline__ bool mbar_complete_in_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
+// The bounded wait where a CTA of the cluster arrives on the barrier that wrote what is to be seen after.
 __device__ __forceinline__ bool mbar_wait_in_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
     uint32_t ok;
