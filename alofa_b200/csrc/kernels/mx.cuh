@@ -107,8 +107,9 @@ __device__ __forceinline__ void mx_put8(const float (&v)[8], uint8_t* codes, uin
 // silu(g) * u, or (CLAMPED) the clamped form (gate_times in common.cuh), where what comes out is rounded to 8 bits: a number
 // near the border of two codes takes the other one if it is off by little, so e^-z is taken with the product z log2(e) in two
 // parts (the rounding of that product alone would cost up to |z| / 2 units in the last place).  ex2.approx is within 2 units,
-// rcp.approx within 1.  From z = -88 down it is zero.
+// rcp.approx within 1.  From z = -88 down it is zero; from 30 up it is one, infinity among them.
 __device__ __forceinline__ float mx_logistic(float z) {
+  z = fminf(z, 30.f);  // of what is not a number the factor beside this one is not either
   const float hi = fminf(-1.4426950408889634f * z, 126.f);
   const float lo = fmaf(-1.4426950408889634f, z, -hi) - 1.92596299e-8f * z;  // log2(e) is 1.92596299e-8 more than the float
   float e, r;
@@ -120,7 +121,7 @@ __device__ __forceinline__ float mx_logistic(float z) {
 template <bool CLAMPED>
 __device__ __forceinline__ float mx_gate_times(float g, float u, float alpha, float limit) {
   if (!CLAMPED) return g * mx_logistic(g) * u;
-  g = fminf(g, limit);
-  u = fminf(fmaxf(u, -limit), limit);
+  g = g > limit ? limit : g;  // not fminf: what is not a number stays so
+  u = u > limit ? limit : u < -limit ? -limit : u;
   return g * mx_logistic(alpha * g) * (u + 1.0f);
 }

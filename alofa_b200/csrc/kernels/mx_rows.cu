@@ -341,7 +341,7 @@ ALOFA_API int alofa_mx_norm(void* codes, void* scales, float* h, const float* ba
 // bfloat16.  A lane has eight channels; the loads of eight splits are in flight together.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(128) mx_merge_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const float* __restrict__ po, const float* __restrict__ pml, const int* __restrict__ positions,
-                                                       unsigned chunks, int t, int heads, int hd, int kp, int window, int split_keys) {
+                                                       unsigned chunks, int t, int heads, int hd, int kp, int splits, int window, int split_keys) {
   pdl_wait();
   pdl_launch();
   const unsigned i = blockIdx.x * blockDim.x + threadIdx.x, per_row = (unsigned)kp >> 3;
@@ -353,7 +353,8 @@ __global__ void __launch_bounds__(128) mx_merge_kernel(uint8_t* __restrict__ cod
   if (live && c < heads * hd) {
     const int head = c / hd, d = c - head * hd, p = positions[row];
     const size_t rows = (size_t)t * heads, at = (size_t)row * heads + head;
-    const int first = (window > 0 ? max(0, p - window + 1) : 0) / split_keys, last = p / split_keys;  // splits that hold keys of this token
+    // splits that hold keys of this token: none before the first position
+    const int first = (window > 0 ? max(0, p - window + 1) : 0) / split_keys, last = p < 0 ? -1 : min(p / split_keys, splits - 1);
     float m = -INFINITY, l = 0.f;
     for (int s0 = first; s0 <= last; s0 += 8) {
       float2 ml[8];
@@ -390,13 +391,13 @@ __global__ void __launch_bounds__(128) mx_merge_kernel(uint8_t* __restrict__ cod
   mx_put8(v, codes + (size_t)row * kp + c, scales + (size_t)row * (kp / MX_BLOCK) + c / MX_BLOCK, live);
 }
 
-ALOFA_API int alofa_mx_merge(void* codes, void* scales, const float* po, const float* pml, const int* positions, int t, int heads, int hd, int window, int split_keys, void* stream) {
-  if (t < 0 || heads <= 0 || hd <= 0 || hd % 8 || heads > (1 << 30) / hd || window < 0 || split_keys <= 0 || !aligned(codes, 16) || !aligned(po, 16) || !aligned(pml, 8)) return ALOFA_ERR_ARGUMENT;
+ALOFA_API int alofa_mx_merge(void* codes, void* scales, const float* po, const float* pml, const int* positions, int t, int heads, int hd, int splits, int window, int split_keys, void* stream) {
+  if (t < 0 || heads <= 0 || hd <= 0 || hd % 8 || heads > (1 << 30) / hd || splits < 0 || window < 0 || split_keys <= 0 || !aligned(codes, 16) || !aligned(po, 16) || !aligned(pml, 8)) return ALOFA_ERR_ARGUMENT;
   if (t == 0) return ALOFA_OK;
   const int kp = padded(heads * hd);
   const long long chunks = (long long)t * (kp / 8);
   if (chunks > 0x7fffffffll) return ALOFA_ERR_ARGUMENT;
-  launch_dep(mx_merge_kernel, (unsigned)((chunks + 127) / 128), 128, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, po, pml, positions, (unsigned)chunks, t, heads, hd, kp, window, split_keys);
+  launch_dep(mx_merge_kernel, (unsigned)((chunks + 127) / 128), 128, 0, (cudaStream_t)stream, (uint8_t*)codes, (uint8_t*)scales, po, pml, positions, (unsigned)chunks, t, heads, hd, kp, splits, window, split_keys);
   return launch_status();
 }
 

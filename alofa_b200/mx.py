@@ -33,6 +33,7 @@ from .errors import AlofaError
 
 BLOCK, GROUP, TILE_ROWS, TILE_BYTES, GATE_ROWS = 32, 128, 128, 8704, 16  # as in kernels/mx.cuh
 MOST_WIDTH = 32768  # numbers of a row that the norm takes
+MOST_TILES = 65535  # of tokens that the product for a few of them takes
 
 _BF16, _F32, _U8, _I32 = torch.bfloat16, torch.float32, torch.uint8, torch.int32
 
@@ -278,7 +279,8 @@ def merge_rows(partial_o, partial_ml, positions, heads: int, window: int, split_
     heads, 2]``: each split's maximum, in log2 units, and sum; float32), joined,
     as rows ``[T, heads * head_dim]`` in 8 bits.  ``positions [T]`` (int32): a
     token's splits of ``split_keys`` keys are those that hold keys up to its
-    position, and (``window`` > 0) of its last ``window`` keys."""
+    position, and (``window`` > 0) of its last ``window`` keys.  A head that saw
+    nothing is not a number."""
     here = _here()
     if not isinstance(partial_o, torch.Tensor) or partial_o.dim() != 3 or heads <= 0 or partial_o.shape[1] % heads or not partial_o.shape[2] or partial_o.shape[2] % 8 or window < 0 or split_keys <= 0:
         raise AlofaError("invalid_argument", "splits of heads of a multiple of 8 channels", f"partial_o={tuple(getattr(partial_o, 'shape', ()))} heads={heads} window={window} split_keys={split_keys}")
@@ -286,7 +288,7 @@ def merge_rows(partial_o, partial_ml, positions, heads: int, window: int, split_
     t = n // heads
     o_at, ml_at, p_at = _at(partial_o, "partial_o", _F32, (splits, n, hd), here), _at(partial_ml, "partial_ml", _F32, (splits, n, 2), here), _at(positions, "positions", _I32, (t,), here)
     rows = MxRows._empty(t, heads * hd, here, buf)
-    rc = _lib.alofa_mx_merge(rows.codes_at, rows.scales_at, o_at, ml_at, p_at, t, heads, hd, window, split_keys, _stream(here))
+    rc = _lib.alofa_mx_merge(rows.codes_at, rows.scales_at, o_at, ml_at, p_at, t, heads, hd, splits, window, split_keys, _stream(here))
     ops.mx_launched(rc, 1 if t else 0, "merge_rows", lambda: f"tokens={t} heads={heads} head_dim={hd} splits={splits}")
     return rows
 
@@ -351,7 +353,7 @@ def plan(tokens: int, rows: int, depth: int, gated: bool = False) -> tuple:
     if found is None:
         slices, sms = padded(depth) // GROUP, _sms(_here())
         tiles = (16,) if tokens <= 16 else (32,) if tokens <= 32 else (32, 64) if tokens <= 64 else (32, 64, 128) if tokens <= 96 else (64, 128)
-        ways = [(_few_us(tokens, rows, slices, gated, bn, parts, sms), bn, parts) for bn in tiles for parts in (1, 2, 3, 4, 6, 8) if parts <= slices]
+        ways = [(_few_us(tokens, rows, slices, gated, bn, parts, sms), bn, parts) for bn in tiles if tokens <= MOST_TILES * bn for parts in (1, 2, 3, 4, 6, 8) if parts <= slices]
         if tokens > 64:
             ways.append((_pair_us(tokens, rows, slices, sms), 256, 1))
         if len(_plans) >= 4096:
@@ -364,7 +366,7 @@ def _product(x: MxRows, w: MxWeight, out_at, scales_at, bias_at, add_at, feature
     if not x.rows:
         return
     bn, parts = how or plan(x.rows, w.rows, w.k, w.gated)
-    status_at = 0 if status is None else _at(status, "status", _I32, status.shape, here)
+    status_at = 0 if status is None else _at(status, "status", _I32, getattr(status, "shape", ()), here)
     call = _CALL(out_at, scales_at, x.codes_at, x.scales_at, w.at, w.maps_at, bias_at, add_at, status_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16)
     rc = _lib.alofa_mx_gemm(call, _stream(here))
     ops.mx_launched(rc, 1, what, lambda: f"tokens={x.rows} rows={w.rows} depth={w.k} how={(bn, parts)}")
@@ -387,8 +389,8 @@ def linear(x, w: MxWeight, bias=None, add=None, out=None, dtype=None, buf=None, 
         out_at, out_bf16 = out.data_ptr(), dtype is _BF16
     else:
         out_at, rows, columns, out_bf16 = _matrix(out, "out", here)
-        if rows != t or columns != n:
-            _refuse(out, "out", f"({t}, {n})", here)
+        if rows != t or columns != n or (dtype is not None and out.dtype is not dtype):
+            _refuse(out, "out", f"{dtype or out.dtype} ({t}, {n})", here)
     bias_at = 0 if bias is None else _at(bias, "bias", _F32, (n,), here)
     add_at = 0 if add is None else _at(add, "add", _F32, (t, n), here)
     _product(x, w, out_at, 0, bias_at, add_at, 0, ops.SILU_GATE, out_bf16, status, how, here, "linear")
@@ -397,9 +399,11 @@ def linear(x, w: MxWeight, bias=None, add=None, out=None, dtype=None, buf=None, 
 
 def gated_linear(x, w: MxWeight, gate=ops.SILU_GATE, buf=None, status=None, how: Optional[tuple] = None) -> MxRows:
     """``silu(x Wg^T) * (x Wu^T)`` as rows in 8 bits; ``gate`` = (alpha,
-    limit): the clamped form ``g = min(g, limit), u = clamp(u, -limit, limit):
+    limit), both over 0: the clamped form ``g = min(g, limit), u = clamp(u, -limit, limit):
     g sigmoid(alpha g) (u + 1)``."""
     here = _here()
+    if gate is not ops.SILU_GATE and gate != ops.SILU_GATE and not (gate[0] > 0 and gate[1] > 0):
+        raise AlofaError("invalid_argument", "a clamped gate's alpha and limit are over 0", f"gate={gate}")
     x = _operands(x, w, "gated_linear", True, here, buf)
     features = w.n // 2
     rows = MxRows._empty(x.rows, features, here, buf)

@@ -179,6 +179,13 @@ def test_merged_splits(t, heads, hd, splits, split_keys, window):
             want[i, h * hd : (h + 1) * hd] = sum(a * o[s, r].double().numpy() for a, s in zip(w, seen)) / low if seen else np.nan
     got = host(rows.dequantize(F32)).astype(np.float64)
     bad = np.isnan(want)
+    # positions behind the splits see all of them, negative ones nothing
+    ml = torch.stack([m, l], -1).cuda()
+    ends = mx.merge_rows(o.cuda(), ml, torch.full((t,), splits * split_keys - 1, dtype=torch.int32, device="cuda"), heads, 0, split_keys)
+    beyond = mx.merge_rows(o.cuda(), ml, torch.full((t,), 2**31 - 1, dtype=torch.int32, device="cuda"), heads, 0, split_keys)
+    assert torch.equal(beyond.codes, ends.codes) and torch.equal(beyond.scales, ends.scales)
+    nothing = mx.merge_rows(o.cuda(), ml, torch.full((t,), -1, dtype=torch.int32, device="cuda"), heads, 0, split_keys)
+    assert torch.isnan(nothing.dequantize(F32)).all()
     if bad.any():  # a head that saw nothing: not a number, and its blocks
         assert np.isnan(got[bad]).all()
     keep = ~np.isnan(got)
@@ -346,6 +353,36 @@ def test_gated_linear(t, f, k, how, gate):
     assert (scales >= plain.scale_bytes(np.maximum(sizes - room, 0).max(-1), False)).all() and (scales <= plain.scale_bytes((sizes + room).max(-1), False)).all()
 
 
+@pytest.mark.parametrize("t,how", [(5, None), (40, None), (300, None), (5, (256, 1))])
+@pytest.mark.parametrize("gate", [ops.SILU_GATE, (1.702, 7.0)])
+def test_gated_rows_of_nan(t, how, gate):
+    """Sums that are not numbers are none behind either gate, in their row only."""
+    xr, wp, xv, wv = product_operands(t, 2 * 70, 300, 41, gated=True)
+    xr.scales[2, 1] = 255
+    got = host(mx.gated_linear(xr, wp, gate, how=how).dequantize(F32))
+    assert np.isnan(got[2]).all() and np.isfinite(np.delete(got, 2, 0)).all()
+
+
+def test_a_gate_near_the_largest_number():
+    """silu(g) u of g = 1.75 2^127 (g log2(e) is beyond 32 bits) and u = 0.875: 1.53125 2^127, as a code 1.5 2^127."""
+    x, w = torch.zeros(1, 32), torch.zeros(2, 32)
+    x[0, 0], w[0, 0], w[1, 0] = 1.75 * 2.0**63, 2.0**64, 2.0**-64
+    wp = mx.pack_weight(w.cuda(), True)
+    for how in (None, (256, 1)):
+        assert mx.gated_linear(x.cuda(), wp, how=how).dequantize(F32).item() == 1.5 * 2.0**127
+
+
+def test_more_tokens_than_tiles_of_a_few():
+    """So many tokens that the kernel for a few of them has no grid: they go by pairs."""
+    t = 64 * mx.MOST_TILES + 3
+    x = torch.zeros(t, 128, dtype=BF16, device="cuda")
+    x[-1], x[-2] = 1, 2
+    w = numbers(8, 128, 42)
+    got, want = mx.linear(x, mx.pack_weight(w.cuda()), dtype=F32), plain.values(w.double().numpy(), True).sum(1)
+    bound = 128 * 2.0**-23 * np.abs(plain.values(w.double().numpy(), True)).sum(1)
+    assert (np.abs(host(got[-1]) - want) <= bound).all() and (np.abs(host(got[-2]) - 2 * want) <= 2 * bound).all() and not got[:-2].any()
+
+
 # ---- as a program uses them ------------------------------------------------------------------------------------------
 
 
@@ -481,6 +518,10 @@ def test_refusals():
     refused("invalid_argument", mx.linear, rows, w, add=torch.zeros(4, 65, device="cuda"))
     refused("invalid_argument", mx.linear, rows, w, out=torch.zeros(5, 64, device="cuda"))
     refused("unsupported", mx.linear, rows, w, dtype=torch.float16)
+    refused("invalid_argument", mx.linear, rows, w, out=torch.zeros(4, 64, device="cuda"), dtype=BF16)
+    refused("invalid_argument", mx.linear, rows, w, status=1)
+    refused("invalid_argument", mx.gated_linear, rows, wg, (0.0, 7.0))
+    refused("invalid_argument", mx.gated_linear, rows, wg, (1.702, 0.0))
     refused("unsupported", mx.linear, rows, w, how=(48, 1))
     refused("unsupported", mx.linear, rows, w, how=(16, 2))  # a part without a slice
     refused("unsupported", mx.linear, rows, w, how=(256, 2))
