@@ -160,7 +160,8 @@ class MxWeight:
     """A weight ``[n, k]`` in 4 bits, laid out in tiles of 128 rows and 128
     numbers as the product reads them.  ``gated``: the first half of the rows
     are a gate's, the second an up projection's.  Made by :func:`pack_weight`
-    or :meth:`from_codes`."""
+    or :meth:`from_codes`, and constant from then on: products read it ahead of
+    the kernel before them in the stream."""
 
     __slots__ = ("tiles", "n", "k", "gated", "rows", "device", "at", "maps", "maps_at")
 
