@@ -1608,7 +1608,7 @@ def mx_library():
             "alofa_mx_rows": [_P, _P, _P, _I, _I, _I, _P],
             "alofa_mx_rows_values": [_P, _P, _P, _I, _I, _I, _P],
             "alofa_mx_norm": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _F, _P],
-            "alofa_mx_merge": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P],
+            "alofa_mx_merge": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
             "alofa_mx_pack": [_P, _P, _I, _I, _I, _I, _P],
             "alofa_mx_settle": [_P],
             "alofa_mx_weight_values": [_P, _P, _I, _I, _I, _I, _P],

@@ -1,4 +1,7 @@
 """What microscaled weights refuse, and their definition; no GPU needed."""
+import pathlib
+import re
+
 import numpy as np
 import pytest
 import torch
@@ -55,6 +58,18 @@ def test_operators_need_a_gpu():
     refused("unsupported", mx.norm_rows, x, torch.ones(128), 1e-6)
     refused("unsupported", mx.MxRows, u8, torch.zeros(2, 4, dtype=torch.uint8), 128)
     refused("unsupported", mx.MxWeight.from_codes, u8, torch.zeros(2, 8, dtype=torch.uint8), 256)
+
+
+def test_arguments_as_the_library_has_them():
+    """Every entry point is declared with as many arguments, of the same sizes, as its source has: one more would go through unconverted, an address cut to 32 bits."""
+    from alofa_b200.csrc import ops
+
+    lib, kernels = ops.mx_library(), pathlib.Path(ops.__file__).parent / "kernels"
+    found = re.findall(r"ALOFA_API int (alofa_mx_\w+)\(([^)]*)\)", "".join((kernels / name).read_text() for name in ("mx_rows.cu", "mx_gemm.cu")))
+    assert len(found) == 9
+    for name, args in found:
+        kinds = ["c_void_p" if "*" in a else {"int": "c_int", "float": "c_float", "long long": "c_long"}[a.strip().rsplit(" ", 1)[0]] for a in args.split(",")]
+        assert [{"c_longlong": "c_long"}.get(t.__name__, t.__name__) for t in getattr(lib, name).argtypes] == kinds, name
 
 
 def test_the_definition():

@@ -486,6 +486,27 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, ref) for x in g)
 
 
+def test_joined_splits_in_a_graph_on_another_stream():
+    g = torch.Generator(device="cuda").manual_seed(21)
+    po, ml = torch.randn(3, 4 * 5, 32, generator=g, device="cuda"), 1 + torch.rand(3, 4 * 5, 2, generator=g, device="cuda")
+    at = torch.tensor([5, 64, 100, 191], dtype=torch.int32, device="cuda")
+    want = mx.merge_rows(po, ml, at, 5, 0, 64)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        aside = mx.merge_rows(po, ml, at, 5, 0, 64)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = mx.merge_rows(po, ml, at, 5, 0, 64)
+    first = want.codes.clone()
+    po.mul_(2)
+    graph.replay()
+    again = mx.merge_rows(po, ml, at, 5, 0, 64)
+    assert torch.equal(aside.codes, first) and torch.equal(aside.scales, want.scales)
+    assert torch.equal(got.codes, again.codes) and torch.equal(got.scales, again.scales) and torch.equal(again.scales[:, :5], want.scales[:, :5] + 1)  # five blocks of numbers; those behind the width are zeros, scale byte 0
+
+
 def test_no_tokens():
     w, wg = mx.pack_weight(torch.randn(64, 96, device="cuda")), mx.pack_weight(torch.randn(64, 96, device="cuda"), True)
     x = mx.quantize_rows(torch.empty(0, 96, device="cuda"))
