@@ -78,10 +78,12 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sy
 
 // After a wait that ran out: what is still in flight ends in a bounded time.
 constexpr uint32_t DRAIN_LIMIT = 1u << 14;
-__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
-  for (uint32_t w = 0; w < DRAIN_LIMIT && !mbar_try_wait(bar, parity); ++w) {
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, uint32_t limit = DRAIN_LIMIT) {
+  for (uint32_t w = 0; w < limit && !mbar_try_wait(bar, parity); ++w) {
   }
 }
+// `count` arrivals at once, in the place of those who gave up before they made theirs.
+__device__ __forceinline__ void arrive_for(uint64_t* bar, uint32_t count) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory"); }
 
 // Shared memory seen as rows of 16 bytes, groups of 8 rows 128 bytes apart, no swizzle.
 __device__ __forceinline__ uint64_t scales_desc(uint32_t smem) { return (uint64_t)((smem & 0x3FFFFu) >> 4) | (8ull << 16) | (8ull << 32) | (1ull << 46); }
@@ -228,11 +230,13 @@ template <int BN>
 __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MxArgs args, const int parts) {
   using Tile = FewTile<BN>;
   constexpr int STAGES = Tile::STAGES;
+  constexpr uint32_t BY_WEIGHTS = 1, BY_TOKENS = 1 + 32;  // arrivals a slice: the weight's bytes; the tokens', and the copies of their scales
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  __shared__ uint64_t landed[STAGES], stage_free[STAGES], sums_done;
+  // asked_all: both copying warps have said in `asked` how many slices they asked for; quiet: no copy writes the ring any more
+  __shared__ uint64_t landed[STAGES], stage_free[STAGES], sums_done, asked_all, quiet;
   __shared__ uint32_t tmem_base_smem;
-  __shared__ int abort_flag;
+  __shared__ int abort_flag, asked[2];
 
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int part = blockIdx.x % parts, f_tile = blockIdx.x / parts;  // a cluster: the parts of one tile's depth
@@ -242,10 +246,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&landed[s], 1 + 1 + 32);  // the weight's bytes, the tokens', the copies of their scales
+      mbar_init(&landed[s], BY_WEIGHTS + BY_TOKENS);
       mbar_init(&stage_free[s], 1);
     }
     mbar_init(&sums_done, 1);
+    mbar_init(&asked_all, 2);
+    mbar_init(&quiet, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 5) tmem_alloc(&tmem_base_smem, Tile::TMEM_COLS);
@@ -273,6 +279,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
         load_bytes(stage + Tile::A_BYTES + Tile::B_BYTES, args.tiles + (size_t)tile * MX_TILE_BYTES + MX_TILE_CODES, MX_TILE_BYTES - MX_TILE_CODES, bar);
       }
     }
+    if (lane == 0) asked[0] = i, mbar_arrive(&asked_all);
   } else if (warp == 4) {
     pdl_wait();
     pdl_launch();
@@ -299,8 +306,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
       }
       arrive_when_landed(bar);
     }
-    if (*(volatile int*)&abort_flag)
-      for (int j = max(0, i - STAGES); j < i; ++j) drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+    if (lane == 0) asked[1] = i, mbar_arrive(&asked_all);
   } else if (warp == 5) {
     const bool chosen = elect_lane();
     const uint32_t sums = uniform(tmem);
@@ -329,7 +335,19 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
     }
     if (chosen) {
       umma_commit(&sums_done);
-      if (!ok) drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
+      if (!ok) {
+        drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
+        // and the copies asked for land before the sums take the ring's room, or another CTA this one's: the last slice in each
+        // stage, where a warp that gave up first did not ask for its part of it without that part
+        drain(&asked_all, 0);
+        const int w = *(volatile int*)&asked[0], x = *(volatile int*)&asked[1], most = max(w, x);
+        for (int j = max(0, most - STAGES); j < most; ++j) {
+          if (j >= w) arrive_for(&landed[j % STAGES], BY_WEIGHTS);
+          if (j >= x) arrive_for(&landed[j % STAGES], BY_TOKENS);
+          drain(&landed[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+        }
+      }
+      mbar_arrive(&quiet);
     }
   }
   if (warp == 4) copies_wait();  // landed long ago, unless a wait ran out
@@ -339,6 +357,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   if (warp < 4) {
     const bool good = mbar_wait(&sums_done, 0, &abort_flag) && !*(volatile int*)&abort_flag;
     tc_fence_after();
+    if (!good) drain(&quiet, 0, (STAGES + 3) * DRAIN_LIMIT);  // longer than what arrives there may take
     if (!good && threadIdx.x == 0 && args.status) atomicExch(args.status, 2);
     const uint32_t mine = tiles + (uint32_t)(warp * 32 + lane) * 4;
     for (int c = 0; c < live; c += 16) {

@@ -7,7 +7,11 @@
 
 #include "common.cuh"
 
-constexpr uint32_t WAIT_LIMIT = 1u << 24;
+// Tries of a bounded wait.  A library that is built with 0 gives up at its first wait: its kernels' way out is tested so.
+#ifndef ALOFA_WAIT_LIMIT
+#define ALOFA_WAIT_LIMIT (1u << 24)
+#endif
+constexpr uint32_t WAIT_LIMIT = ALOFA_WAIT_LIMIT;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
