@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 import torch
 
@@ -170,27 +171,33 @@ def _elementwise():
     return lib
 
 
-_bound_stream = None  # the stream handle of the step in progress, looked up once per step
+class _Bound(threading.local):
+    """The stream handle of the step that this thread is in, looked up once per step."""
+
+    stream = None
+
+
+_bound = _Bound()
 
 
 def _stream() -> int:
-    return _bound_stream if _bound_stream is not None else torch.cuda.current_stream().cuda_stream
+    stream = _bound.stream
+    return stream if stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 class bound_stream:
-    """Within the block, every launch of this module goes to the stream that is
-    current on entry, without asking torch for it at each launch (the lookup
-    costs as much as a launch).  The caller must not switch streams inside."""
+    """Within the block, every launch of this module by this thread goes to the
+    stream that is current on entry, without asking torch for it at each launch
+    (the lookup costs as much as a launch).  The caller must not switch streams
+    inside.  Other threads' launches go where theirs do."""
 
     def __enter__(self):
-        global _bound_stream
-        self._before = _bound_stream
-        _bound_stream = torch.cuda.current_stream().cuda_stream
+        self._before = _bound.stream
+        _bound.stream = torch.cuda.current_stream().cuda_stream
         return self
 
     def __exit__(self, *exc):
-        global _bound_stream
-        _bound_stream = self._before
+        _bound.stream = self._before
         return False
 
 
@@ -1632,5 +1639,6 @@ def mx_launched(rc: int, launches: int, what: str, detail) -> None:
 
 
 def current_stream_handle(device: int) -> int:
-    """The handle of the device's current stream (the step's, inside a step), without the object around it that takes longer to make than a launch."""
-    return _bound_stream if _bound_stream is not None else torch._C._cuda_getCurrentRawStream(device)
+    """The handle of the device's current stream (the step's, inside a step of this thread), without the object around it that takes longer to make than a launch."""
+    stream = _bound.stream
+    return stream if stream is not None else torch._C._cuda_getCurrentRawStream(device)
