@@ -12,8 +12,8 @@ from ..config.registry import get_architecture, read_model_config
 from ..errors import AlofaError
 from ..parts.base import Runtime
 from ..parts.model import Model
-from ..weights.loader import load_state
-from ..weights.random_init import random_state
+from ..weights.loader import open_weights
+from ..weights.random_init import random_weights
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}
 
@@ -44,8 +44,8 @@ def load_model(folder, dtype="bfloat16", device=None, weight_format=None):
     arch, cfg = read_model_config(folder)
     spec = arch.build_spec(cfg)
     model = Model(spec, Runtime(dev, compute_dtype(dtype), weight_format))
-    state = load_state(model.tensors(), folder, model.rt.dtype, dev)
-    model.load(state)
+    with open_weights(model.tensors(), folder, model.rt.dtype, dev) as weights:
+        model.load(weights)
     return model, cfg, arch
 
 
@@ -57,6 +57,7 @@ def random_model(architecture: str, config, seed: int, dtype="bfloat16", device=
     arch = get_architecture(architecture)
     spec = arch.build_spec(config)
     model = Model(spec, Runtime(dev, compute_dtype(dtype), weight_format))
-    state = random_state(model.tensors(), seed, torch.bfloat16, dev if generate_on_device else "cpu")
-    model.load(load_state(model.tensors(), state, model.rt.dtype, dev))
+    drawn = random_weights(model.tensors(), seed, torch.bfloat16, dev if generate_on_device else "cpu")
+    with open_weights(model.tensors(), drawn, model.rt.dtype, dev) as weights:
+        model.load(weights)
     return model, config, arch

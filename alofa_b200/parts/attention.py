@@ -20,7 +20,7 @@ import torch
 from ..csrc import ops
 from ..errors import AlofaError
 from . import fast_linear
-from .base import PagedKV, Part, TensorSpec, as_float32_vector, build_part, register_part
+from .base import PagedKV, Part, TensorSpec, as_float32_vector, build_part, register_part, stacked
 from .linear import RESIDUAL, STORE, MergedSplits, add_into_stream
 from .mx_linear import make_linear
 
@@ -201,7 +201,7 @@ class GQAttention(PagedAttend, Part):
 
     def load(self, state):
         pre = self.prefix
-        w = torch.cat([state[pre + f"{n}_proj.weight"] for n in "qkv"], dim=0)
+        w = stacked(state, [pre + f"{n}_proj.weight" for n in "qkv"], self.q_dim + 2 * self.kv_dim)
         b = None
         if self.qkv_bias:
             b = as_float32_vector(torch.cat([state[pre + f"{n}_proj.bias"] for n in "qkv"], dim=0))
@@ -209,6 +209,7 @@ class GQAttention(PagedAttend, Part):
         # a run of this layer that reads another run's cache needs q only
         q_weight = self.qkv.weight.first_rows(self.q_dim) if self.rt.weight_format is not None else w[: self.q_dim]
         self.q_only = make_linear(self.rt, q_weight, b[: self.q_dim] if b is not None else None, STORE)
+        del w, q_weight  # where the products hold a form of their own, before the next weight is made
         ob = as_float32_vector(state[pre + "o_proj.bias"]) if self.out_bias else None
         self.out = make_linear(self.rt, state[pre + "o_proj.weight"], ob, RESIDUAL)
         self.position.load(state)

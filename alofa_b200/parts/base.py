@@ -141,6 +141,23 @@ def build_part(family: str, spec: PartSpec, rt: Runtime):
     return kinds[spec.kind](spec, rt)
 
 
+def stacked(state, names, rows: int) -> torch.Tensor:
+    """The matrices of these names above one another, ``rows`` in all, taken
+    one after another: where ``state`` makes a tensor when it is asked for, no
+    more than one of them is there beside the result."""
+    out, at = None, 0
+    for name in names:
+        t = state[name]
+        if out is None:
+            out = t.new_empty((rows, *t.shape[1:]))
+        elif out.dtype != t.dtype:
+            out = out.to(torch.promote_types(out.dtype, t.dtype))
+        out[at : at + t.shape[0]].copy_(t)
+        at += t.shape[0]
+        del t  # before the next one is made
+    return out
+
+
 def as_float32_vector(t: torch.Tensor) -> torch.Tensor:
     """Norm weights and biases are handed to the kernels in fp32 (widening
     bf16 is exact)."""

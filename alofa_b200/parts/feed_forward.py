@@ -10,7 +10,7 @@ import torch
 from ..csrc import ops
 from ..errors import AlofaError
 from . import fast_linear
-from .base import Part, TensorSpec, as_float32_vector, register_part
+from .base import Part, TensorSpec, as_float32_vector, register_part, stacked
 from .linear import GATED, RESIDUAL, STORE, Linear, add_into_stream
 from .mx_linear import make_linear
 
@@ -38,7 +38,7 @@ class GatedMLP(Part):
 
     def load(self, state):
         pre = self.prefix
-        self.gate_up = make_linear(self.rt, torch.cat([state[pre + "gate_proj.weight"], state[pre + "up_proj.weight"]], dim=0), None, GATED)
+        self.gate_up = make_linear(self.rt, stacked(state, (pre + "gate_proj.weight", pre + "up_proj.weight"), 2 * self.inter), None, GATED)
         self.down = make_linear(self.rt, state[pre + "down_proj.weight"], None, RESIDUAL)
 
     def scratch_row_bytes(self) -> int:

@@ -68,8 +68,10 @@ class Model:
             out.update(part.tensors())
         return out
 
-    def load(self, state: dict) -> None:
-        state = dict(state)
+    def load(self, state) -> None:
+        """``state``: name -> device tensor, a dict or :class:`~alofa_b200.weights.loader.Weights`, which has each made when its part asks."""
+        if isinstance(state, dict):
+            state = dict(state)  # parts leave tables in it for one another
         self.loads += 1
         for part in self.parts():
             part.load(state)

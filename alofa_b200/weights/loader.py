@@ -22,9 +22,15 @@ that two shards hold.
 
 To the device: the files are memory-mapped; each tensor goes through two
 pinned staging buffers in turn (the copy of one chunk to the device runs while
-the next chunk is read from the mapping) into device memory of its own."""
+the next chunk is read from the mapping) into device memory of its own.  A
+tensor is copied when a part asks for it (:func:`open_weights`), and is gone
+again when the part has made its own form of it: on the device there is never
+more beside the parts' own weights than the part that is loading takes."""
 from __future__ import annotations
 
+import weakref
+from collections.abc import MutableMapping
+from contextlib import contextmanager
 from pathlib import Path
 
 import torch
@@ -151,13 +157,56 @@ def open_checkpoint(folder) -> tuple:
     return list(files.values()), where, problems
 
 
-def load_state(expected: dict, source, compute_dtype: torch.dtype, device) -> dict:
-    """name -> device tensor.  ``source`` is a model folder or a dict of
-    CPU/GPU tensors (the in-memory random mode)."""
-    if isinstance(source, dict):
-        found = {n: tuple(t.shape) for n, t in source.items()}
+class Weights(MutableMapping):
+    """name -> tensor, made when it is asked for.  ``shapes``: the names that
+    there are, with their shapes; ``fetch(name)`` makes a tensor.  One that is
+    still in use is given again, one that nobody holds any more is made anew.
+    What is set (tables that parts share) is kept."""
+
+    def __init__(self, shapes: dict, fetch):
+        self.shapes, self._fetch = dict(shapes), fetch
+        self._in_use, self._kept = weakref.WeakValueDictionary(), {}
+
+    def __getitem__(self, name):
+        if name in self._kept:
+            return self._kept[name]
+        if name not in self.shapes:
+            raise KeyError(name)
+        t = self._in_use.get(name)
+        if t is None:
+            t = self._in_use[name] = self._fetch(name)
+        return t
+
+    def __setitem__(self, name, value):
+        self._kept[name] = value
+
+    def __delitem__(self, name):
+        if name not in self:
+            raise KeyError(name)
+        self._kept.pop(name, None)
+        self.shapes.pop(name, None)
+
+    def __contains__(self, name):
+        return name in self._kept or name in self.shapes
+
+    def __iter__(self):
+        yield from self.shapes
+        yield from (n for n in self._kept if n not in self.shapes)
+
+    def __len__(self):
+        return len(self.shapes) + sum(n not in self.shapes for n in self._kept)
+
+
+@contextmanager
+def open_weights(expected: dict, source, compute_dtype: torch.dtype, device):
+    """The :class:`Weights` of a model folder, or of a mapping of CPU/GPU
+    tensors (the in-memory random mode), on the device; compared with what the
+    model expects before any is read.  Open while tensors are asked for."""
+    if not isinstance(source, (str, Path)):
+        found = source.shapes if isinstance(source, Weights) else {n: tuple(t.shape) for n, t in source.items()}
         check_names_and_shapes(expected, found, "in-memory state")
-        return {n: _place(t, compute_dtype, device) for n, t in source.items()}
+        yield Weights(found, lambda n: _place(source[n], compute_dtype, device))
+        return
     files, where, problems = open_checkpoint(source)
     try:
         found = {n: st.entries[n].shape for n, st in where.items()}
@@ -169,18 +218,25 @@ def load_state(expected: dict, source, compute_dtype: torch.dtype, device) -> di
             raise
         if problems:
             raise AlofaError("invalid_argument", "weights do not match the model", f"shard index ({len(problems)}): " + "; ".join(problems) + f" | source={source}")
-        on_gpu = torch.device(device).type == "cuda"
-        staging = _Staging(device) if on_gpu else None
-        out = {}
         for n, st in where.items():
-            t = st.tensor(n)
-            if on_gpu:
-                out[n] = _place(staging.to_device(t), compute_dtype, device)
-            else:
-                out[n] = _place(t, compute_dtype, device).clone()
-        if staging is not None:
-            staging.finish()
-        return out
+            st.check_supported(n)
+        staging = _Staging(device) if torch.device(device).type == "cuda" else None
+
+        def fetch(n):
+            t = where[n].tensor(n)
+            return _place(t, compute_dtype, device).clone() if staging is None else _place(staging.to_device(t), compute_dtype, device)
+
+        try:
+            yield Weights(found, fetch)
+        finally:
+            if staging is not None:
+                staging.finish()
     finally:
         for st in files:
             st.close()
+
+
+def load_state(expected: dict, source, compute_dtype: torch.dtype, device) -> dict:
+    """name -> device tensor, all of them; ``source`` as in :func:`open_weights`."""
+    with open_weights(expected, source, compute_dtype, device) as weights:
+        return dict(weights)

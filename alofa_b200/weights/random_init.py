@@ -15,6 +15,7 @@ import torch
 
 from ..config.registry import get_architecture
 from ..errors import AlofaError
+from .loader import Weights
 from .safetensors_io import write_safetensors
 
 
@@ -41,12 +42,14 @@ def random_tensor(seed: int, name: str, shape, init: str, dtype, device="cpu") -
 def random_state(model_tensors: dict, seed: int, dtype=torch.bfloat16, device="cpu") -> dict:
     """``model_tensors``: name -> TensorSpec (see parts.base).  Optional
     tensors are not made."""
-    out = {}
-    for name, spec in model_tensors.items():
-        if spec.optional:
-            continue
-        out[name] = random_tensor(seed, name, spec.shape, spec.init, dtype, device)
-    return out
+    return dict(random_weights(model_tensors, seed, dtype, device))
+
+
+def random_weights(model_tensors: dict, seed: int, dtype=torch.bfloat16, device="cpu") -> Weights:
+    """The same, each tensor drawn when it is asked for."""
+    made = {name: spec for name, spec in model_tensors.items() if not spec.optional}
+    shapes = {name: tuple(abs(d) for d in spec.shape) for name, spec in made.items()}
+    return Weights(shapes, lambda name: random_tensor(seed, name, made[name].shape, made[name].init, dtype, device))
 
 
 def write_random_model(folder, architecture: str, config, seed: int, dtype=torch.bfloat16) -> Path:

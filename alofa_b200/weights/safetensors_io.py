@@ -84,13 +84,16 @@ class SafeTensorFile:
     def names(self):
         return list(self.entries)
 
-    def tensor(self, name: str) -> torch.Tensor:
-        """A CPU tensor viewing the mapped bytes (read-only; copy before writing)."""
+    def check_supported(self, name: str) -> None:
         if name not in self.entries:
             raise AlofaError("invalid_argument", "entry is not in the file", f"name={name} file={self.path}")
-        e = self.entries[name]
-        if e.dtype == "F16":
+        if self.entries[name].dtype == "F16":
             raise AlofaError("unsupported", "float16 tensors are not supported", f"name={name} file={self.path}")
+
+    def tensor(self, name: str) -> torch.Tensor:
+        """A CPU tensor viewing the mapped bytes (read-only; copy before writing)."""
+        self.check_supported(name)
+        e = self.entries[name]
         dtype, width = _DTYPES[e.dtype]
         count = (e.end - e.begin) // width
         if count == 0:
