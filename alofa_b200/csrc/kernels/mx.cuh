@@ -107,21 +107,38 @@ __device__ __forceinline__ void mx_put8(const float (&v)[8], uint8_t* codes, uin
 // silu(g) * u, or (CLAMPED) the clamped form (gate_times in common.cuh), where what comes out is rounded to 8 bits: a number
 // near the border of two codes takes the other one if it is off by little, so e^-z is taken with the product z log2(e) in two
 // parts (the rounding of that product alone would cost up to |z| / 2 units in the last place).  ex2.approx is within 2 units,
-// rcp.approx within 1.  From z = -88 down it is zero; from 30 up it is one, infinity among them.
-__device__ __forceinline__ float mx_logistic(float z) {
-  z = fminf(z, 30.f);  // of what is not a number the factor beside this one is not either
-  const float hi = fminf(-1.4426950408889634f * z, 126.f);
-  const float lo = fmaf(-1.4426950408889634f, z, -hi) - 1.92596299e-8f * z;  // log2(e) is 1.92596299e-8 more than the float
-  float e, r;
+// rcp.approx within 1.  The logistic function is one from z = 30 up, infinity among them; from z = MX_GATE_FAR down, where e^-z and
+// then its reciprocal leave the normal numbers, it is e^z to 2^-125 of itself, and its two halves e^(z/2) go to one factor each:
+// g e^z alone would be zero, or a subnormal number of a few bits, beside a u that makes it large.
+constexpr float MX_GATE_FAR = -87.f;
+// 2^(c z) for c next to log2(e) or half of it: `rest` is what c as a float leaves out of it.
+__device__ __forceinline__ float mx_power_of(float z, float c, float rest) {
+  const float hi = c * z, lo = fmaf(c, z, -hi) + rest * z;
+  float e;
   asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(hi));
-  e = fmaf(e, 0.6931471805599453f * lo, e);
+  return fmaf(e, 0.6931471805599453f * lo, e);
+}
+__device__ __forceinline__ float mx_logistic(float z) {  // z above MX_GATE_FAR, or not a number
+  z = fminf(z, 30.f);  // of what is not a number the factor beside this one is not either
+  const float e = mx_power_of(z, -1.4426950408889634f, -1.92596299e-8f);  // log2(e) is 1.92596299e-8 more than the float
+  float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return r;
 }
-template <bool CLAMPED>
+// FAR: gates below MX_GATE_FAR may be among them.
+template <bool CLAMPED, bool FAR>
 __device__ __forceinline__ float mx_gate_times(float g, float u, float alpha, float limit) {
-  if (!CLAMPED) return g * mx_logistic(g) * u;
-  g = g > limit ? limit : g;  // not fminf: what is not a number stays so
-  u = u > limit ? limit : u < -limit ? -limit : u;
-  return g * mx_logistic(alpha * g) * (u + 1.0f);
+  if (CLAMPED) {
+    g = g > limit ? limit : g;  // not fminf: what is not a number stays so
+    u = (u > limit ? limit : u < -limit ? -limit : u) + 1.0f;
+  }
+  const float z = CLAMPED ? alpha * g : g;
+  if (FAR && z < MX_GATE_FAR) {
+    const float half = mx_power_of(fmaxf(z, -1000.f), 0.7213475204444817f, 9.62981495e-9f);  // from -1,000 down it is zero, infinity among them
+    return (g * half) * (u * half);
+  }
+  return g * mx_logistic(z) * u;
 }
+// Whether of several gates the least is so far below zero.
+template <bool CLAMPED>
+__device__ __forceinline__ bool mx_gate_far(float least, float alpha) { return (CLAMPED ? alpha * least : least) < MX_GATE_FAR; }

@@ -169,14 +169,20 @@ struct FewTile {
 template <bool CLAMPED>
 __device__ __forceinline__ void few_gated_token(const MxArgs& args, float4 v, int t, int f0, int lane) {
   const int f = f0 + (lane >> 3) * 16 + (lane & 3) * 4;  // lanes with bit 2 clear have the gate's rows, those with it set the up projection's
-  float g[4] = {v.x, v.y, v.z, v.w};
+  float g[4] = {v.x, v.y, v.z, v.w}, u[4];
   uint32_t largest = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float u = __shfl_xor_sync(0xffffffffu, g[j], 4);
-    const float y = CLAMPED ? mx_gate_times<true>(g[j], u, args.gate_alpha, args.gate_limit) : mx_gate_times<false>(g[j], u, 0.f, 0.f);
-    g[j] = f + j < args.F ? y : 0.f;
+  for (int j = 0; j < 4; ++j) u[j] = __shfl_xor_sync(0xffffffffu, g[j], 4);
+  // told apart once for the four: for every number it took 64 tokens of 8,960 features 12.2 us instead of 11.1
+  if (!mx_gate_far<CLAMPED>(fminf(fminf(g[0], g[1]), fminf(g[2], g[3])), args.gate_alpha)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = mx_gate_times<CLAMPED, false>(g[j], u[j], args.gate_alpha, args.gate_limit);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = mx_gate_times<CLAMPED, true>(g[j], u[j], args.gate_alpha, args.gate_limit);
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) g[j] = f + j < args.F ? g[j] : 0.f;
   if ((lane & 4) == 0)
 #pragma unroll
     for (int j = 0; j < 4; ++j) largest = max(largest, mx_size(g[j]));
@@ -453,17 +459,27 @@ __device__ __forceinline__ void pair_load64(uint32_t tmem, uint32_t (&r)[64]) {
   tmem_ld_wait();
 }
 
-// 64 rows' sums of one token of a gated weight: one block of codes and its scale.  The clamped form and the last
-// features' zeros are told apart once, not for every number: this is what the tensor cores wait for when the depth is short.
+// 64 rows' sums of one token of a gated weight: one block of codes and its scale.  The clamped form, gates far below zero and the
+// last features' zeros are told apart once, not for every number: this is what the tensor cores wait for when the depth is short.
 template <bool CLAMPED>
 __device__ __forceinline__ void pair_gated64(const MxArgs& args, const uint32_t (&r)[64], int t, int row, bool good) {
   const int f = row / 2, fp = (args.F + MX_GROUP - 1) / MX_GROUP * MX_GROUP;
   if (f >= fp) return;
-  float v[32];
+  float v[32], least = 0.f;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const int at = (j / 16) * 32 + j % 16;
-    v[j] = mx_gate_times<CLAMPED>(__uint_as_float(r[at]), __uint_as_float(r[at + 16]), args.gate_alpha, args.gate_limit);
+  for (int j = 0; j < 32; ++j) least = fminf(least, __uint_as_float(r[(j / 16) * 32 + j % 16]));
+  if (!mx_gate_far<CLAMPED>(least, args.gate_alpha)) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const int at = (j / 16) * 32 + j % 16;
+      v[j] = mx_gate_times<CLAMPED, false>(__uint_as_float(r[at]), __uint_as_float(r[at + 16]), args.gate_alpha, args.gate_limit);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const int at = (j / 16) * 32 + j % 16;
+      v[j] = mx_gate_times<CLAMPED, true>(__uint_as_float(r[at]), __uint_as_float(r[at + 16]), args.gate_alpha, args.gate_limit);
+    }
   }
   if (f + 32 > args.F) {
 #pragma unroll

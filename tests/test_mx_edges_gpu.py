@@ -48,3 +48,36 @@ def test_a_gated_product_that_gives_up(no_patience):
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     rows = mx.gated_linear(xr, wp, how=(32, 3), status=status)
     assert torch.isnan(rows.dequantize(F32)).all() and int(status) == 2
+
+
+# ---- the gate far below zero ---------------------------------------------------------------------------------------------
+
+#: gates as sums of numbers that weights in 4 bits have, and how large the factors beside them are
+FAR = [([64, 16, 6, q], 120) for q in (0, 0.5, 1, 1.5, 2, 3)] + [([64, 16, 8, q], 122) for q in (0, 0.5, 1, 1.5, 2, 3)] + [([64, 16, 12, 0], 125), ([64, 32, 4, 0], 125), ([64, 48, 8, 0], 126), ([128, 16, 6, 0], 126), ([128, 48, 0, 0], 126),
+      ([64, 16, 6, 0.5], 0), ([64, 24, 1, 0], 30), ([64, 16, 1, 0], 100), ([2**20, 0, 0, 0], 126), ([2**100, 0, 0, 0], 126)]
+
+
+@pytest.mark.parametrize("how", [None, (256, 1)])
+@pytest.mark.parametrize("t", [1, 5, 300])
+@pytest.mark.parametrize("gate", [None, (1.0, 2.0**127), (2.0, 2.0**127)])
+def test_a_gate_far_below_zero(gate, t, how):
+    """silu(g) u where the logistic function is next to the smallest numbers of 32 bits and below them, and u is large: each
+    feature alone in its block, so that its own size decides its scale.  Sums here are exact, so what is rounded is off by
+    ROWS_SLACK of itself (the exponential, by two factors of at most 4 units each) where it is a normal number."""
+    w = torch.zeros(2 * 32 * len(FAR), 160)
+    g, u = np.zeros(32 * len(FAR)), np.zeros(32 * len(FAR))
+    for i, (parts, power) in enumerate(FAR):
+        w[32 * i, 0:128:32] = -torch.tensor(parts, dtype=F32)
+        w[32 * len(FAR) + 32 * i, 128] = -1.5 * 2.0**power
+        g[32 * i], u[32 * i] = -float(sum(parts)), -1.5 * 2.0**power
+    x = torch.zeros(t, 160)
+    x[:, ::32] = 1
+    rows = mx.gated_linear(x.cuda(), mx.pack_weight(w.cuda(), True), *([] if gate is None else [gate]), how=how)
+    alpha = 1.0 if gate is None else gate[0]
+    with np.errstate(over="ignore"):
+        want = g / (1 + np.exp(-alpha * g)) * (u if gate is None else np.maximum(u, -(2.0**127)) + 1)
+    got, scales = host(rows.dequantize(F32)).astype(np.float64), host(rows.scales).astype(np.float64)
+    unit = np.exp2(scales - 127).repeat(32, -1)[:, : len(g)]
+    step = unit * np.exp2(np.maximum(np.frexp(np.maximum(np.abs(got), np.abs(want)) / unit)[1] - 1, -6) - 3.0)
+    off = np.abs(got - want) - step / 2 - 2.0**-18 * np.abs(want)
+    assert (off <= 0).all(), [(float(g[32 * i]), got[0, 32 * i], want[32 * i]) for i in range(len(FAR)) if (off[:, 32 * i] > 0).any()]
