@@ -174,7 +174,7 @@ __device__ __forceinline__ void few_gated_token(const MxArgs& args, float4 v, in
 #pragma unroll
   for (int j = 0; j < 4; ++j) u[j] = __shfl_xor_sync(0xffffffffu, g[j], 4);
   // told apart once for the four: for every number it took 64 tokens of 8,960 features 12.2 us instead of 11.1
-  if (!mx_gate_far<CLAMPED>(fminf(fminf(g[0], g[1]), fminf(g[2], g[3])), args.gate_alpha)) {
+  if (__builtin_expect(!mx_gate_far<CLAMPED>(fminf(fminf(g[0], g[1]), fminf(g[2], g[3])), args.gate_alpha), 1)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] = mx_gate_times<CLAMPED, false>(g[j], u[j], args.gate_alpha, args.gate_limit);
   } else {
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
     }
     if (chosen) {
       umma_commit(&sums_done);
-      if (!ok) {
+      if (__builtin_expect(!ok, 0)) {
         drain(&sums_done, 0);  // the products issued so far end before tensor memory is given back
         // and the copies asked for land before the sums take the ring's room, or another CTA this one's: the last slice in each
         // stage, where a warp that gave up first did not ask for its part of it without that part
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   if (warp < 4) {
     const bool good = mbar_wait(&sums_done, 0, &abort_flag) && !*(volatile int*)&abort_flag;
     tc_fence_after();
-    if (!good) drain(&quiet, 0, (STAGES + 3) * DRAIN_LIMIT);  // longer than what arrives there may take
+    if (__builtin_expect(!good, 0)) drain(&quiet, 0, (STAGES + 3) * DRAIN_LIMIT);  // longer than what arrives there may take
     if (!good && threadIdx.x == 0 && args.status) atomicExch(args.status, 2);
     const uint32_t mine = tiles + (uint32_t)(warp * 32 + lane) * 4;
     for (int c = 0; c < live; c += 16) {
