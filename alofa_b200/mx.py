@@ -337,8 +337,9 @@ def _pair_us(tokens: int, rows: int, slices: int, sms: int) -> float:
     return 5.4 + -(-tiles // (sms // 2)) * (0.8 + 0.499 * slices)
 
 
-def plan(tokens: int, rows: int, depth: int, gated: bool = False) -> tuple:
-    """(tokens a tile, parts of the depth) of a product; 256 tokens: pairs of CTAs.
+def plan(tokens: int, rows: int, depth: int, gated: bool = False, here: Optional[int] = None) -> tuple:
+    """(tokens a tile, parts of the depth) of a product on device ``here`` (the
+    current one); 256 tokens: pairs of CTAs.
 
     The kernel for a few tokens has tiles of up to 32 of them in steps of as many,
     of 32 or 64 in larger ones; its depth goes in as many parts as make it
@@ -349,10 +350,11 @@ def plan(tokens: int, rows: int, depth: int, gated: bool = False) -> tuple:
     tokens, 3,584 x 4,608 11.4 in tiles of 64 and 16.7 on pairs; 192 tokens, 3,584
     x 37,888 gated 51.8 and 33.2; 1,024 tokens, 18,944 x 3,584 91.5 and 59.3,
     8,960 x 1,536 27.0 and 30.2."""
-    key = (tokens, rows, depth, gated)
+    sms = _sms(_here() if here is None else here)
+    key = (tokens, rows, depth, gated, sms)
     found = _plans.get(key)
     if found is None:
-        slices, sms = padded(depth) // GROUP, _sms(_here())
+        slices = padded(depth) // GROUP
         tiles = (16,) if tokens <= 16 else (32,) if tokens <= 32 else (32, 64) if tokens <= 64 else (32, 64, 128) if tokens <= 96 else (64, 128)
         ways = [(_few_us(tokens, rows, slices, gated, bn, parts, sms), bn, parts) for bn in tiles if tokens <= MOST_TILES * bn for parts in (1, 2, 3, 4, 6, 8) if parts <= slices]
         if tokens > 64:
@@ -366,7 +368,7 @@ def plan(tokens: int, rows: int, depth: int, gated: bool = False) -> tuple:
 def _product(x: MxRows, w: MxWeight, out_at, scales_at, bias_at, add_at, features: int, gate, out_bf16, status, how, here: int, what: str) -> None:
     if not x.rows:
         return
-    bn, parts = how or plan(x.rows, w.rows, w.k, w.gated)
+    bn, parts = how or plan(x.rows, w.rows, w.k, w.gated, here)
     status_at = 0 if status is None else _at(status, "status", _I32, getattr(status, "shape", ()), here)
     call = _CALL(out_at, scales_at, x.codes_at, x.scales_at, w.at, w.maps_at, bias_at, add_at, status_at, x.rows, w.rows, w.k, features, gate[0], gate[1], bn, parts, _sms(here), out_bf16)
     rc = _lib.alofa_mx_gemm(call, _stream(here))
