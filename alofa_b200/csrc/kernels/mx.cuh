@@ -79,9 +79,6 @@ __device__ __forceinline__ float2 mx_from_e2m1(uint32_t codes) {
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 
-// The row of a gated weight that holds feature f of the gate (half 0) or of the up projection (half 1).
-__host__ __device__ __forceinline__ int mx_gated_row(int f, int half) { return (f / MX_GATE_ROWS) * 2 * MX_GATE_ROWS + half * MX_GATE_ROWS + f % MX_GATE_ROWS; }
-
 // Eight neighbouring numbers a lane, four lanes a block: every lane gets the block's largest magnitude.
 __device__ __forceinline__ uint32_t mx_largest4(const float (&v)[8]) {
   uint32_t m = 0;

@@ -11,7 +11,6 @@ from __future__ import annotations
 import torch
 
 from .. import mx
-from ..csrc import ops
 from ..errors import AlofaError
 from .linear import GATED, RESIDUAL, STORE, Linear, Partial
 
@@ -21,12 +20,11 @@ WEIGHT_FORMATS = (None, MXFP4)
 
 class MxLinear:
     """``epi`` STORE: out = x W^T + b.  RESIDUAL: out (fp32) += x W^T + b.
-    GATED: W = [gate; up]; :meth:`gated_rows` instead of a call."""
+    GATED: W = [gate; up]; :meth:`gated_rows` (silu) instead of a call."""
 
-    def __init__(self, weight, bias, epi: int = STORE, gate=ops.SILU_GATE):
+    def __init__(self, weight, bias, epi: int = STORE):
         self.weight = weight if isinstance(weight, mx.MxWeight) else mx.pack_weight(weight.contiguous(), gated=epi == GATED)
-        self.bias, self.epi, self.gate, self.act = bias, epi, gate, 0
-        self.in_features, self.out_features = self.weight.k, self.weight.n // 2 if epi == GATED else self.weight.n
+        self.bias, self.epi = bias, epi
         if bias is not None and epi == GATED:
             raise AlofaError("unsupported", "a gated product with weights in 4 bits takes no bias")
 
@@ -51,11 +49,11 @@ class MxLinear:
         return None
 
     def gated_rows(self, x, buf=None, status=None) -> mx.MxRows:
-        return mx.gated_linear(self._rows(x, buf), self.weight, self.gate, buf, status)
+        return mx.gated_linear(self._rows(x, buf), self.weight, buf=buf, status=status)
 
 
-def make_linear(rt, weight, bias, epi: int = STORE, gate=ops.SILU_GATE):
+def make_linear(rt, weight, bias, epi: int = STORE):
     """A product of a part's: in the model's compute dtype, or with its weight in 4 bits."""
     if rt.weight_format == MXFP4:
-        return MxLinear(weight, bias, epi, gate)
-    return Linear(weight, bias, epi, gate=gate)
+        return MxLinear(weight, bias, epi)
+    return Linear(weight, bias, epi)
