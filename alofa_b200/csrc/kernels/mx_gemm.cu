@@ -4,9 +4,9 @@
 // silu(y of the gate) * (y of the up projection)  (src/alofa/kernels/cpu/scalar.mojo:132-231).
 // One tcgen05.mma.kind::mxf8f6f4.block_scale takes one block of 32 numbers of its rows; the scales are its
 // operands too, in tensor memory, so sums are of the numbers themselves and in fp32.  The tensor cores' additions cut off towards zero
-// where scalar ones round: at depth 3,584 with scales over a range of 2^14, 1,999 x 37,888 sums are 1.5e-7 of their norm off,
-// 0.9e-7 of it a common share of every sum, so that of 37.9 million gated numbers 150 are coded on the other side of a tie, and 110
-// from sums of scalar additions (0.54e-4 to 0.63e-4 and 1.0e-4 to 1.3e-4 of the rows' norm; one rounding to 8 bits is up to 2^-4).
+// where scalar ones round; sums go in runs so that this stays small (RUN_SLICES).  At depth 3,584 with scales over a range of 2^14, 1,999 x
+// 18,944 gated numbers are then 0.6e-4 to 1.3e-4 of the rows' norm off, and from sums of scalar additions 0.5e-4 to 1.1e-4: some hundred of
+// 37.9 million that fall on the other side of a tie of two codes (one rounding to 8 bits is up to 2^-4).
 //
 // A k-slice is 128 numbers: four blocks.  A weight's tile of a slice is 8,704 contiguous bytes of memory
 // (8,192 of codes, 512 of scales), fetched by one thread with two copies: TMA, which unpacks 4-bit numbers on
@@ -111,6 +111,15 @@ __device__ __forceinline__ void umma_mx_pair(uint32_t tmem_d, uint64_t desc_a, u
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
       : "memory");
 }
+// The tensor cores' additions cut off towards zero some bits below the accumulator's last one, which takes 3.9e-9 off every sum for
+// each slice that went into it: 1.1e-7 over 28 slices, 7.7e-7 over 148.  The depth therefore goes in runs of slices, each with an accumulator
+// of its own, added up by additions that round.  With 14 slices a run 1,999 x 37,888 sums of depth 3,584 are 0.9e-7 of their norm
+// off, with 28 1.55e-7, and 0.7e-7 by scalar additions; of depth 18,944 (2.0e-7 with 37, 9.4e-7 with 148) 1.8e-7.
+// Runs cost next to nothing for a few tokens, whose accumulators are small enough to stand beside one another.  For prompts each
+// takes the accumulator from the products for 1,100 clocks: gate and up of 7B, 1,999 tokens, 227 us in one run and 237 in two.  What is
+// stored takes twice the slices a run there, as its rounding to bfloat16 is 10^4 times as much, and fp32 sums of any depth are within 2e-7:
+// q, k and v of 7B, 2,048 tokens, 33.5 us in one run and 35.6 in two.
+constexpr int RUN_SLICES = 16, RUN_SLICES_STORED = 32;
 constexpr uint32_t E4M3 = 0, E2M1 = 5;
 // The instruction: types of A and B, scales E8M0, M and N, the scales' byte `block` of their column.
 constexpr uint32_t mx_idesc(uint32_t a, uint32_t b, int m, int n, int block) {
@@ -159,8 +168,8 @@ struct FewTile {
   static constexpr uint32_t A_BYTES = MX_TILE_ROWS * MX_GROUP, B_BYTES = BN * MX_GROUP;
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES + 1024;  // tiles, 512 bytes of the weight's scales, 512 of the tokens'
   static constexpr uint32_t SMEM = STAGES * STAGE_BYTES + 1024;
-  static constexpr int COLS = BN + STAGES * 8;  // the scales have as many places as the ring has stages: those of a slice are written when the products of the slice before them there are complete
-  static constexpr uint32_t TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+  static constexpr int SCALE_COLS = STAGES * 8;  // the scales have as many places as the ring has stages: those of a slice are written when the products of the slice before them there are complete
+  static constexpr int MOST_RUNS = (256 - SCALE_COLS) / BN;  // two CTAs an SM: 256 columns each at most
   static_assert(BN * SUM_PITCH * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's room");
 };
 
@@ -245,10 +254,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   __shared__ int abort_flag, asked[2];
 
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int part = blockIdx.x % parts, f_tile = blockIdx.x / parts;  // a cluster: the parts of one tile's depth
+  const int f_tile = blockIdx.x / (unsigned)parts, part = blockIdx.x - f_tile * parts;  // a cluster: the parts of one tile's depth
   const int f0 = f_tile * MX_TILE_ROWS, t0 = blockIdx.y * BN;
   // parts that differ by one slice at most
-  const int first = (int)((long long)args.slices * part / parts), n = (int)((long long)args.slices * (part + 1) / parts) - first;
+  const int first = (unsigned)(args.slices * part) / (unsigned)parts, n = (unsigned)(args.slices * (part + 1)) / (unsigned)parts - first;  // at most 2^23 slices in 8 parts
+  const int runs = min((n + RUN_SLICES - 1) / RUN_SLICES, Tile::MOST_RUNS);  // of slices, each with sums of its own
+  const uint32_t need = (uint32_t)(runs * BN + Tile::SCALE_COLS), tmem_cols = need <= 64 ? 64 : need <= 128 ? 128 : 256;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
@@ -260,7 +271,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
     mbar_init(&quiet, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 5) tmem_alloc(&tmem_base_smem, Tile::TMEM_COLS);
+  if (warp == 5) tmem_alloc(&tmem_base_smem, tmem_cols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -315,15 +326,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
     if (lane == 0) asked[1] = i, mbar_arrive(&asked_all);
   } else if (warp == 5) {
     const bool chosen = elect_lane();
-    const uint32_t sums = uniform(tmem);
-    int s = 0;
+    const uint32_t place = uniform(tmem) + (uint32_t)(runs * BN);
+    uint32_t sums = uniform(tmem), add = 0;  // a run's first products begin its sums
+    const int run_slices = runs > 1 ? (unsigned)n / (unsigned)runs : n, longer = n - runs * run_slices;  // the first `longer` runs have one slice more
+    int s = 0, run = 0, left = run_slices + (longer > 0 ? 1 : 0);
     uint32_t round = 0;
     bool ok = true, ready = false;
     for (int i = 0; i < n; ++i) {
       if (!all_lanes(ready)) ok = all_lanes(mbar_wait(&landed[s], round, &abort_flag));
       if (!ok) break;
       const uint32_t stage = tiles + s * Tile::STAGE_BYTES, scales = stage + Tile::A_BYTES + Tile::B_BYTES;
-      const uint32_t scale_a = sums + BN + s * 8, scale_b = scale_a + 4;
+      const uint32_t scale_a = place + s * 8, scale_b = scale_a + 4;
       uint64_t* freed = &stage_free[s];
       s = s + 1 == STAGES ? 0 : s + 1;
       round ^= s == 0 ? 1u : 0u;
@@ -335,9 +348,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
         scales_to_tmem(scale_a, scales);
         scales_to_tmem(scale_b, scales + 512);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) umma_mx(sums, a + 2 * j, b + 2 * j, mx_idesc(E2M1, E4M3, 128, BN, j), scale_a, scale_b, (i | j) ? 1u : 0u);
+        for (int j = 0; j < 4; ++j) umma_mx(sums, a + 2 * j, b + 2 * j, mx_idesc(E2M1, E4M3, 128, BN, j), scale_a, scale_b, j ? 1u : add);
         umma_commit(freed);
       }
+      add = 1;
+      if (--left == 0) ++run, left = run_slices + (run < longer ? 1 : 0), sums += BN, add = 0;
     }
     if (chosen) {
       umma_commit(&sums_done);
@@ -370,6 +385,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
       uint32_t r[16];
       tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c, r);
       tmem_ld_wait();
+      for (int z = 1; z < runs; ++z) {
+        uint32_t q[16];
+        tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + z * BN + c, q);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(q[j]));
+      }
 #pragma unroll
       for (int j = 0; j < 16; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + (uint32_t)((c + j) * SUM_PITCH * 4)), "f"(good ? __uint_as_float(r[j]) : __uint_as_float(0x7fc00000u)) : "memory");
     }
@@ -414,7 +436,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   else __syncthreads();
   if (warp == 5) {
     tc_fence_after();
-    tmem_dealloc(tmem, Tile::TMEM_COLS);
+    tmem_dealloc(tmem, tmem_cols);
   }
 }
 
@@ -457,6 +479,21 @@ __device__ __forceinline__ void pair_load64(uint32_t tmem, uint32_t (&r)[64]) {
     for (int i = 0; i < 16; ++i) r[j * 16 + i] = q[i];
   }
   tmem_ld_wait();
+}
+
+// What a run left, on top of the runs before it (`first`: there are none).  `have()` when it is in registers.
+template <typename Have>
+__device__ __forceinline__ void pair_take64(uint32_t tmem, uint32_t (&r)[64], bool first, Have have) {
+  if (first) {
+    pair_load64(tmem, r);
+    have();
+  } else {
+    uint32_t a[64];
+    pair_load64(tmem, a);
+    have();
+#pragma unroll
+    for (int i = 0; i < 64; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(a[i]));
+  }
 }
 
 // 64 rows' sums of one token of a gated weight: one block of codes and its scale.  The clamped form, gates far below zero and the
@@ -568,6 +605,10 @@ __device__ __forceinline__ void pair_stored64(const MxArgs& args, const uint32_t
   }
 }
 
+// LONG: depths of several runs (RUN_SLICES).  Each has an accumulator to itself, in turns as tiles have where they are one run,
+// and the epilogue's warps keep the tile's sums in registers, 128 a thread.  The four other warps hand over what those need: of the
+// 168 registers that 384 threads are launched with, 128 threads keep 88 and 256 have 208, which is all of them.
+template <bool LONG>
 __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_x, const MxArgs args) {
   constexpr int STAGES = PAIR_STAGES;
   constexpr uint32_t A_BYTES = 128 * MX_GROUP, B_BYTES = 128 * MX_GROUP;
@@ -604,166 +645,212 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) mx_pair_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = tmem_base_smem;
 
+  const int most = args.F ? RUN_SLICES : RUN_SLICES_STORED;
+  const int runs = LONG ? (slices + most - 1) / most : 1, run_slices = LONG ? slices / runs : slices, longer = slices - runs * run_slices;  // the first `longer` runs have one slice more
   const uint32_t chunk_room = tiles + STAGES * PAIR_STAGE_BYTES;
-  if (warp < 2) {
-    // warp 0 the weight's rows and the scales of all 256, warp 1 the tokens: both CTAs' copies count on the first one's barrier
-    if (warp == 1) {
-      pdl_wait();
-      pdl_launch();
-    }
-    const bool chosen = elect_lane();
-    int it = 0, s = 0;  // slices asked for so far, over all tiles; the ring's stage
-    uint32_t round = 1;  // parity of the phase in which it was last freed; the first round waits for nothing
-    bool ok = true, free = true;
-    const uint32_t first_landed = uniform(in_cluster_cta(&landed[0], 0));
-    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
-      // a number of rows that is no multiple of 256 leaves the second CTA without any: it reads the last ones, and what comes of them is not stored
-      const int even = tile % f_tiles * 2 * slices, odd = min(tile % f_tiles * 2 + 1, last_weight_tile) * slices;
-      const int t0 = tile / f_tiles * 256 + (int)rank * 128;
-      for (int i = 0; i < slices; ++i, ++it) {
-        if (!all_lanes(free)) ok = all_lanes(mbar_wait(&stage_free[s], round, &abort_flag));
-        if (!ok) break;
-        const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, bar = first_landed + (uint32_t)s * 8;
-        uint64_t* mine = &landed[s];
-        s = s + 1 == STAGES ? 0 : s + 1;
-        round ^= s == 0 ? 1u : 0u;
-        free = it + 1 < STAGES || mbar_complete(&stage_free[s], round);
-        if (chosen) {
-          if (warp == 0) {
-            if (rank == 0) mbar_expect_tx(mine, 2 * (A_BYTES + MX_TILE_CODES + 1024));
-            load_tile_pair(stage + A_BYTES, &map_w, bar, 0, ((rank ? odd : even) + i) * MX_TILE_MAP_ROWS);
-            load_tile_pair(stage + A_BYTES + B_BYTES, &map_s, bar, 0, (even + i) * MX_TILE_MAP_ROWS + MX_TILE_ROWS);
-            load_tile_pair(stage + A_BYTES + B_BYTES + 512, &map_s, bar, 0, (odd + i) * MX_TILE_MAP_ROWS + MX_TILE_ROWS);
-          } else {
-            load_tile_pair(stage, &map_x, bar, i * MX_GROUP, t0);
-          }
-        }
+  static_assert(128 * 88 + (PAIR_THREADS - 128) * 208 <= PAIR_THREADS * 168, "the shares are of what the block was launched with");
+  if (warp < 4) {
+    if constexpr (LONG) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp < 2) {
+      // warp 0 the weight's rows and the scales of all 256, warp 1 the tokens: both CTAs' copies count on the first one's barrier
+      if (warp == 1) {
+        pdl_wait();
+        pdl_launch();
       }
-    }
-    // what the first CTA's products say to this one's barriers has come before this one leaves
-    for (int j = max(0, it - STAGES); warp == 0 && ok && j < it; ++j) ok = all_lanes(mbar_wait(&stage_free[j % STAGES], (uint32_t)(j / STAGES) & 1u, &abort_flag));
-  } else if (warp == 3) {
-    pdl_wait();
-    const int row_bytes = 4 * slices;
-    const bool wide = slices % 4 == 0 && (uintptr_t)args.x_scales % 16 == 0;
-    const uint32_t tell = in_cluster_cta(&scales_in[0], 0);
-    int c = 0;  // chunks so far
-    bool ok = true;
-    for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
-      const int t0 = tile / f_tiles * 256 + (int)rank * 128;
-      for (int i = 0; i < slices; i += PAIR_CHUNK, ++c) {
-        const int have = min(PAIR_CHUNK, slices - i);
-        uint32_t v[4][PAIR_CHUNK];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {  // a lane has rows lane, 32 + lane, ...
-          const int t = t0 + r * 32 + lane;
-          const uint8_t* src = args.x_scales + (size_t)min(t, args.T - 1) * row_bytes + 4 * i;
-          if (wide && have >= 4) {
-            const uint4 a = *reinterpret_cast<const uint4*>(src);
-            const uint4 b = have == 8 ? *reinterpret_cast<const uint4*>(src + 16) : make_uint4(0u, 0u, 0u, 0u);
-            v[r][0] = a.x, v[r][1] = a.y, v[r][2] = a.z, v[r][3] = a.w, v[r][4] = b.x, v[r][5] = b.y, v[r][6] = b.z, v[r][7] = b.w;
-          } else {
-#pragma unroll
-            for (int j = 0; j < PAIR_CHUNK; ++j) v[r][j] = j < have ? *reinterpret_cast<const uint32_t*>(src + 4 * j) : 0u;
-          }
-        }
-        if (c >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&chunk_free[c & 1], (uint32_t)(c / 2 - 1) & 1u, &abort_flag));
-        if (!ok) break;
-        const uint32_t room = chunk_room + (uint32_t)((c & 1) * PAIR_CHUNK * 512 + lane * 16);
-#pragma unroll
-        for (int j = 0; j < PAIR_CHUNK; ++j)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(room + j * 512), "r"(v[0][j]), "r"(v[1][j]), "r"(v[2][j]), "r"(v[3][j]) : "memory");
-        fence_to_tensor_core();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_in_cluster(tell + (uint32_t)(c & 1) * 8);
-      }
-    }
-    for (int j = max(0, c - 2); ok && j < c; ++j) ok = __all_sync(0xffffffffu, mbar_wait(&chunk_free[j & 1], (uint32_t)(j / 2) & 1u, &abort_flag));
-  } else if (warp == 2) {
-    if (rank == 0) {
       const bool chosen = elect_lane();
-      const uint32_t base = uniform(tmem);
-      int done = 0, it = 0, c = 0, s = 0, place = 0;  // tiles begun, slices and chunks so far, the ring's stage, the scales' place
-      uint32_t round = 0;
-      bool ok = true, ready = false, place_free = true;
-      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs, ++done) {
-        // the tile's first slice and scales are there before the epilogue has the columns that this accumulator shares with the last one
-        ok = all_lanes(mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag));
-        if (ok && !all_lanes(ready)) ok = all_lanes(mbar_wait(&landed[s], round, &abort_flag));
-        ready = true;
-        if (ok && done) ok = all_lanes(mbar_wait(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t sums = base + (done & 1 ? PAIR_SECOND : 0);
+      int it = 0, s = 0;  // slices asked for so far, over all tiles; the ring's stage
+      uint32_t round = 1;  // parity of the phase in which it was last freed; the first round waits for nothing
+      bool ok = true, free = true;
+      const uint32_t first_landed = uniform(in_cluster_cta(&landed[0], 0));
+      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+        // a number of rows that is no multiple of 256 leaves the second CTA without any: it reads the last ones, and what comes of them is not stored
+        const int even = tile % f_tiles * 2 * slices, odd = min(tile % f_tiles * 2 + 1, last_weight_tile) * slices;
+        const int t0 = tile / f_tiles * 256 + (int)rank * 128;
         for (int i = 0; i < slices; ++i, ++it) {
-          if (i % PAIR_CHUNK == 0 && i) ok = all_lanes(mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag));
-          if (ok && !all_lanes(ready)) ok = all_lanes(mbar_wait(&landed[s], round, &abort_flag));
-          // the slice before it in this place of the scales: five slices ago, whose stage is the next one's now
-          if (ok && !all_lanes(place_free)) ok = all_lanes(mbar_wait(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it - PAIR_SCALE_PLACES) / STAGES) & 1u, &abort_flag));
+          if (!all_lanes(free)) ok = all_lanes(mbar_wait(&stage_free[s], round, &abort_flag));
           if (!ok) break;
-          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES;
-          const uint32_t token_scales = chunk_room + (uint32_t)((c & 1) * PAIR_CHUNK + i % PAIR_CHUNK) * 512;
-          const uint32_t scale_a = base + PAIR_SCALES + place * 12, scale_b = scale_a + 4;
-          uint64_t* freed = &stage_free[s];
+          const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, bar = first_landed + (uint32_t)s * 8;
+          uint64_t* mine = &landed[s];
           s = s + 1 == STAGES ? 0 : s + 1;
-          place = place + 1 == PAIR_SCALE_PLACES ? 0 : place + 1;
           round ^= s == 0 ? 1u : 0u;
-          tc_fence_after();
-          ready = mbar_complete(&landed[s], round);
-          place_free = it + 1 < PAIR_SCALE_PLACES || mbar_complete(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it + 1 - PAIR_SCALE_PLACES) / STAGES) & 1u);
-          const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + A_BYTES);
-          const bool chunk_ends = i % PAIR_CHUNK == PAIR_CHUNK - 1 || i == slices - 1;
+          free = it + 1 < STAGES || mbar_complete(&stage_free[s], round);
           if (chosen) {
-            scales_to_tmem_pair(scale_a, token_scales);
-            scales_to_tmem_pair(scale_b, scales);
-            scales_to_tmem_pair(scale_b + 4, scales + 512);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) umma_mx_pair(sums, a + 2 * j, b + 2 * j, mx_idesc(E4M3, E2M1, 256, 256, j), scale_a, scale_b, (i | j) ? 1u : 0u);
-            umma_commit_pair(freed, 3);
-            if (chunk_ends) umma_commit_pair(&chunk_free[c & 1], 3);
+            if (warp == 0) {
+              if (rank == 0) mbar_expect_tx(mine, 2 * (A_BYTES + MX_TILE_CODES + 1024));
+              load_tile_pair(stage + A_BYTES, &map_w, bar, 0, ((rank ? odd : even) + i) * MX_TILE_MAP_ROWS);
+              load_tile_pair(stage + A_BYTES + B_BYTES, &map_s, bar, 0, (even + i) * MX_TILE_MAP_ROWS + MX_TILE_ROWS);
+              load_tile_pair(stage + A_BYTES + B_BYTES + 512, &map_s, bar, 0, (odd + i) * MX_TILE_MAP_ROWS + MX_TILE_ROWS);
+            } else {
+              load_tile_pair(stage, &map_x, bar, i * MX_GROUP, t0);
+            }
           }
-          c += chunk_ends ? 1 : 0;
         }
-        if (ok && chosen) umma_commit_pair(&sums_ready, 3);
       }
-      if (!ok && chosen) {  // the products issued so far end before tensor memory is given back
-        umma_commit_pair(&gave_up, 3);
-        drain(&gave_up, 0);
-        // and the copies asked for land
-        for (int j = 0; j < STAGES; ++j) drain(&landed[j], 0), drain(&landed[j], 1);
+      // what the first CTA's products say to this one's barriers has come before this one leaves
+      for (int j = max(0, it - STAGES); warp == 0 && ok && j < it; ++j) ok = all_lanes(mbar_wait(&stage_free[j % STAGES], (uint32_t)(j / STAGES) & 1u, &abort_flag));
+    } else if (warp == 3) {
+      pdl_wait();
+      const int row_bytes = 4 * slices;
+      const bool wide = slices % 4 == 0 && (uintptr_t)args.x_scales % 16 == 0;
+      const uint32_t tell = in_cluster_cta(&scales_in[0], 0);
+      int c = 0;  // chunks so far
+      bool ok = true;
+      for (int tile = pair; tile < n_tiles && ok; tile += n_pairs) {
+        const int t0 = tile / f_tiles * 256 + (int)rank * 128;
+        for (int i = 0; i < slices; i += PAIR_CHUNK, ++c) {
+          const int have = min(PAIR_CHUNK, slices - i);
+          uint32_t v[4][PAIR_CHUNK];
+  #pragma unroll
+          for (int r = 0; r < 4; ++r) {  // a lane has rows lane, 32 + lane, ...
+            const int t = t0 + r * 32 + lane;
+            const uint8_t* src = args.x_scales + (size_t)min(t, args.T - 1) * row_bytes + 4 * i;
+            if (wide && have >= 4) {
+              const uint4 a = *reinterpret_cast<const uint4*>(src);
+              const uint4 b = have == 8 ? *reinterpret_cast<const uint4*>(src + 16) : make_uint4(0u, 0u, 0u, 0u);
+              v[r][0] = a.x, v[r][1] = a.y, v[r][2] = a.z, v[r][3] = a.w, v[r][4] = b.x, v[r][5] = b.y, v[r][6] = b.z, v[r][7] = b.w;
+            } else {
+  #pragma unroll
+              for (int j = 0; j < PAIR_CHUNK; ++j) v[r][j] = j < have ? *reinterpret_cast<const uint32_t*>(src + 4 * j) : 0u;
+            }
+          }
+          if (c >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&chunk_free[c & 1], (uint32_t)(c / 2 - 1) & 1u, &abort_flag));
+          if (!ok) break;
+          const uint32_t room = chunk_room + (uint32_t)((c & 1) * PAIR_CHUNK * 512 + lane * 16);
+  #pragma unroll
+          for (int j = 0; j < PAIR_CHUNK; ++j)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(room + j * 512), "r"(v[0][j]), "r"(v[1][j]), "r"(v[2][j]), "r"(v[3][j]) : "memory");
+          fence_to_tensor_core();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_in_cluster(tell + (uint32_t)(c & 1) * 8);
+        }
+      }
+      for (int j = max(0, c - 2); ok && j < c; ++j) ok = __all_sync(0xffffffffu, mbar_wait(&chunk_free[j & 1], (uint32_t)(j / 2) & 1u, &abort_flag));
+    } else if (warp == 2) {
+      if (rank == 0) {
+        const bool chosen = elect_lane();
+        const uint32_t base = uniform(tmem);
+        int done = 0, it = 0, c = 0, s = 0, place = 0;  // runs begun, slices and chunks so far, the ring's stage, the scales' place
+        uint32_t round = 0;
+        bool ok = true, ready = false, place_free = true;
+        for (int tile = pair; tile < n_tiles && ok; tile += n_pairs, ++done) {
+          // the tile's first slice and scales are there before the epilogue has the columns that this accumulator shares with the last one
+          ok = all_lanes(mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag));
+          if (ok && !all_lanes(ready)) ok = all_lanes(mbar_wait(&landed[s], round, &abort_flag));
+          ready = true;
+          if (ok && done) ok = all_lanes(mbar_wait(&sums_taken, (uint32_t)(done - 1) & 1u, &abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t sums = base + (done & 1 ? PAIR_SECOND : 0), add = 0;  // a run's first products begin its sums
+          int run = 0, left = run_slices + (LONG && longer > 0 ? 1 : 0);
+          for (int i = 0; i < slices; ++i, ++it) {
+            if (i % PAIR_CHUNK == 0 && i) ok = all_lanes(mbar_wait_in_cluster(&scales_in[c & 1], (uint32_t)(c / 2) & 1u, &abort_flag));
+            if (ok && !all_lanes(ready)) ok = all_lanes(mbar_wait(&landed[s], round, &abort_flag));
+            // the slice before it in this place of the scales: five slices ago, whose stage is the next one's now
+            if (ok && !all_lanes(place_free)) ok = all_lanes(mbar_wait(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it - PAIR_SCALE_PLACES) / STAGES) & 1u, &abort_flag));
+            if (LONG && left == 0) {  // the next run: the same waits as for a tile's first one
+              if (ok) ok = all_lanes(mbar_wait(&sums_taken, (uint32_t)done & 1u, &abort_flag));
+              ++done, ++run, left = run_slices + (run < longer ? 1 : 0), add = 0;
+              sums = base + (done & 1 ? PAIR_SECOND : 0);
+            }
+            if (!ok) break;
+            const uint32_t stage = tiles + s * PAIR_STAGE_BYTES, scales = stage + A_BYTES + B_BYTES;
+            const uint32_t token_scales = chunk_room + (uint32_t)((c & 1) * PAIR_CHUNK + i % PAIR_CHUNK) * 512;
+            const uint32_t scale_a = base + PAIR_SCALES + place * 12, scale_b = scale_a + 4;
+            uint64_t* freed = &stage_free[s];
+            s = s + 1 == STAGES ? 0 : s + 1;
+            place = place + 1 == PAIR_SCALE_PLACES ? 0 : place + 1;
+            round ^= s == 0 ? 1u : 0u;
+            tc_fence_after();
+            ready = mbar_complete(&landed[s], round);
+            place_free = it + 1 < PAIR_SCALE_PLACES || mbar_complete(&stage_free[s + 1 == STAGES ? 0 : s + 1], (uint32_t)((it + 1 - PAIR_SCALE_PLACES) / STAGES) & 1u);
+            const uint64_t a = smem_desc_sw128(stage), b = smem_desc_sw128(stage + A_BYTES);
+            const bool chunk_ends = i % PAIR_CHUNK == PAIR_CHUNK - 1 || i == slices - 1;
+            if (chosen) {
+              scales_to_tmem_pair(scale_a, token_scales);
+              scales_to_tmem_pair(scale_b, scales);
+              scales_to_tmem_pair(scale_b + 4, scales + 512);
+  #pragma unroll
+              for (int j = 0; j < 4; ++j) umma_mx_pair(sums, a + 2 * j, b + 2 * j, mx_idesc(E4M3, E2M1, 256, 256, j), scale_a, scale_b, j ? 1u : add);
+              umma_commit_pair(freed, 3);
+              if (chunk_ends) umma_commit_pair(&chunk_free[c & 1], 3);
+              if (LONG && left == 1 && i + 1 < slices) umma_commit_pair(&sums_ready, 3);
+            }
+            c += chunk_ends ? 1 : 0;
+            add = 1;
+            if (LONG) --left;
+          }
+          if (ok && chosen) umma_commit_pair(&sums_ready, 3);
+        }
+        if (!ok && chosen) {  // the products issued so far end before tensor memory is given back
+          umma_commit_pair(&gave_up, 3);
+          drain(&gave_up, 0);
+          // and the copies asked for land
+          for (int j = 0; j < STAGES; ++j) drain(&landed[j], 0), drain(&landed[j], 1);
+        }
       }
     }
-  } else if (warp >= 4) {
+  } else {
+    if constexpr (LONG) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int q = warp & 3, half = (warp - 4) >> 2;  // a quarter of the lanes (warps read 32 (w % 4) and on), half of the columns
     pdl_wait();  // what is written here, an earlier kernel may have been reading
     const uint32_t taken = in_cluster_cta(&sums_taken, 0);
     float* turn = reinterpret_cast<float*>(smem_raw + (tiles - smem_u32(smem_raw)) + PAIR_TURN) + (warp - 4) * 32 * TURN_PITCH;
     bool good = true;
-    int done = 0;
+    int done = 0;  // runs so far
+    auto finish = [&](const uint32_t (&r)[64], int t, int row) {
+      if (!args.F) pair_stored64(args, r, t - lane, row, good, turn, lane);
+      else if (t >= args.T) ;
+      else if (args.gate_alpha == 0.f) pair_gated64<false>(args, r, t, row, good);
+      else pair_gated64<true>(args, r, t, row, good);
+      __syncwarp();
+    };
     for (int tile = pair; tile < n_tiles; tile += n_pairs, ++done) {
       const int row0 = (tile % f_tiles) * 256 + half * 128, t = tile / f_tiles * 256 + (int)rank * 128 + q * 32 + lane;
-      good = good && __all_sync(0xffffffffu, mbar_wait(&sums_ready, (uint32_t)done & 1u, &abort_flag));
-      tc_fence_after();
-      const bool second = done & 1, shared_half = half == (second ? 0 : 1);  // the shared columns: the first tile's last, the second's first
-      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (second ? PAIR_SECOND : 0) + half * 128;
-      if (!shared_half && lane == 0) tell_in_cluster(taken);  // this half's columns are no part of the next tile's accumulator
+      uint32_t lo[LONG ? 64 : 1], hi[LONG ? 64 : 1];
 #pragma unroll 1
-      for (int k = 0; k < 2; ++k) {
-        const int block = second ? k : 1 - k;  // the block with the shared columns first
-        uint32_t r[64];
-        pair_load64(at + block * 64, r);
-        if (k == 0 && shared_half) {
+      for (int run = 0;; ++run, ++done) {
+        good = good && __all_sync(0xffffffffu, mbar_wait(&sums_ready, (uint32_t)done & 1u, &abort_flag));
+        tc_fence_after();
+        const bool second = done & 1, shared_half = half == (second ? 0 : 1);  // the shared columns: the first accumulator's last, the second's first
+        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (second ? PAIR_SECOND : 0) + half * 128;
+        auto have_shared = [&]() {
+          if (!shared_half) return;
           tc_fence_before();
           __syncwarp();
           if (lane == 0) tell_in_cluster(taken);
+        };
+        if (!shared_half && lane == 0) tell_in_cluster(taken);  // this half's columns are no part of the next accumulator
+        if constexpr (LONG) {  // the block with the shared columns first
+          if (second) {
+            pair_take64(at, lo, run == 0, have_shared);
+            pair_take64(at + 64, hi, run == 0, [] {});
+          } else {
+            pair_take64(at + 64, hi, run == 0, have_shared);
+            pair_take64(at, lo, run == 0, [] {});
+          }
+          if (run + 1 < runs) {
+            tc_fence_before();
+            continue;
+          }
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k) {  // the epilogue's instructions once
+            finish(lo, t, row0 + k * 64);
+#pragma unroll
+            for (int j = 0; j < 64; ++j) lo[j] = hi[j];
+          }
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k) {
+            const int block = second ? k : 1 - k;
+            uint32_t r[64];
+            pair_load64(at + block * 64, r);
+            if (k == 0) have_shared();
+            finish(r, t, row0 + block * 64);
+          }
         }
-        if (!args.F) pair_stored64(args, r, t - lane, row0 + block * 64, good, turn, lane);
-        else if (t >= args.T) ;
-        else if (args.gate_alpha == 0.f) pair_gated64<false>(args, r, t, row0 + block * 64, good);
-        else pair_gated64<true>(args, r, t, row0 + block * 64, good);
-        __syncwarp();
+        tc_fence_before();
+        break;
       }
-      tc_fence_before();
     }
   }
   __syncwarp();
@@ -819,7 +906,7 @@ static bool allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& d
   return true;
 }
 template <int BN> static std::atomic<uint64_t> few_allowed{0};
-static std::atomic<uint64_t> pair_allowed{0};
+template <bool LONG> static std::atomic<uint64_t> pair_allowed{0};
 
 template <int BN>
 static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const MxArgs& args, int parts, cudaStream_t stream) {
@@ -830,8 +917,15 @@ static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const 
   return launch_status();
 }
 
+template <bool LONG>
+static int launch_pair(const CUtensorMap& map_w, const CUtensorMap& map_s, const CUtensorMap& map_x, const MxArgs& args, unsigned grid, cudaStream_t stream) {
+  if (!allow_shared((const void*)mx_pair_kernel<LONG>, (int)PAIR_SMEM, pair_allowed<LONG>)) return ALOFA_ERR_LAUNCH;
+  launch_dep_cluster(mx_pair_kernel<LONG>, dim3(grid), PAIR_THREADS, PAIR_SMEM, stream, 2, map_w, map_s, map_x, args);
+  return launch_status();
+}
+
 // A product as its caller packs it: one argument, where twenty-two would take longer to hand over than the launch.
-// bn: 256: pairs of CTAs (`parts` 1, a grid of `ctas` of them); 16, 32, 64 or 128 tokens a CTA, the depth in `parts` parts.
+// bn: 256: pairs of CTAs (`parts` 1, a grid of `ctas` of them); 16, 32, 64, 96 or 128 tokens a CTA, the depth in `parts` parts.
 // features > 0: out are the codes and out_scales the scales of that many gated features, n the rows of the gated weight.
 // weight_maps: alofa_mx_weight_maps' of the tiles.
 struct MxCall {
@@ -866,7 +960,7 @@ ALOFA_API int alofa_mx_gemm(const MxCall* call, void* stream) {
   args.T = t, args.N = n, args.slices = (k + MX_GROUP - 1) / MX_GROUP, args.F = features, args.out_bf16 = out_bf16, args.status = status;
   args.gate_alpha = gate_alpha, args.gate_limit = gate_limit;
   args.wide = n % 4 == 0 && ((uintptr_t)out | (uintptr_t)bias | (uintptr_t)add) % 16 == 0;
-  const bool few = bn == 16 || bn == 32 || bn == 64 || bn == 128;
+  const bool few = bn == 16 || bn == 32 || bn == 64 || bn == 96 || bn == 128;
   if (!few && bn != 256) return ALOFA_ERR_ARGUMENT;
   if (parts < 1 || parts > args.slices || parts > (few ? FEW_PARTS : 1)) return ALOFA_ERR_ARGUMENT;
   CUtensorMap map_w, map_s, map_x;
@@ -878,12 +972,11 @@ ALOFA_API int alofa_mx_gemm(const MxCall* call, void* stream) {
     case 16: return launch_few<16>(map_w, map_x, args, parts, s);
     case 32: return launch_few<32>(map_w, map_x, args, parts, s);
     case 64: return launch_few<64>(map_w, map_x, args, parts, s);
+    case 96: return launch_few<96>(map_w, map_x, args, parts, s);
     case 128: return launch_few<128>(map_w, map_x, args, parts, s);
   }
   const long long pair_tiles = (((long long)n + 255) / 256) * (((long long)t + 255) / 256);
   if (ctas < 2 || pair_tiles > 0x3fffffffll) return ALOFA_ERR_ARGUMENT;
-  if (!allow_shared((const void*)mx_pair_kernel, (int)PAIR_SMEM, pair_allowed)) return ALOFA_ERR_LAUNCH;
-  const long long grid = 2 * pair_tiles < ctas ? 2 * pair_tiles : ctas / 2 * 2;
-  launch_dep_cluster(mx_pair_kernel, dim3((unsigned)grid), PAIR_THREADS, PAIR_SMEM, s, 2, map_w, map_s, map_x, args);
-  return launch_status();
+  const unsigned grid = (unsigned)(2 * pair_tiles < ctas ? 2 * pair_tiles : ctas / 2 * 2);
+  return args.slices > (features ? RUN_SLICES : RUN_SLICES_STORED) ? launch_pair<true>(map_w, map_s, map_x, args, grid, s) : launch_pair<false>(map_w, map_s, map_x, args, grid, s);
 }

@@ -316,10 +316,13 @@ def _sms(here: int) -> int:
     return _SMS[here]
 
 
+# As in kernels/mx_gemm.cu: slices that one accumulator sums (for prompts, of what is stored), and accumulators of a tile by its tokens.
+RUN_SLICES, RUN_SLICES_STORED, MOST_RUNS = 16, 32, {16: 13, 32: 6, 64: 3, 96: 2, 128: 1}
+
 # What a product takes, fitted to the times of every way at the shapes of 0.5 to 7 billion parameters and 1 to 1,024 tokens: the way
 # it chooses is 1.3 % off the fastest on the average.  Microseconds for a slice of 128 numbers of a CTA of the kernel for a few
 # tokens, by its tokens: alone on its SM, and where two share one.
-_FEW_SLICE = {16: (0.354, 0.400), 32: (0.225, 0.241), 64: (0.326, 0.420), 128: (0.743, 0.866)}
+_FEW_SLICE = {16: (0.354, 0.400), 32: (0.225, 0.241), 64: (0.326, 0.420), 96: (0.743, 0.866), 128: (0.743, 0.866)}
 
 
 def _few_us(tokens: int, rows: int, slices: int, gated: bool, bn: int, parts: int, sms: int) -> float:
@@ -332,9 +335,9 @@ def _few_us(tokens: int, rows: int, slices: int, gated: bool, bn: int, parts: in
     return 4.94 + 0.226 * parts + last + rounds * -(-slices // parts) + 3.69 * (whole - (rest == 0))
 
 
-def _pair_us(tokens: int, rows: int, slices: int, sms: int) -> float:
-    tiles = -(-rows // 256) * -(-tokens // 256)
-    return 5.4 + -(-tiles // (sms // 2)) * (0.8 + 0.499 * slices)
+def _pair_us(tokens: int, rows: int, slices: int, gated: bool, sms: int) -> float:
+    tiles, runs = -(-rows // 256) * -(-tokens // 256), -(-slices // (RUN_SLICES if gated else RUN_SLICES_STORED))
+    return 5.4 + -(-tiles // (sms // 2)) * (0.8 + 0.499 * slices + 1.3 * (runs - 1))
 
 
 def plan(tokens: int, rows: int, depth: int, gated: bool = False, here: Optional[int] = None) -> tuple:
@@ -355,10 +358,14 @@ def plan(tokens: int, rows: int, depth: int, gated: bool = False, here: Optional
     found = _plans.get(key)
     if found is None:
         slices = padded(depth) // GROUP
-        tiles = (16,) if tokens <= 16 else (32,) if tokens <= 32 else (32, 64) if tokens <= 64 else (32, 64, 128) if tokens <= 96 else (64, 128)
-        ways = [(_few_us(tokens, rows, slices, gated, bn, parts, sms), bn, parts) for bn in tiles if tokens <= MOST_TILES * bn for parts in (1, 2, 3, 4, 6, 8) if parts <= slices]
+        tiles = (16,) if tokens <= 16 else (32,) if tokens <= 32 else (32, 64) if tokens <= 64 else (32, 64, 96) if tokens <= 96 else (64, 128)
+        # a part's slices go in as many runs as there are accumulators for: where more parts can make them so, no longer ones than RUN_SLICES in
+        # front of a rounding to 8 bits, and of four times as many else (50 leave 2.7e-7; 512 tokens, 18,944 x 3,584 49.6 us, and 61.5 with 32 at most)
+        run = RUN_SLICES if gated else 4 * RUN_SLICES
+        ways = [(_few_us(tokens, rows, slices, gated, bn, parts, sms), bn, parts) for bn in tiles if tokens <= MOST_TILES * bn for parts in (1, 2, 3, 4, 6, 8)
+                if parts <= slices and (parts == 8 or -(-slices // parts) <= run * MOST_RUNS[bn])]
         if tokens > 64:
-            ways.append((_pair_us(tokens, rows, slices, sms), 256, 1))
+            ways.append((_pair_us(tokens, rows, slices, gated, sms), 256, 1))
         if len(_plans) >= 4096:
             _plans.clear()
         found = _plans[key] = min(ways)[1:]

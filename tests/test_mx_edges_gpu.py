@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+import plain_mx as plain
 from alofa_b200 import mx
 from alofa_b200.csrc.build import load_library
 from test_mx_gpu import host, product_operands, sum_bound
@@ -81,3 +82,65 @@ def test_a_gate_far_below_zero(gate, t, how):
     step = unit * np.exp2(np.maximum(np.frexp(np.maximum(np.abs(got), np.abs(want)) / unit)[1] - 1, -6) - 3.0)
     off = np.abs(got - want) - step / 2 - 2.0**-18 * np.abs(want)
     assert (off <= 0).all(), [(float(g[32 * i]), got[0, 32 * i], want[32 * i]) for i in range(len(FAR)) if (off[:, 32 * i] > 0).any()]
+
+
+# ---- sums of deep products -----------------------------------------------------------------------------------------------
+
+
+def deep_operands(t, n, k, seed):
+    """Rows and weights in their codes as a model has them: most of a block's numbers well below its largest, scales over a range of 2^14."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kp = mx.padded(k)
+    x = (120 * torch.randn(t, kp, generator=g, device="cuda")).clamp(-448, 448)
+    x[:, k:] = 0
+    xs = torch.randint(117, 121, (t, kp // 32), generator=g, device="cuda").to(torch.uint8)
+    wc = torch.randint(0, 256, (n, kp // 2), generator=g, device="cuda").to(torch.uint8)
+    ws = (120 + 1.5 * torch.randn(n, kp // 32, generator=g, device="cuda")).round().clamp(112, 126).to(torch.uint8)
+    return mx.MxRows(x.to(torch.float8_e4m3fn).view(torch.uint8), xs, k), wc, ws
+
+
+@pytest.mark.parametrize("k,how", [(k, how) for k, hows in {3584: [None, (16, 1), (32, 1), (64, 2), (96, 1), (128, 2), (256, 1)], 8960: [None, (16, 2), (64, 3), (96, 4), (256, 1)], 18944: [None, (16, 1), (16, 8), (32, 2), (64, 4), (128, 8), (256, 1)]}.items()
+                                  for how in hows])
+def test_deep_sums_are_as_exact_as_rounded_ones(k, how):
+    """The tensor cores' additions cut off towards zero.  Measured on one accumulator over such operands, that takes 3.95e-9 off every
+    sum for each slice of 128 (0.55e-7 over 14, 1.1e-7 over 28; 5.2e-9 each over 148), and the rest of what sums are off by is 1.1e-7 of them over 28
+    slices and 5.5e-7 over 148; scalar additions leave no common share and 0.7e-7 at depth 3,584, 1.8e-7 at 18,944.  In runs the common share is
+    that of the longest run (of 16, or 32 for prompts, or what eight parts leave), and the rest no more than that of sums which round: half as much again is allowed on each."""
+    t, n = (300, 512) if how in (None, (256, 1), (128, 8), (128, 2)) else (60, 512)
+    x, wc, ws = deep_operands(t, n, k, 90)
+    w = mx.MxWeight.from_codes(wc, ws, k)
+    want = x.dequantize(F32).double() @ w.dequantize(F32).double().T
+    off = mx.linear(x, w, dtype=F32, how=how).double() - want
+    share = float((off * want).sum() / (want * want).sum())
+    slices, (bn, parts) = -(-k // 128), how or mx.plan(t, n, k)
+    part = -(-slices // parts)
+    runs = -(-part // 32) if bn == 256 else min(-(-part // 16), mx.MOST_RUNS[bn])
+    assert abs(share) <= 1.5 * 3.95e-9 * -(-part // runs) and float((off - share * want).norm() / want.norm()) <= 1.5 * 1.8e-7, (share, float(off.norm() / want.norm()))
+
+
+@pytest.mark.parametrize("t,n,k,parts", [(70, 200, 1100, 1), (96, 128, 3000, 3), (200, 515, 1000, 2), (97, 130, 2600, 1), (65, 129, 130, 2)])
+def test_tiles_of_96_tokens(t, n, k, parts):
+    xr, wp, xv, wv = product_operands(t, n, k, 82)
+    want, loose = xv @ wv.T, sum_bound(xv, wv)
+    assert (np.abs(host(mx.linear(xr, wp, dtype=F32, how=(96, parts))) - want) <= loose).all()
+    f = n // 2
+    xr, wp, xv, wv = product_operands(t, 2 * f, k, 83, gated=True)
+    g, u = xv @ wv[:f].T, xv @ wv[f:].T
+    want, slope = plain.silu(g) * u, 1.1 * np.abs(u) * sum_bound(xv, wv[:f]) + (np.abs(g) + 1) * sum_bound(xv, wv[f:])
+    rows = mx.gated_linear(xr, wp, how=(96, parts))
+    largest = np.abs(np.pad(want, ((0, 0), (0, -f % 32)))).reshape(t, -1, 32).max(-1).repeat(32, -1)[:, :f]
+    # half a step of E4M3: 2^-4 of the number, or of the smallest normal number by a scale that is at most 2^-7 of the block's largest
+    assert (np.abs(host(rows.dequantize(F32)).astype(np.float64) - want) <= np.maximum(2.0**-4 * np.abs(want), 2.0**-17 * largest) * (1 + 2.0**-10) + slope).all()
+
+
+@pytest.mark.parametrize("t", [3, 72, 300])
+def test_gated_products_of_several_runs(t):
+    """Depths of two and more runs in a row, tiles behind one another: every accumulator begins anew."""
+    for f, k in ((70, 2200), (9500, 2304), (40, 9000)):
+        xr, wp, xv, wv = product_operands(t, 2 * f, k, 84, gated=True)
+        g, u = xv @ wv[:f].T, xv @ wv[f:].T
+        want, slope = plain.silu(g) * u, 1.1 * np.abs(u) * sum_bound(xv, wv[:f]) + (np.abs(g) + 1) * sum_bound(xv, wv[f:])
+        largest = np.abs(np.pad(want, ((0, 0), (0, -f % 32)))).reshape(t, -1, 32).max(-1).repeat(32, -1)[:, :f]
+        for how in (None, (256, 1)):
+            rows = mx.gated_linear(xr, wp, how=how)
+            assert (np.abs(host(rows.dequantize(F32)).astype(np.float64) - want) <= np.maximum(2.0**-4 * np.abs(want), 2.0**-17 * largest) * (1 + 2.0**-10) + slope).all()
