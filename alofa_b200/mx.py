@@ -127,6 +127,9 @@ class MxRows:
         self.scales_at = self.codes_at + rows * kp
         return self
 
+    def __reduce__(self):  # a copy knows where its own memory is
+        return MxRows, (self.codes, self.scales, self.width)
+
     @property
     def shape(self) -> tuple:
         return self.rows, self.width
@@ -211,6 +214,12 @@ class MxWeight:
         ops.mx_launched(_lib.alofa_mx_settle(_stream(here)), 1, "mx weight", str)
         return w
 
+    def __copy__(self) -> "MxWeight":
+        return self  # constant
+
+    def __reduce__(self):  # a copy knows where its own memory is
+        return _weight_of_tiles, (self.tiles, self.n, self.k, self.gated)
+
     def first_rows(self, n: int) -> "MxWeight":
         """The weight's first ``n`` rows, in the same memory."""
         if self.gated or not 0 < n <= self.n:
@@ -229,6 +238,14 @@ class MxWeight:
         rc = _lib.alofa_mx_weight_values(out.data_ptr(), self.at, self.n, self.k, self.gated, dtype is _BF16, _stream(here))
         ops.mx_launched(rc, 1, "mx weight's values", lambda: f"rows={self.n} depth={self.k}")
         return out
+
+
+def _weight_of_tiles(tiles, n: int, k: int, gated: bool) -> MxWeight:
+    here = _here()
+    w = MxWeight(n, k, gated, here)
+    w.tiles.copy_(tiles)
+    ops.mx_launched(_lib.alofa_mx_settle(_stream(here)), 1, "mx weight", str)  # as in from_codes
+    return w
 
 
 def pack_weight(w: torch.Tensor, gated: bool = False) -> MxWeight:

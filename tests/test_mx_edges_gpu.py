@@ -1,5 +1,7 @@
 """Microscaled operators at their edges on the GPU: what a product does whose waits run out."""
+import copy
 import ctypes
+import pickle
 
 import numpy as np
 import pytest
@@ -144,3 +146,22 @@ def test_gated_products_of_several_runs(t):
         for how in (None, (256, 1)):
             rows = mx.gated_linear(xr, wp, how=how)
             assert (np.abs(host(rows.dequantize(F32)).astype(np.float64) - want) <= np.maximum(2.0**-4 * np.abs(want), 2.0**-17 * largest) * (1 + 2.0**-10) + slope).all()
+
+
+# ---- copies --------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_a_copied_weight_has_its_own_memory(gated):
+    xr, wp, _, _ = product_operands(5, 300, 500, 85, gated)
+    product = (lambda w: mx.gated_linear(xr, w).dequantize()) if gated else (lambda w: mx.linear(xr, w))
+    want, made = product(wp), copy.deepcopy({"w": wp, "same": wp})
+    again, part = pickle.loads(pickle.dumps(wp)), None if gated else copy.deepcopy(wp.first_rows(140))
+    assert made["w"] is made["same"] and copy.copy(wp) is wp
+    for w in (made["w"], again):
+        assert w.at == w.tiles.data_ptr() != wp.at and w.maps_at == ctypes.addressof(w.maps) != wp.maps_at and torch.equal(w.tiles, wp.tiles)
+    wp.tiles.zero_()
+    torch.cuda.synchronize()
+    assert torch.equal(product(made["w"]), want) and torch.equal(product(again), want)
+    if part is not None:
+        assert torch.equal(product(part), want[:, :140].contiguous())
