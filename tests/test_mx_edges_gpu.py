@@ -165,3 +165,51 @@ def test_a_copied_weight_has_its_own_memory(gated):
     assert torch.equal(product(made["w"]), want) and torch.equal(product(again), want)
     if part is not None:
         assert torch.equal(product(part), want[:, :140].contiguous())
+
+
+# ---- a weight made on another stream ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_weight_packed_on_another_stream(recorded):
+    """Products read their weight ahead of the kernel before them in their own stream, but not ahead of a wait for the stream
+    that packed it.  The weights take one another's memory, so that a product that came too early would see the last one's."""
+    w = [torch.randn(1152, 896, device="cuda") * 0.05 for _ in range(3)]
+    x = mx.quantize_rows(torch.randn(8, 896, device="cuda"))
+    want = [mx.linear(x, mx.pack_weight(v)).clone() for v in w]
+    src = w[0].clone()
+    packer, user = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def once():
+        main = torch.cuda.current_stream()
+        packer.wait_stream(main)
+        user.wait_stream(main)
+        with torch.cuda.stream(packer):
+            for _ in range(3):
+                v = src * 1.0  # something before it, so that it is late
+            packed = mx.pack_weight(v)
+        with torch.cuda.stream(user):
+            before = mx.linear(x, other)  # the kernel before it, whose last CTAs are far from done when it lets the next one begin
+            user.wait_stream(packer)
+            out = mx.linear(x, packed)
+        main.wait_stream(user)
+        packed.tiles.record_stream(user)
+        return out, before
+
+    other = mx.pack_weight(w[2])
+    torch.cuda.synchronize()
+    if recorded:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            once()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, before = once()
+    for i in (1, 0, 2, 1, 1, 0) * 10:
+        src.copy_(w[i])
+        if recorded:
+            graph.replay()
+        else:
+            out, before = once()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i]) and torch.equal(before, want[2])
