@@ -155,7 +155,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // through memory, nothing is launched to add them, and the last step is spread over as many SMs as the first.
 //
 // In a graph, weights from memory: 0.5B's q, k and v 3.2 us for one token; 7B's 5.5 for one and 8.8 for 128; 7B's
-// down projection for eight 10.4 (its 36 MB take 5.6), gate and up for one 15.9 (72 MB, 11.0).  Small products are a
+// down projection for eight 10.6 (its 36 MB take 5.6), gate and up for one 13.9 (72 MB, 11.0).  Small products are a
 // launch, a cluster's start and two trips to memory one after the other; large ones two CTAs an SM whose rings hold 200 KB.
 // ---------------------------------------------------------------------------
 constexpr int FEW_THREADS = 192;  // warp 0 weights, 4 tokens, 5 products; then warps 0-3 read the sums and all write rows
@@ -456,9 +456,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
 // the first one's barrier, and the tokens' scales, which no copy of the tensor kind can fetch (rows of 4 bytes a slice),
 // come eight slices at a time, ahead of the ring, by loads of a warp of their own.
 //
-// 7B's gate and up projections, 2,048 tokens 205 us: 2.7 PFLOP/s, the tensor cores busy 68 % of the time at a clock that
-// the power cap holds to 1.6 to 1.8 GHz; q, k and v 30.2 us (144 tiles on 74 pairs, the second round of two nearly
-// full), the down projection 117 (112 tiles: a quarter of the pairs idle in the second round).
+// In a graph, 7B's gate and up projections, 2,048 tokens 249 us: 2.2 PFLOP/s, the tensor cores busy 65 to 69 % of the time at a clock
+// that the power cap holds to 1.6 to 1.8 GHz; q, k and v 30.2 us (144 tiles on 74 pairs, two rounds, each with a beginning and an end;
+// 46 to 51 % busy), the down projection 122 (112 tiles: half of the pairs idle in the second round).  A slice takes 560 to 590 clocks, 800 while
+// the epilogue of the tile before it runs.
 // ---------------------------------------------------------------------------
 constexpr int PAIR_THREADS = 384;  // warp 0 weights, 1 tokens, 2 products (first CTA), 3 the tokens' scales, 4-11 epilogue
 constexpr int PAIR_STAGES = 6;
