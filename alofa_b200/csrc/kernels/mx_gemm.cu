@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) mx_few_kernel(const __grid_con
   const int runs = min((n + RUN_SLICES - 1) / RUN_SLICES, Tile::MOST_RUNS);  // of slices, each with sums of its own
   const uint32_t need = (uint32_t)(runs * BN + Tile::SCALE_COLS), tmem_cols = need <= 64 ? 64 : need <= 128 ? 128 : 256;
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    abort_flag = asked[0] = asked[1] = 0;
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&landed[s], BY_WEIGHTS + BY_TOKENS);
       mbar_init(&stage_free[s], 1);
