@@ -364,7 +364,7 @@ def plan(tokens: int, rows: int, depth: int, gated: bool = False, here: Optional
     current one); 256 tokens: pairs of CTAs.
 
     The kernel for a few tokens has tiles of up to 32 of them in steps of as many,
-    of 32 or 64 in larger ones; its depth goes in as many parts as make it
+    of 32, 64 or 96 (128 beyond) in larger ones; its depth goes in as many parts as make it
     shortest (us, depth x rows): 1 token, 18,944 x 3,584 in 8 parts 10.4, in 4
     12.8; 64 tokens, 896 x 9,728 gated in tiles of 32 8.1 and of 64 8.4.  Beyond 64
     tokens it is weighed against pairs, which take long to begin and then do a
